@@ -26,6 +26,8 @@
  *                        the serve tier calls it (kv_cache.rs:199-209,
  *                        :341-351), agc.rs OdeAgc
  *   wb_layer_norm     <- src/common/model.rs:154 layer_norm
+ *   wb_gqa_*           (no counterpart: grouped-head dot-product attention
+ *                        with a paged 16- or 8-bit cache)
  *   wb_embed, wb_residual_add, wb_phase_native_decode, wb_lm_head
  *                     <- the rest of kv_cache.rs prefill / forward_one
  *                        (:106-113, :220, :18-33, :365-378)
@@ -34,8 +36,8 @@
  *   - Every function returns int status: WB_OK (0) or a negative WB_E*.
  *     No exceptions cross the ABI; nothing aborts or traps.  The message of
  *     the last failure on the calling thread is returned by wb_last_error().
- *   - All floating point data is fp32, row-major, in the reference's
- *     layouts (a Rust Vec<Vec<f32>> [rows][cols] flattened row by row).
+ *   - All floating point data (but that of wb_gqa_*) is fp32, row-major, in
+ *     the reference's layouts (a Rust Vec<Vec<f32>> [rows][cols] flattened row by row).
  *   - Data pointers may be host or device memory; the library detects which
  *     (cudaPointerGetAttributes).  Host inputs are copied into the
  *     context's device staging buffer with cudaMemcpyAsync (pinned host
@@ -431,6 +433,92 @@ WB_API int wb_phase_native_decode(wb_context *ctx, const float *hidden, int n_ro
                                   const float *corrector, const float *wte, int vocab, int flags, float *logits);
 WB_API int wb_lm_head(wb_context *ctx, const float *hidden, int n_rows, int n_embd, const float *lm_head, int vocab,
                       int flags, float *logits);
+
+/* ---- grouped-head dot-product attention in 16 bits --------------------- */
+/* Serving form of the dot-product attention (compute.rs:357-414) for models
+ * whose query heads share key-value heads: query head h reads key-value head
+ * h / (n_head / n_kv_head).  No counterpart in the reference, which has
+ * whole fp32 layer calls and no cache for this attention.  The projections
+ * around it stay with the caller.  Data pointers here are DEVICE memory;
+ * index arrays (cu_*, slots, start) may be host memory, which is checked in
+ * full before anything is queued, or device memory, which the host does not
+ * read (no synchronisation; can be captured in a CUDA graph): the kernels
+ * then skip what lies outside the buffers and set bit 0x8 (bounds) of the
+ * device error word. */
+/* element types */
+#define WB_BF16 0
+#define WB_F16 1
+#define WB_INT8 2
+#define WB_E4M3 3
+
+/* Attention over whole prompts, sequences of different lengths packed one
+ * after another: sequence b's queries are rows cu_q[b] .. cu_q[b+1]-1 of q
+ * and its keys rows cu_k[b] .. cu_k[b+1]-1 of k and v.
+ *   out = softmax(scale q k^T) v over the sequence's keys; causal: query i
+ *   of n_q sees keys j <= i + (n_k - n_q), so queries that continue a cached
+ *   prefix are given with all keys of the sequence.
+ *   lse = log sum exp of the visible scaled scores.
+ * A query that sees no key gives out 0 and lse -inf.  Values of keys that a
+ * query does not see never reach it, not even as infinities or NaN.
+ * Scores, softmax statistics and the output sums are fp32; the
+ * unnormalised probabilities are rounded to dtype for the product with v. */
+typedef struct {
+    int32_t dtype;                 /* WB_BF16 or WB_F16: q, k, v, out */
+    int32_t n_head, n_kv_head;     /* n_head a multiple of n_kv_head, at most 128 times it */
+    int32_t head_dim;              /* 1 .. 128 */
+    int32_t n_seq;
+    int32_t causal;
+    float scale;
+    int64_t total_q, total_k;      /* rows of q / of k and v */
+    const void *q, *k, *v;         /* element (token, head, d) at token*ts + head*hs + d, strides in elements */
+    int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+    const int32_t *cu_q, *cu_k;    /* [n_seq + 1]; cu_k NULL: the same as cu_q */
+    void *out;
+    int64_t o_ts, o_hs;
+    float *lse;                    /* NULL or [n_head][total_q] */
+} wb_gqa_attn_desc;
+WB_API int wb_gqa_attention(wb_context *ctx, const wb_gqa_attn_desc *d);
+
+/* One layer of a paged key-value cache in the caller's memory.  Position p
+ * of slot s is row p % WB_KV_PAGE of page table[s][p / WB_KV_PAGE].  A
+ * row is head_dim values padded with zeros to the next multiple of 16.
+ * store: WB_BF16 / WB_F16 (the rows as given; store = dtype) or WB_INT8 /
+ * WB_E4M3: per (position, head) scale = max(max|x| * (1 / top), 2^-126), top =
+ * 127 or 448, and value = x / scale rounded to the nearest representable
+ * (ties to even), in fp32; a row with an infinity or NaN reads back as NaN throughout. */
+typedef struct {
+    int32_t dtype;                 /* WB_BF16 or WB_F16: rows and queries */
+    int32_t store;                 /* dtype, WB_INT8 or WB_E4M3 */
+    int32_t n_kv_head, head_dim;   /* head_dim 1 .. 128 */
+    int32_t n_pages, n_slots, max_pages;
+    void *k_pages, *v_pages;       /* [n_pages][n_kv_head][WB_KV_PAGE][row], 16-byte aligned */
+    float *k_scale, *v_scale;      /* [n_pages][n_kv_head][WB_KV_PAGE], 16-byte aligned; 8-bit stores only */
+    const int32_t *table;          /* [n_slots][max_pages] page ids, -1 unmapped */
+    int32_t *lens;                 /* [n_slots] positions held */
+} wb_gqa_cache_desc;
+
+/* Store packed rows: sequence i's rows cu[i] .. cu[i+1]-1 of k and v
+ * (strides as above) become positions start[i], start[i] + 1, ... of slot
+ * slots[i], and lens[slots[i]] the position after the last.  cu NULL: one
+ * row per sequence; start NULL: append (start = lens); slots NULL: 0, 1, ...
+ * total: rows of k and v (cu's last entry).  A slot may appear once. */
+WB_API int wb_gqa_cache_write(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq,
+                              const int32_t *cu, int64_t total, const int32_t *start, const void *k, int64_t k_ts,
+                              int64_t k_hs, const void *v, int64_t v_ts, int64_t v_hs);
+/* Read positions back, in the layout of the write: k, v [total][n_kv_head]
+ * [head_dim] contiguous, of dtype (an 8-bit row as value * scale, rounded
+ * once).  start NULL: from position 0.  Positions outside the table's pages
+ * read 0. */
+WB_API int wb_gqa_cache_read(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq,
+                             const int32_t *cu, int64_t total, const int32_t *start, void *k, void *v);
+/* Attention of one new token per sequence over positions 0 .. lens-1 of its
+ * slot (the token's own key and value among them: write it first).  q
+ * element (sequence, head, d) at sequence*q_ss + head*q_hs + d; out [n_seq]
+ * [n_head][head_dim] contiguous, lse NULL or [n_seq][n_head].  An empty slot
+ * gives 0 and -inf; positions before the length whose page is unmapped are
+ * left out and flagged. */
+WB_API int wb_gqa_decode(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq, int n_head,
+                         const void *q, int64_t q_ss, int64_t q_hs, float scale, void *out, float *lse);
 
 #ifdef __cplusplus
 }

@@ -24,6 +24,12 @@ WB_PATH_EXACT = 0x1
 WB_NO_CONTENT = 0x2
 WB_RETURN_PATHWAY = 0x4
 
+# element types of the grouped-head attention (wb_gqa_*)
+WB_BF16 = 0
+WB_F16 = 1
+WB_INT8 = 2
+WB_E4M3 = 3
+
 _F = C.POINTER(C.c_float)
 _VP = C.c_void_p
 
@@ -73,6 +79,11 @@ SIGNATURES = {
     "wb_embed": (C.c_int, [_VP, _VP, _VP, C.c_int, _VP, C.c_int, _VP, C.c_int, C.c_int, _VP]),
     "wb_phase_native_decode": (C.c_int, [_VP, _VP, C.c_int, C.c_int, _VP, _VP, C.c_int, C.c_int, _VP]),
     "wb_lm_head": (C.c_int, [_VP, _VP, C.c_int, C.c_int, _VP, C.c_int, C.c_int, _VP]),
+    "wb_gqa_attention": (C.c_int, [_VP, _VP]),
+    "wb_gqa_cache_write": (C.c_int, [_VP, _VP, _VP, C.c_int, _VP, C.c_int64, _VP, _VP, C.c_int64, C.c_int64, _VP,
+                                     C.c_int64, C.c_int64]),
+    "wb_gqa_cache_read": (C.c_int, [_VP, _VP, _VP, C.c_int, _VP, C.c_int64, _VP, _VP, _VP]),
+    "wb_gqa_decode": (C.c_int, [_VP, _VP, _VP, C.c_int, C.c_int, _VP, C.c_int64, C.c_int64, C.c_float, _VP, _VP]),
     # include/wave_b200_testing.h
     "wb_test_gemm_bf16": (C.c_int, [_VP, _VP, _VP, _VP, _VP, C.c_int, C.c_int, C.c_int]),
     "wb_test_gemm_tf32": (C.c_int, [_VP, _VP, _VP, _VP, _VP, C.c_int, C.c_int, C.c_int]),
@@ -111,6 +122,22 @@ class FfnWeightsDesc(C.Structure):
                 ("mo_squeeze_w", _VP), ("mo_squeeze_b", _VP), ("mo_process_w", _VP), ("mo_process_b", _VP),
                 ("gamma_raw", _VP), ("omega", _VP), ("alpha", C.c_float), ("beta", C.c_float),
                 ("phase_correction", _VP), ("rk4_weights", _VP), ("out_w", _VP), ("out_b", _VP)]
+
+
+class GqaAttnDesc(C.Structure):
+    """wb_gqa_attn_desc (include/wave_b200.h)."""
+    _fields_ = [("dtype", C.c_int32), ("n_head", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32),
+                ("n_seq", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float), ("total_q", C.c_int64),
+                ("total_k", C.c_int64), ("q", _VP), ("k", _VP), ("v", _VP), ("q_ts", C.c_int64), ("q_hs", C.c_int64),
+                ("k_ts", C.c_int64), ("k_hs", C.c_int64), ("v_ts", C.c_int64), ("v_hs", C.c_int64), ("cu_q", _VP),
+                ("cu_k", _VP), ("out", _VP), ("o_ts", C.c_int64), ("o_hs", C.c_int64), ("lse", _VP)]
+
+
+class GqaCacheDesc(C.Structure):
+    """wb_gqa_cache_desc (include/wave_b200.h)."""
+    _fields_ = [("dtype", C.c_int32), ("store", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32),
+                ("n_pages", C.c_int32), ("n_slots", C.c_int32), ("max_pages", C.c_int32), ("k_pages", _VP),
+                ("v_pages", _VP), ("k_scale", _VP), ("v_scale", _VP), ("table", _VP), ("lens", _VP)]
 
 
 class WaveB200Error(RuntimeError):

@@ -6,12 +6,14 @@
 #include "wb_tc.h"
 #include "wb_bwd.h"
 #include "wb_decode.h"
+#include "wb_gqa.h"
 #include "wb_serve.h"
 
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <map>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -119,6 +121,11 @@ struct wb_context {
     // host-buffer pipelines: copies up, copies down, and their events
     cudaStream_t cp_in = nullptr, cp_out = nullptr;
     std::vector<cudaEvent_t> ev;
+    // wb_gqa_* scratch, one per stream (calls on different streams never
+    // share one), and the buffers that growth replaced (a captured graph may
+    // still name them)
+    std::map<cudaStream_t, DevBuf> gqa_ws;
+    std::vector<void *> gqa_old;
 };
 
 // Creates ctx's copy streams and at least n events on first need.
@@ -380,6 +387,9 @@ int wb_context_destroy(wb_context *ctx) {
         cudaStreamDestroy(ctx->cp_out);
     }
     for (cudaEvent_t e : ctx->ev) cudaEventDestroy(e);
+    for (auto &w : ctx->gqa_ws)
+        if (w.second.p) cudaFree(w.second.p);
+    for (void *p : ctx->gqa_old) cudaFree(p);
     if (ctx->own) cudaStreamDestroy(ctx->own);
     wb::prof_destroy(ctx->prof);
     delete ctx;
@@ -1857,3 +1867,292 @@ extern "C" int wb_kv_decode_noalloc(wb_context *ctx, wb_kv_cache *c, int layer_i
     c->len_stale = true;
     return WB_OK;
 }
+
+// ---------------------------------------------------------------------------
+// Grouped-head dot-product attention in 16 bits (wb_gqa_*)
+// ---------------------------------------------------------------------------
+namespace {
+
+// No C++ exception (an allocation on the host) leaves a C entry.
+template <class F>
+int guarded(F &&f) {
+    try {
+        return f();
+    } catch (...) {
+        try {
+            return fail(WB_ENOMEM, "out of host memory");
+        } catch (...) {
+            return WB_ENOMEM;
+        }
+    }
+}
+
+// At least `bytes` of the context's scratch for its current stream.  Growing
+// keeps the replaced buffer until the context ends (kernels in flight and
+// captured graphs may name it) and doubles, so the kept ones sum to less than
+// the live one.  A new buffer is zeroed before first use, also during a
+// stream capture (where nothing may run on the captured stream itself).
+int gqa_workspace(wb_context *ctx, size_t bytes, DevBuf **out) {
+    DevBuf &w = ctx->gqa_ws[ctx->stream];
+    *out = &w;
+    if (bytes <= w.n) return WB_OK;
+    const size_t want = std::max(bytes, 2 * w.n);
+    if (w.p) ctx->gqa_old.push_back(w.p);
+    w = DevBuf{};
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    void *p = nullptr;
+    cudaError_t e = cudaMalloc(&p, want);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, want, ctx->own);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->own);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        if (p) ctx->gqa_old.push_back(p);
+        return fail(p ? WB_ECUDA : WB_ENOMEM, "scratch of " + std::to_string(want) + " bytes: " + cudaGetErrorString(e));
+    }
+    w.p = p;
+    w.n = want;
+    return WB_OK;
+}
+
+// Index arrays of one call: device ones are used in place, host ones go into
+// one upload into the front of the call's scratch.
+struct IndexArgs {
+    struct One {
+        const int32_t *src;
+        int n;
+        const int32_t **dst;
+    };
+    std::vector<One> host;
+    size_t ints = 0;
+    // *dst becomes the device address; host arrays only at upload()
+    bool add(const int32_t *p, int n, const int32_t **dst) {  // true: p is host memory
+        *dst = p;
+        if (!p || is_device_ptr(p)) return false;
+        host.push_back({p, n, dst});
+        ints += ((size_t)n + 63) & ~size_t(63);
+        return true;
+    }
+    size_t bytes() const { return ints * sizeof(int32_t); }
+    int upload(void *at, cudaStream_t st) {
+        if (host.empty()) return WB_OK;
+        std::vector<int32_t> all(ints, 0);
+        size_t off = 0;
+        for (const One &o : host) {
+            std::copy(o.src, o.src + o.n, all.begin() + off);
+            *o.dst = (const int32_t *)at + off;
+            off += ((size_t)o.n + 63) & ~size_t(63);
+        }
+        // pageable: the driver has taken the bytes when the call returns
+        WB_CUDA(cudaMemcpyAsync(at, all.data(), ints * sizeof(int32_t), cudaMemcpyHostToDevice, st));
+        return WB_OK;
+    }
+};
+
+// Host copies of an index array that ascends from 0 to total.
+int check_starts(const int32_t *cu, int n_seq, int64_t total, const char *name) {
+    if (cu[0] != 0) return fail(WB_EINVAL, std::string(name) + "[0] is not 0");
+    for (int i = 0; i < n_seq; i++)
+        if (cu[i + 1] < cu[i]) return fail(WB_EINVAL, std::string(name) + " descends");
+    if (cu[n_seq] != total) return fail(WB_EINVAL, std::string(name) + "'s last entry is not the number of rows");
+    return WB_OK;
+}
+
+bool good_strides(int64_t a, int64_t b) {
+    return a >= 0 && b >= 0 && a < ((int64_t)1 << 40) && b < ((int64_t)1 << 40);
+}
+
+bool all_device(std::initializer_list<const void *> ps) {
+    for (const void *p : ps)
+        if (!is_device_ptr(p)) return false;
+    return true;
+}
+
+int gqa_cache_checks(wb_context *ctx, const wb_gqa_cache_desc *c, int n_seq, bool need_lens, wb::GqaCacheArgs *out) {
+    if (!ctx || !c) return fail(WB_EINVAL, "NULL argument");
+    if (c->dtype != WB_BF16 && c->dtype != WB_F16) return fail(WB_EINVAL, "dtype must be WB_BF16 or WB_F16");
+    if (c->store != c->dtype && c->store != WB_INT8 && c->store != WB_E4M3)
+        return fail(WB_EINVAL, "store must be dtype, WB_INT8 or WB_E4M3");
+    if (c->n_kv_head < 1 || c->n_kv_head > 4096) return fail(WB_EINVAL, "n_kv_head out of range");
+    if (c->head_dim < 1 || c->head_dim > wb::GQA_MAX_HD) return fail(WB_EINVAL, "head_dim must be 1 .. 128");
+    if (c->n_pages < 1 || c->n_slots < 1 || c->max_pages < 1 || c->max_pages > (1 << 23))
+        return fail(WB_EINVAL, "bad cache dimensions");
+    if (n_seq < 0 || n_seq > c->n_slots) return fail(WB_EINVAL, "n_seq out of range for the cache");
+    const bool quant = c->store == WB_INT8 || c->store == WB_E4M3;
+    if (!c->k_pages || !c->v_pages || !c->table || (need_lens && !c->lens) ||
+        (quant && (!c->k_scale || !c->v_scale)))
+        return fail(WB_EINVAL, "NULL cache array");
+    for (const void *p : {(const void *)c->k_pages, (const void *)c->v_pages, (const void *)c->k_scale,
+                          (const void *)c->v_scale})
+        if (p && reinterpret_cast<uintptr_t>(p) % 16)
+            return fail(WB_EINVAL, "pages and scales must be 16-byte aligned");
+    if (!all_device({c->k_pages, c->v_pages, c->table}) || (need_lens && !is_device_ptr(c->lens)) ||
+        (quant && !all_device({c->k_scale, c->v_scale})))
+        return fail(WB_EINVAL, "cache arrays must be device memory");
+    *out = wb::GqaCacheArgs{c->k_pages, c->v_pages, quant ? c->k_scale : nullptr, quant ? c->v_scale : nullptr,
+                            c->table, c->lens, nullptr, c->store, c->n_kv_head, c->head_dim,
+                            wb::gqa_row(c->head_dim), c->n_pages, c->n_slots, c->max_pages, n_seq, ctx->dev_err};
+    return WB_OK;
+}
+
+int check_slots(const int32_t *slots, int n_seq, int n_slots) {
+    std::vector<char> seen(n_slots, 0);
+    for (int i = 0; i < n_seq; i++) {
+        if (slots[i] < 0 || slots[i] >= n_slots) return fail(WB_EINVAL, "slot out of range");
+        if (seen[slots[i]]++) return fail(WB_EINVAL, "duplicate slot");
+    }
+    return WB_OK;
+}
+
+// What the write and the read share: their index arrays.
+int gqa_move_indexes(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq, const int32_t *cu,
+                     int64_t total, const int32_t *start, wb::GqaCacheArgs *ca, const int32_t **cu_d,
+                     const int32_t **start_d) {
+    if (total < 0 || total > 0x7fffffff) return fail(WB_EINVAL, "total out of range");
+    if (!cu && total != n_seq) return fail(WB_EINVAL, "without cu there is one row per sequence");
+    IndexArgs ix;
+    const bool cu_h = ix.add(cu, n_seq + 1, cu_d);
+    if (cu_h) WB_TRY(check_starts(cu, n_seq, total, "cu"));
+    if (ix.add(slots, n_seq, &ca->slots)) WB_TRY(check_slots(slots, n_seq, c->n_slots));
+    if (ix.add(start, n_seq, start_d))
+        for (int i = 0; i < n_seq; i++) {
+            const int64_t n = !cu ? 1 : cu_h ? cu[i + 1] - cu[i] : 0;
+            if (start[i] < 0 || start[i] + n > (int64_t)c->max_pages * WB_PAGE)
+                return fail(WB_EINVAL, "positions outside the slot's table");
+        }
+    if (ix.bytes()) {
+        DevBuf *w;
+        WB_TRY(gqa_workspace(ctx, wb::GQA_WS_HEAD + ix.bytes(), &w));
+        WB_TRY(ix.upload((char *)w->p + wb::GQA_WS_HEAD, ctx->stream));
+    }
+    return WB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int wb_gqa_attention(wb_context *ctx, const wb_gqa_attn_desc *d) {
+    return guarded([&]() -> int {
+        if (!ctx || !d) return fail(WB_EINVAL, "NULL argument");
+        if (d->dtype != WB_BF16 && d->dtype != WB_F16) return fail(WB_EINVAL, "dtype must be WB_BF16 or WB_F16");
+        if (d->n_head < 1 || d->n_kv_head < 1 || d->n_head % d->n_kv_head || d->n_head > 65535)
+            return fail(WB_EINVAL, "n_head must be a multiple of n_kv_head");
+        if (d->n_head / d->n_kv_head > wb::GQA_MAX_GROUP)
+            return fail(WB_EINVAL, "more than 128 query heads on one key-value head");
+        if (d->head_dim < 1 || d->head_dim > wb::GQA_MAX_HD) return fail(WB_EINVAL, "head_dim must be 1 .. 128");
+        if (d->n_seq < 0 || d->total_q < 0 || d->total_k < 0 || d->total_q > 0x7fffffff || d->total_k > 0x7fffffff)
+            return fail(WB_EINVAL, "n_seq or a number of rows out of range");
+        if (!std::isfinite(d->scale)) return fail(WB_EINVAL, "scale is not finite");
+        if (!good_strides(d->q_ts, d->q_hs) || !good_strides(d->k_ts, d->k_hs) || !good_strides(d->v_ts, d->v_hs) ||
+            !good_strides(d->o_ts, d->o_hs))
+            return fail(WB_EINVAL, "negative or huge stride");
+        if (d->total_q == 0) return WB_OK;
+        if (d->n_seq == 0) return fail(WB_EINVAL, "rows without a sequence");
+        if (!d->q || !d->out || !d->cu_q || (d->total_k && (!d->k || !d->v))) return fail(WB_EINVAL, "NULL argument");
+        if (!d->cu_k && d->total_k != d->total_q) return fail(WB_EINVAL, "cu_k NULL needs total_k == total_q");
+        DeviceGuard g(ctx->device);
+        if (!g.ok) return fail(WB_ECUDA, "cudaSetDevice failed");
+        if (!all_device({d->q, d->out}) || (d->total_k && !all_device({d->k, d->v})) ||
+            (d->lse && !is_device_ptr(d->lse)))
+            return fail(WB_EINVAL, "q, k, v, out and lse must be device memory");
+        ProfBind pb(ctx);
+        wb::GqaAttnArgs a{d->q, d->k, d->v, d->out, d->lse, d->q_ts, d->q_hs, d->k_ts, d->k_hs, d->v_ts, d->v_hs,
+                          d->o_ts, d->o_hs, nullptr, nullptr, d->total_q, d->total_k, d->n_head, d->n_kv_head,
+                          d->head_dim, d->n_seq, d->causal != 0, d->scale, ctx->dev_err};
+        IndexArgs ix;
+        if (ix.add(d->cu_q, d->n_seq + 1, &a.cu_q)) WB_TRY(check_starts(d->cu_q, d->n_seq, d->total_q, "cu_q"));
+        if (ix.add(d->cu_k, d->n_seq + 1, &a.cu_k)) WB_TRY(check_starts(d->cu_k, d->n_seq, d->total_k, "cu_k"));
+        DevBuf *w;
+        size_t extra = wb::gqa_attention_scratch(a, d->dtype);
+        WB_TRY(gqa_workspace(ctx, wb::GQA_WS_HEAD + ix.bytes() + extra, &w));
+        WB_TRY(ix.upload((char *)w->p + wb::GQA_WS_HEAD, ctx->stream));
+        if (!d->cu_k) a.cu_k = a.cu_q;
+        std::string msg;
+        int rc = wb::launch_gqa_attention(a, d->dtype, (char *)w->p + wb::GQA_WS_HEAD + ix.bytes(), ctx->sm_count,
+                                          ctx->stream, &msg);
+        if (rc != WB_OK) return fail(rc, msg);
+        WB_CUDA(cudaGetLastError());
+        return WB_OK;
+    });
+}
+
+int wb_gqa_cache_write(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq, const int32_t *cu,
+                       int64_t total, const int32_t *start, const void *k, int64_t k_ts, int64_t k_hs, const void *v,
+                       int64_t v_ts, int64_t v_hs) {
+    return guarded([&]() -> int {
+        wb::GqaCacheArgs ca;
+        WB_TRY(gqa_cache_checks(ctx, c, n_seq, true, &ca));
+        if (!good_strides(k_ts, k_hs) || !good_strides(v_ts, v_hs)) return fail(WB_EINVAL, "negative or huge stride");
+        if (n_seq == 0) return total == 0 ? WB_OK : fail(WB_EINVAL, "rows without a sequence");
+        if (total != 0 && (!k || !v)) return fail(WB_EINVAL, "NULL argument");
+        DeviceGuard g(ctx->device);
+        if (!g.ok) return fail(WB_ECUDA, "cudaSetDevice failed");
+        if (total != 0 && !all_device({k, v})) return fail(WB_EINVAL, "k and v must be device memory");
+        ProfBind pb(ctx);
+        const int32_t *cu_d, *start_d;
+        WB_TRY(gqa_move_indexes(ctx, c, slots, n_seq, cu, total, start, &ca, &cu_d, &start_d));
+        std::string msg;
+        int rc = wb::launch_gqa_cache_write(ca, c->dtype, cu_d, total, start_d, k, v, k_ts, k_hs, v_ts, v_hs,
+                                            ctx->stream, &msg);
+        if (rc != WB_OK) return fail(rc, msg);
+        WB_CUDA(cudaGetLastError());
+        return WB_OK;
+    });
+}
+
+int wb_gqa_cache_read(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq, const int32_t *cu,
+                      int64_t total, const int32_t *start, void *k, void *v) {
+    return guarded([&]() -> int {
+        wb::GqaCacheArgs ca;
+        WB_TRY(gqa_cache_checks(ctx, c, n_seq, false, &ca));
+        if (n_seq == 0) return total == 0 ? WB_OK : fail(WB_EINVAL, "rows without a sequence");
+        if (total == 0) return WB_OK;
+        if (!k || !v) return fail(WB_EINVAL, "NULL argument");
+        DeviceGuard g(ctx->device);
+        if (!g.ok) return fail(WB_ECUDA, "cudaSetDevice failed");
+        if (!all_device({k, v})) return fail(WB_EINVAL, "k and v must be device memory");
+        ProfBind pb(ctx);
+        const int32_t *cu_d, *start_d;
+        WB_TRY(gqa_move_indexes(ctx, c, slots, n_seq, cu, total, start, &ca, &cu_d, &start_d));
+        std::string msg;
+        int rc = wb::launch_gqa_cache_read(ca, c->dtype, cu_d, total, start_d, k, v, ctx->stream, &msg);
+        if (rc != WB_OK) return fail(rc, msg);
+        WB_CUDA(cudaGetLastError());
+        return WB_OK;
+    });
+}
+
+int wb_gqa_decode(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq, int n_head,
+                  const void *q, int64_t q_ss, int64_t q_hs, float scale, void *out, float *lse) {
+    return guarded([&]() -> int {
+        wb::GqaCacheArgs ca;
+        WB_TRY(gqa_cache_checks(ctx, c, n_seq, true, &ca));
+        if (n_head < 1 || n_head % c->n_kv_head || n_head > 65535)
+            return fail(WB_EINVAL, "n_head must be a multiple of n_kv_head");
+        if (!good_strides(q_ss, q_hs)) return fail(WB_EINVAL, "negative or huge stride");
+        if (!std::isfinite(scale)) return fail(WB_EINVAL, "scale is not finite");
+        if (n_seq == 0) return WB_OK;
+        if (!q || !out) return fail(WB_EINVAL, "NULL argument");
+        DeviceGuard g(ctx->device);
+        if (!g.ok) return fail(WB_ECUDA, "cudaSetDevice failed");
+        if (!all_device({q, out}) || (lse && !is_device_ptr(lse)))
+            return fail(WB_EINVAL, "q, out and lse must be device memory");
+        ProfBind pb(ctx);
+        IndexArgs ix;
+        if (ix.add(slots, n_seq, &ca.slots)) WB_TRY(check_slots(slots, n_seq, c->n_slots));
+        DevBuf *w;
+        const size_t extra = wb::gqa_decode_scratch(ca, n_head, ctx->sm_count);
+        WB_TRY(gqa_workspace(ctx, wb::GQA_WS_HEAD + ix.bytes() + extra, &w));
+        WB_TRY(ix.upload((char *)w->p + wb::GQA_WS_HEAD, ctx->stream));
+        std::string msg;
+        int rc = wb::launch_gqa_decode(ca, c->dtype, n_head, q, q_ss, q_hs, scale, out, lse, (unsigned int *)w->p,
+                                       (char *)w->p + wb::GQA_WS_HEAD + ix.bytes(), ctx->sm_count, ctx->stream, &msg);
+        if (rc != WB_OK) return fail(rc, msg);
+        WB_CUDA(cudaGetLastError());
+        return WB_OK;
+    });
+}
+
+}  // extern "C"

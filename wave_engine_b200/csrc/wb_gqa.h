@@ -1,0 +1,97 @@
+// wb_gqa.h -- grouped-head dot-product attention in 16 bits: attention over
+// packed prompts, a paged key-value cache of 16- or 8-bit values, and the
+// attention of one new token over it.
+#pragma once
+#include "wave_b200.h"
+#include "wb_internal.h"
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <string>
+
+namespace wb {
+
+static constexpr int GQA_MAX_HD = 128;
+static constexpr int GQA_MAX_GROUP = 128;
+
+// columns of a stored cache row: head_dim up to whole 16s, so that rows of
+// either width are whole 16-byte pieces
+__host__ __device__ inline int gqa_row(int hd) { return (hd + 15) & ~15; }
+
+// Packed prompts (device pointers; strides in elements).
+struct GqaAttnArgs {
+    const void *q, *k, *v;
+    void *out;
+    float *lse;  // nullable, [H][total_q]
+    long long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
+    const int32_t *cu_q, *cu_k;
+    long long total_q, total_k;
+    int H, Hkv, hd, n_seq, causal;
+    float scale;
+    uint32_t *dev_err;
+};
+
+// One layer's paged cache and the sequences of a call (device pointers).
+struct GqaCacheArgs {
+    void *k_pages, *v_pages;
+    float *k_scale, *v_scale;
+    const int32_t *table;
+    int32_t *lens;
+    const int32_t *slots;  // [n_seq], nullptr = 0, 1, ..
+    int store, Hkv, hd, row, n_pages, n_slots, max_pages, n_seq;
+    uint32_t *dev_err;
+};
+
+// A stream's scratch begins with counters that every call finds and leaves
+// zero.
+static constexpr size_t GQA_WS_HEAD = 16384;
+
+// scratch bytes (after the counters and index arrays) of the calls below
+size_t gqa_attention_scratch(const GqaAttnArgs &a, int dtype);
+size_t gqa_decode_scratch(const GqaCacheArgs &c, int H, int sm_count);
+
+int launch_gqa_attention(const GqaAttnArgs &a, int dtype, void *scratch, int sm_count, cudaStream_t st,
+                         std::string *msg);
+// cu: nullptr = one token per sequence; start: nullptr = the slots' lengths
+int launch_gqa_cache_write(const GqaCacheArgs &c, int dtype, const int32_t *cu, long long total, const int32_t *start,
+                           const void *k, const void *v, long long k_ts, long long k_hs, long long v_ts, long long v_hs,
+                           cudaStream_t st, std::string *msg);
+int launch_gqa_cache_read(const GqaCacheArgs &c, int dtype, const int32_t *cu, long long total, const int32_t *start,
+                          void *k, void *v, cudaStream_t st, std::string *msg);
+int launch_gqa_decode(const GqaCacheArgs &c, int dtype, int H, const void *q, long long q_ss, long long q_hs,
+                      float scale, void *out, float *lse, unsigned int *counters, void *scratch, int sm_count,
+                      cudaStream_t st, std::string *msg);
+
+#ifdef __CUDACC__
+// The last sequence b with cu[b] <= t (cu[0] = 0, n sequences).  Empty
+// sequences share their start with the next one and are never found.
+__device__ __forceinline__ int gqa_find_seq(const int32_t *cu, int n, long long t) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cu[mid] <= t) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(int8_t x) { return (float)x; }
+__device__ __forceinline__ float to_f(__nv_fp8_e4m3 x) { return (float)x; }
+template <class T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+// A non-finite quotient (of a non-finite value) stores 0: its scale is not
+// finite either, so the position reads back as NaN.
+template <>
+__device__ __forceinline__ int8_t from_f<int8_t>(float x) { return isfinite(x) ? (int8_t)__float2int_rn(x) : (int8_t)0; }
+template <>
+__device__ __forceinline__ __nv_fp8_e4m3 from_f<__nv_fp8_e4m3>(float x) { return __nv_fp8_e4m3(x); }
+#endif
+
+}  // namespace wb

@@ -1,0 +1,296 @@
+"""Grouped-head dot-product attention in 16 bits, for serving: attention over
+packed prompts, a paged key-value cache (16-bit, or quantised to int8 / e4m3
+as it is written) and the attention of one new token over it.
+
+    out = gqa_attention(q, k, v, cu_q)                       # whole prompts
+    cache = GqaCache(n_layers, n_kv_head, head_dim, max_seqs, max_ctx, n_pages, dtype, store="e4m3")
+    cache.reserve(seq, n); cache.write(layer, k, v, seqs, cu)
+    out = cache.decode(layer, q, seqs)                       # one new token each
+
+Tensors are torch CUDA tensors, bf16 or fp16, used in place on torch's
+current stream; q, k and v may be slices of a fused projection's rows (only
+the last dimension has to be contiguous).  Index arrays (``cu``, ``start``,
+``slots``) are int32 CUDA tensors, which the host does not read, or host
+sequences, which are checked.  The work runs in the CUDA library
+(``wb_gqa_*``, include/wave_b200.h); there is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import _lib
+from .runtime import Context, default_context
+
+try:  # the package imports without torch; these entry points take torch tensors
+    import torch
+    _DTYPES = {torch.bfloat16: _lib.WB_BF16, torch.float16: _lib.WB_F16}
+    _STORES = {**_DTYPES, torch.int8: _lib.WB_INT8, torch.float8_e4m3fn: _lib.WB_E4M3}
+except Exception:  # pragma: no cover
+    torch, _DTYPES, _STORES = None, {}, {}
+
+PAGE = 128  # positions per page (WB_KV_PAGE)
+
+
+def _row(head_dim: int) -> int:
+    """Stored columns of a head: head_dim up to whole 16s."""
+    return -(-head_dim // 16) * 16
+
+
+def _index(a, n: int, name: str):
+    """(pointer, object to keep) of an int32 index array of n entries; None stays None."""
+    if a is None:
+        return None, None
+    if isinstance(a, torch.Tensor) and a.is_cuda:
+        if a.dtype != torch.int32 or a.dim() != 1 or not a.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 vector")
+        keep, size, ptr = a, a.shape[0], a.data_ptr()
+    else:
+        keep = np.ascontiguousarray(a.numpy() if isinstance(a, torch.Tensor) else a, dtype=np.int32)
+        size, ptr = keep.size, keep.ctypes.data
+    if size != n:
+        raise ValueError(f"{name} must have {n} entries, has {size}")
+    return ptr, keep
+
+
+def _rows(x, name: str, dtype=None):
+    """Shape and strides check of [tokens][heads][head_dim] rows."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 3:
+        raise ValueError(f"{name} must be a CUDA tensor [tokens][heads][head_dim]")
+    if x.dtype not in _DTYPES or (dtype is not None and x.dtype != dtype):
+        raise ValueError(f"{name} must be bfloat16 or float16, as the others")
+    if x.stride(2) != 1 and x.shape[2] > 1:
+        raise ValueError(f"{name}'s last dimension must be contiguous")
+    return x.stride(0), x.stride(1)
+
+
+def _context(ctx, x) -> Context:
+    """The context for x's device, on torch's current stream there."""
+    if ctx is None:
+        ctx = default_context(x.device.index)
+    elif ctx.device != x.device.index:
+        raise ValueError("the context is on another device")
+    ctx.set_stream(torch.cuda.current_stream(x.device).cuda_stream)
+    return ctx
+
+
+def _out(out, shape, dtype, like, name):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != like.device:
+        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on {like.device}")
+    return out
+
+
+def _same_device(x, **others) -> None:
+    for name, t in others.items():
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.device != x.device:
+            raise ValueError(f"{name} is on another device")
+
+
+def gqa_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float | None = None,
+                  return_lse: bool = False, out=None, ctx: Context | None = None):
+    """Attention over packed prompts (wb_gqa_attention).
+
+    q [tokens][n_head][head_dim]; k, v [tokens][n_kv_head][head_dim]; sequence
+    b's rows are cu[b] .. cu[b+1]-1 (``cu_k`` None: as ``cu_q``).  ``scale``
+    None: head_dim ** -0.5.  Returns out like q, and with ``return_lse`` also
+    the log sum exp of every query's scores, [n_head][tokens] fp32."""
+    q_ts, q_hs = _rows(q, "q")
+    k_ts, k_hs = _rows(k, "k", q.dtype)
+    v_ts, v_hs = _rows(v, "v", q.dtype)
+    Tq, H, hd = q.shape
+    Tk, Hkv, _ = k.shape
+    if k.shape != v.shape or k.shape[2] != hd:
+        raise ValueError("k and v must be [tokens][n_kv_head][head_dim], head_dim as q's")
+    _same_device(q, k=k, v=v, cu_q=cu_q, cu_k=cu_k)
+    n_seq = len(cu_q) - 1
+    if n_seq < 0:
+        raise ValueError("cu_q must have one entry more than there are sequences")
+    pq, keep_q = _index(cu_q, n_seq + 1, "cu_q")
+    pk, keep_k = _index(cu_k, n_seq + 1, "cu_k")
+    out = _out(out, (Tq, H, hd), q.dtype, q, "out")
+    o_ts, o_hs = _rows(out, "out", q.dtype)
+    lse = torch.empty((H, Tq), dtype=torch.float32, device=q.device) if return_lse else None
+    ctx = _context(ctx, q)
+    d = _lib.GqaAttnDesc(_DTYPES[q.dtype], H, Hkv, hd, n_seq, int(causal), hd ** -0.5 if scale is None else scale, Tq,
+                         Tk, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, pq, pk,
+                         out.data_ptr(), o_ts, o_hs, None if lse is None else lse.data_ptr())
+    _lib.call("wb_gqa_attention", ctx.handle, C.byref(d))
+    return (out, lse) if return_lse else out
+
+
+def _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, dtype, head_dim):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError("k_pages and v_pages must be [n_pages][n_kv_head][128][row]")
+    n_pages, Hkv, page, row = k_pages.shape
+    store = _STORES.get(k_pages.dtype)
+    if store is None or page != PAGE or row != _row(head_dim):
+        raise ValueError(f"pages must hold {PAGE} rows of {_row(head_dim)} bf16, fp16, int8 or float8_e4m3fn values")
+    if store in (_lib.WB_INT8, _lib.WB_E4M3):
+        for x in (k_scale, v_scale):
+            if x is None or tuple(x.shape) != (n_pages, Hkv, PAGE) or x.dtype != torch.float32:
+                raise ValueError("an 8-bit cache needs fp32 k_scale and v_scale [n_pages][n_kv_head][128]")
+    else:
+        k_scale = v_scale = None
+    if table.dim() != 2 or table.dtype != torch.int32 or (lens is not None and (lens.dtype != torch.int32 or
+                                                          tuple(lens.shape) != (table.shape[0],))):
+        raise ValueError("table must be int32 [n_slots][max_pages] and lens int32 [n_slots]")
+    for x in (k_pages, v_pages, k_scale, v_scale, table, lens):
+        if x is not None and (not x.is_contiguous() or x.device != k_pages.device or not x.is_cuda):
+            raise ValueError("cache arrays must be contiguous CUDA tensors of one device")
+    p = lambda x: None if x is None else x.data_ptr()  # noqa: E731
+    return _lib.GqaCacheDesc(_DTYPES[dtype], store, Hkv, head_dim, n_pages, table.shape[0], table.shape[1],
+                             k_pages.data_ptr(), v_pages.data_ptr(), p(k_scale), p(v_scale), table.data_ptr(), p(lens))
+
+
+def _n_seq(table, cu, slots, rows=None):
+    if cu is not None:
+        return len(cu) - 1
+    if slots is not None:
+        return len(slots)
+    return int(table.shape[0] if rows is None else rows)
+
+
+def gqa_cache_write(k, v, k_pages, v_pages, table, lens, *, cu=None, start=None, slots=None, k_scale=None,
+                    v_scale=None, ctx: Context | None = None) -> None:
+    """Write packed rows into a paged cache (wb_gqa_cache_write).
+
+    Sequence i's rows cu[i] .. cu[i+1]-1 of k and v [tokens][n_kv_head]
+    [head_dim] become positions start[i], .. of slot slots[i] and set its
+    length.  ``cu`` None: one row per sequence; ``start`` None: append;
+    ``slots`` None: 0, 1, .."""
+    k_ts, k_hs = _rows(k, "k")
+    v_ts, v_hs = _rows(v, "v", k.dtype)
+    if k.shape != v.shape or k.shape[1] != k_pages.shape[1]:
+        raise ValueError("k and v must be [tokens][n_kv_head][head_dim]")
+    total, _, hd = k.shape
+    d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, k.dtype, hd)
+    _same_device(k, v=v, k_pages=k_pages, cu=cu, start=start, slots=slots)
+    n_seq = _n_seq(table, cu, slots, total)
+    pc, keep_c = _index(cu, n_seq + 1, "cu")
+    ps, keep_s = _index(start, n_seq, "start")
+    pl, keep_l = _index(slots, n_seq, "slots")
+    ctx = _context(ctx, k)
+    _lib.call("wb_gqa_cache_write", ctx.handle, C.byref(d), pl, n_seq, pc, total, ps, k.data_ptr(), k_ts, k_hs,
+              v.data_ptr(), v_ts, v_hs)
+
+
+def gqa_cache_read(k_pages, v_pages, table, *, head_dim: int, dtype, cu=None, total: int | None = None, start=None,
+                   slots=None, k_scale=None, v_scale=None, ctx: Context | None = None):
+    """Read positions back (wb_gqa_cache_read): (k, v), each [total]
+    [n_kv_head][head_dim] of ``dtype``, packed as in ``gqa_cache_write``
+    (``start`` None: from position 0).  ``total`` may be left out when ``cu``
+    is None or on the host."""
+    if dtype not in _DTYPES:
+        raise ValueError("dtype must be bfloat16 or float16")
+    d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, None, dtype, head_dim)
+    _same_device(k_pages, cu=cu, start=start, slots=slots)
+    n_seq = _n_seq(table, cu, slots)
+    if total is None:
+        if cu is not None and isinstance(cu, torch.Tensor) and cu.is_cuda:
+            raise ValueError("total must be given when cu is on the device")
+        total = n_seq if cu is None else int(cu[-1])
+    pc, keep_c = _index(cu, n_seq + 1, "cu")
+    ps, keep_s = _index(start, n_seq, "start")
+    pl, keep_l = _index(slots, n_seq, "slots")
+    shape = (total, k_pages.shape[1], head_dim)
+    k = torch.empty(shape, dtype=dtype, device=k_pages.device)
+    v = torch.empty(shape, dtype=dtype, device=k_pages.device)
+    ctx = _context(ctx, k_pages)
+    _lib.call("wb_gqa_cache_read", ctx.handle, C.byref(d), pl, n_seq, pc, total, ps, k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+def gqa_decode(q, k_pages, v_pages, table, lens, *, slots=None, k_scale=None, v_scale=None,
+               scale: float | None = None, return_lse: bool = False, out=None, ctx: Context | None = None):
+    """Attention of one new token per sequence over its cached positions
+    (wb_gqa_decode): q [n_seq][n_head][head_dim] -> out like q (and lse
+    [n_seq][n_head] fp32).  Write the token's own key and value first."""
+    q_ss, q_hs = _rows(q, "q")
+    n_seq, H, hd = q.shape
+    d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, q.dtype, hd)
+    _same_device(q, k_pages=k_pages, slots=slots)
+    pl, keep_l = _index(slots, n_seq, "slots")
+    out = _out(out, (n_seq, H, hd), q.dtype, q, "out")
+    if not out.is_contiguous():
+        raise ValueError("out must be contiguous")
+    lse = torch.empty((n_seq, H), dtype=torch.float32, device=q.device) if return_lse else None
+    ctx = _context(ctx, q)
+    _lib.call("wb_gqa_decode", ctx.handle, C.byref(d), pl, n_seq, H, q.data_ptr(), q_ss, q_hs,
+              hd ** -0.5 if scale is None else scale, out.data_ptr(), None if lse is None else lse.data_ptr())
+    return (out, lse) if return_lse else out
+
+
+class GqaCache:
+    """A paged cache of n_layers layers for max_seqs sequences of up to
+    max_ctx positions, sharing one pool of n_pages pages of 128 positions
+    (every layer holds the pool once; a sequence's page ids are the same in
+    all of them).  ``store``: "native" (values of ``dtype``), "int8" or
+    "e4m3".  Lengths are per layer: a layer's write advances its own."""
+
+    def __init__(self, n_layers: int, n_kv_head: int, head_dim: int, max_seqs: int, max_ctx: int, n_pages: int,
+                 dtype=None, store: str = "native", device: int = 0, ctx: Context | None = None):
+        dtype = torch.bfloat16 if dtype is None else dtype
+        kinds = {"native": dtype, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+        if dtype not in _DTYPES or store not in kinds:
+            raise ValueError('dtype must be bfloat16 or float16, store "native", "int8" or "e4m3"')
+        if min(n_layers, n_kv_head, head_dim, max_seqs, max_ctx, n_pages) < 1 or head_dim > 128:
+            raise ValueError("bad cache dimensions (head_dim 1 .. 128)")
+        self.ctx, self.dtype, self.head_dim = ctx, dtype, head_dim
+        self.max_pages = -(-max_ctx // PAGE)
+        dev = torch.device("cuda", device if ctx is None else ctx.device)
+        shape = (n_layers, n_pages, n_kv_head, PAGE, _row(head_dim))
+        self.k_pages = torch.zeros(shape, dtype=torch.uint8 if store != "native" else dtype, device=dev).view(kinds[store])
+        self.v_pages = torch.zeros_like(self.k_pages)
+        scale = lambda: torch.ones(shape[:-1], device=dev) if store != "native" else [None] * n_layers  # noqa: E731
+        self.k_scale, self.v_scale = scale(), scale()
+        self.table = torch.full((max_seqs, self.max_pages), -1, dtype=torch.int32, device=dev)
+        self.lens = torch.zeros((n_layers, max_seqs), dtype=torch.int32, device=dev)
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._held = [[] for _ in range(max_seqs)]
+
+    def reserve(self, seq: int, n_positions: int) -> None:
+        """Pages so that slot ``seq`` holds ``n_positions`` positions."""
+        held, need = self._held[seq], -(-n_positions // PAGE)
+        if need > self.max_pages:
+            raise ValueError("n_positions exceeds max_ctx")
+        more = need - len(held)
+        if more <= 0:
+            return
+        if more > len(self._free):
+            raise RuntimeError(f"out of cache pages ({len(self._free)} free, {more} needed)")
+        new = [self._free.pop() for _ in range(more)]
+        self.table[seq, len(held):need] = torch.tensor(new, dtype=torch.int32, device=self.table.device)
+        held += new
+
+    def release(self, seq: int) -> None:
+        """Empty slot ``seq`` and return its pages to the pool.  Work already
+        queued on the current stream still sees the slot as it was; later
+        work on that stream does not."""
+        self.table[seq].fill_(-1)
+        self.lens[:, seq].fill_(0)
+        self._free += reversed(self._held[seq])
+        self._held[seq] = []
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _layer(self, layer: int) -> dict:
+        return {"k_scale": self.k_scale[layer], "v_scale": self.v_scale[layer], "ctx": self.ctx}
+
+    def write(self, layer: int, k, v, slots=None, cu=None, start=None) -> None:
+        """gqa_cache_write into one layer."""
+        gqa_cache_write(k, v, self.k_pages[layer], self.v_pages[layer], self.table, self.lens[layer], cu=cu,
+                        start=start, slots=slots, **self._layer(layer))
+
+    def read(self, layer: int, slots=None, cu=None, total: int | None = None, start=None):
+        """gqa_cache_read from one layer, in the cache's dtype."""
+        return gqa_cache_read(self.k_pages[layer], self.v_pages[layer], self.table, head_dim=self.head_dim,
+                              dtype=self.dtype, cu=cu, total=total, start=start, slots=slots, **self._layer(layer))
+
+    def decode(self, layer: int, q, slots=None, *, scale: float | None = None, return_lse: bool = False, out=None):
+        """gqa_decode over one layer."""
+        return gqa_decode(q, self.k_pages[layer], self.v_pages[layer], self.table, self.lens[layer], slots=slots,
+                          scale=scale, return_lse=return_lse, out=out, **self._layer(layer))
