@@ -190,7 +190,8 @@ def _decode(store, dtype, H, Hkv, hd, lens, seed=0, scale=None):
     q = torch.randn(len(lens), H, hd, device="cuda", generator=torch.Generator("cuda").manual_seed(seed)).to(dtype)
     out, lse = cache.decode(0, q, return_lse=True, scale=scale)
     o, m, z = ref.attention(q, k, v, list(range(len(lens) + 1)), cu, True, hd ** -0.5 if scale is None else scale)
-    ref.check(out, lse, o, m, z.T)
+    pair = store == "native" and dtype == torch.bfloat16
+    ref.check(out, lse.T, o, m, z, 2.0 ** -16 if pair else 2.0 ** -11, 0.0 if pair else ref.floor(max(lens), v))
     again = cache.decode(0, q, scale=scale)
     assert torch.equal(again, out)
     assert wb.default_context(0).take_device_error() == 0
@@ -239,7 +240,7 @@ def test_decode_value_sizes(store):
     out, lse = cache.decode(0, q, return_lse=True, scale=1.0)
     kk, vv = (x[0].double() * x[1].double()[..., None] for x in (ref.quantise(t, _kinds()[store]) for t in (k, v)))
     o, m, z = ref.attention(q, kk, vv, [0, 1], [0, n], True, 1.0)
-    ref.check(out, lse, o, m, z.T)
+    ref.check(out, lse.T, o, m, z, 2.0 ** -11, ref.floor(n, vv))
 
 
 def test_decode_slots_strides_and_bounds():
