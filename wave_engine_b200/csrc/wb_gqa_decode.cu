@@ -27,11 +27,11 @@
 //     already holds.
 // 8-bit values become fp16 exactly (e4m3 by cvt, int8 by exponent insertion
 // and a subtraction); the K scale multiplies the finished score.  The V
-// scale s_j joins the exponent, w_j = exp2(s_j + log2 vscale_j - m2), with
-// its own running maximum m2: w_j is then relative to the largest weight
-// times scale, so keys with a large probability and small values survive
-// the rounding of w to fp16 (scaled by 2^8: weights down to 2^-32 of the
-// largest count).  With bf16 values p is the sum of two bf16 numbers, each
+// scale joins the weight, w_j = p_j vscale_j 2^(m - m2), where m2 is a running
+// maximum of its own, of log2 (p_j vscale_j): w_j is then relative to the
+// largest weight times scale, so keys with a large probability and small
+// values survive the rounding of w to fp16 (kept as 2^8 w: weights down to
+// 2^-32 of the largest count).  With bf16 values p is the sum of two bf16 numbers, each
 // with its own product: the tensor pipe has the room, and 8 bits of p would
 // cost as much precision as the output's own rounding.
 #include "wb_gqa.h"
@@ -55,8 +55,10 @@ struct GqaDecodeArgs {
 
 static constexpr int GD_WARPS = 4, GD_THREADS = GD_WARPS * 32;
 static constexpr int GD_UNIT = 64;      // keys per unit: one 16-key block for each warp
+static constexpr int GD_ITEM = 2;       // what an item's start and end cost, in units of the line
+static constexpr int GD_SEQS = 256;     // sequences of a CTA's share whose lengths it holds in shared memory
 static constexpr float GD_SHIFT = 8.0f; // weights are kept as 2^8 exp2(s - m): see above
-static constexpr float GD_LAZY = 6.0f;  // m follows the maximum once it is this far behind (2^14 < 65504)
+static constexpr float GD_MOST = 16384.0f;  // largest weight before m follows the maximum (fp16 ends at 65504)
 
 enum { GD_NATIVE = 0, GD_INT8 = 1, GD_E4M3 = 2 };
 
@@ -72,12 +74,13 @@ struct GdConf {
     static constexpr int STAGE = 2 * 16 * RB + SCALES;
     static constexpr int CTAS = HDP == 64 ? 4 : (ESZ == 2 ? 2 : 3);
     static constexpr int NST = HDP == 64 ? (ESZ == 2 ? 3 : 6) : (ESZ == 2 ? 3 : 4);
+    static constexpr int MST = 16 * HDP * 4 > STAGE ? 2 : 1;  // stages that hold a warp's 16 output rows
     static constexpr int BYTES = GD_WARPS * NST * STAGE;
-    static_assert(BYTES * CTAS <= 224 * 1024, "shared memory of the resident CTAs");
-    static_assert(BYTES >= GD_WARPS * 16 * HDP * 4 && BYTES >= 148 * CTAS * 64, "the joins reuse the ring");
+    static_assert((BYTES + 4096) * CTAS <= 227 * 1024, "shared memory of the resident CTAs");
+    static_assert(16 * HDP * 4 <= MST * STAGE && NST - MST >= 1, "the join uses the ring");
 };
 
-// floats of one piece: 16 rows' log2 sum exp, then 16 rows of HDP values
+// Floats of one piece: 16 rows' log2 sum exp, then 16 rows of HDP values
 __host__ __device__ constexpr int gqa_piece(int hdp) { return 16 + 16 * hdp; }
 
 template <bool BF>
@@ -155,30 +158,40 @@ __device__ __forceinline__ int gd_len(const GqaCacheArgs &c, int b, int *slot) {
     return n;
 }
 
-template <class T, int KIND, int HDP>
+// The part of one item that a CTA takes: units ua .. ub-1 of U, keys k0 .. k1-1.
+struct GdSeg {
+    int b, slot, hk, h0, nrow, ua, ub, U, k0, k1;
+    long long first, last;  // the item's first and last unit on the line
+};
+
+template <class T, int KIND, int HDP, bool FULL>
 __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decode_kernel(GqaDecodeArgs a) {
     using F = GdConf<KIND, HDP>;
-    constexpr bool BF = KIND == GD_NATIVE && sizeof(T) == 2 && __is_same(T, __nv_bfloat16);  // product type
+    constexpr bool BF = KIND == GD_NATIVE && __is_same(T, __nv_bfloat16);  // product type
     constexpr bool QUANT = KIND != GD_NATIVE;
     constexpr int NK = HDP / 16;  // q . k products per 8 keys
     constexpr int NV = HDP / 8;   // p v products per 16 keys
+    constexpr int NST = F::NST, MST = F::MST;
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ long long s_scan[GD_WARPS];
-    __shared__ long long s_pref;
+    __shared__ long long s_pref, s_at;
+    __shared__ GdSeg s_seg[3];
     __shared__ int s_seq;
+    __shared__ int s_len[GD_SEQS], s_slot[GD_SEQS];
     __shared__ float s_m[GD_WARPS][16], s_l[GD_WARPS][16], s_m2[GD_WARPS][16], s_f[GD_WARPS][16], s_row[16];
-    __shared__ int s_last;
+    __shared__ int s_last, s_stage[GD_WARPS];
     const GqaCacheArgs &c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, cc = lane & 3;
     const int G = a.H / c.Hkv, nch = (G + 15) / 16, ips = c.Hkv * nch;  // items of a sequence
 
-    // ---- the line of units and this CTA's share
+    // ---- the line of units and this CTA's share s0 .. s1-1
+    auto line_len = [&](int n) { return n == 0 ? 0LL : (long long)((n + GD_UNIT - 1) / GD_UNIT + GD_ITEM) * ips; };
     const int per = (c.n_seq + GD_THREADS - 1) / GD_THREADS;
     long long mine = 0;
     for (int b = tid * per; b < min((tid + 1) * per, c.n_seq); b++) {
         int slot;
         const int n = gd_len(c, b, &slot);
-        mine += (long long)((n + GD_UNIT - 1) / GD_UNIT) * ips;
+        mine += line_len(n);
         if (n == 0 && b % (int)gridDim.x == (int)blockIdx.x) {
             T *op = (T *)a.out + (long long)b * a.H * c.hd;
             for (int i = 0; i < a.H * c.hd; i++) op[i] = from_f<T>(0.0f);
@@ -207,7 +220,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
         int b = tid * per;
         for (;; b++) {
             int slot;
-            const long long n = (long long)((gd_len(c, b, &slot) + GD_UNIT - 1) / GD_UNIT) * ips;
+            const long long n = line_len(gd_len(c, b, &slot));
             if (s0 < before + n) break;
             before += n;
         }
@@ -215,111 +228,204 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
         s_pref = before;
     }
     __syncthreads();
-    int b = s_seq;
-    long long pref = s_pref;
+    const int b0 = s_seq;
+    for (int i = tid; i < GD_SEQS && b0 + i < c.n_seq; i += GD_THREADS) s_len[i] = gd_len(c, b0 + i, &s_slot[i]);
+    __syncthreads();
 
-    uint8_t *ring = sm + warp * (F::NST * F::STAGE);
-    const int rowb = c.row * F::ESZ;
-    for (long long u = s0; u < s1;) {
-        int slot;
-        const int len = gd_len(c, b, &slot);
-        const int U = (len + GD_UNIT - 1) / GD_UNIT;
-        if (U == 0) {
-            b++;
-            continue;
-        }
-        const long long rel = u - pref;
-        const int item = (int)(rel / U), ua = (int)(rel - (long long)item * U);
-        const int ub = (int)min((long long)U, ua + (s1 - u));
-        const int hk = item / nch, hc = item - hk * nch;
-        const int h0 = hk * G + hc * 16, nrow = min(16, G - hc * 16);
-        const int k0 = ua * GD_UNIT, k1 = min(ub * GD_UNIT, len);
-
-        // ---- loads of this warp's blocks k0 + 16 (warp + 4 i)
-        const int nblk = (k1 - k0 + 15) >> 4;
-        const int cnt = (nblk - warp + GD_WARPS - 1) / GD_WARPS;
-        const int32_t *trow = c.table + (long long)slot * c.max_pages;
-        const int last_page = (k1 - 1) >> WB_PAGE_SHIFT;
-        int pbase = k0 >> WB_PAGE_SHIFT;
-        int pid = pbase + lane <= last_page ? __ldg(trow + pbase + lane) : -1;
-        auto issue = [&](int i) {
-            const int key0 = k0 + 16 * (warp + GD_WARPS * i);
-            const int p = key0 >> WB_PAGE_SHIFT;
-            if (p >= pbase + 32) {
-                pbase = p;
-                pid = pbase + lane <= last_page ? __ldg(trow + pbase + lane) : -1;
+    // The share's parts with keys, one after another, U = 0 past its end.  One
+    // thread finds part x + 2 while part x is joined.
+    auto next_seg = [&](GdSeg &g) {
+        int nb = s_seq;
+        long long pref = s_pref, u = s_at;
+        g.U = 0;
+        while (u < s1) {
+            int slot, len;
+            if (nb - b0 < GD_SEQS) {
+                len = s_len[nb - b0];
+                slot = s_slot[nb - b0];
+            } else len = gd_len(c, nb, &slot);
+            const long long n = line_len(len);
+            if (u >= pref + n) {
+                pref += n;
+                nb++;
+                continue;
             }
-            const int pg = __shfl_sync(0xffffffffu, pid, p - pbase);
-            const bool ok = pg >= 0 && pg < c.n_pages;
-            const long long row0 = ok ? ((long long)pg * c.Hkv + hk) * WB_PAGE + (key0 & (WB_PAGE - 1)) : 0;
-            uint8_t *st = ring + (i % F::NST) * F::STAGE;
-            const uint8_t *kp = (const uint8_t *)c.k_pages + row0 * rowb, *vp = (const uint8_t *)c.v_pages + row0 * rowb;
-            const int ch = lane % F::CPR;
+            const int U = (len + GD_UNIT - 1) / GD_UNIT, il = U + GD_ITEM;
+            const long long rel = u - pref;
+            const int item = (int)(rel / il), o0 = (int)(rel - (long long)item * il);
+            const int o1 = (int)min((long long)il, o0 + (s1 - u));
+            u += o1 - o0;
+            if (o1 <= GD_ITEM) continue;
+            g.b = nb;
+            g.slot = slot;
+            g.hk = item / nch;
+            const int hc = item - g.hk * nch;
+            g.h0 = g.hk * G + hc * 16;
+            g.nrow = min(16, G - hc * 16);
+            g.U = U;
+            g.ua = max(0, o0 - GD_ITEM);
+            g.ub = o1 - GD_ITEM;
+            g.k0 = g.ua * GD_UNIT;
+            g.k1 = min(g.ub * GD_UNIT, len);
+            g.first = pref + (long long)item * il + GD_ITEM;
+            g.last = g.first + U - 1;
+            break;
+        }
+        s_seq = nb;
+        s_pref = pref;
+        s_at = u;
+    };
+    if (tid == 0) {
+        s_at = s0;
+        next_seg(s_seg[0]);
+        next_seg(s_seg[1]);
+    }
+    __syncthreads();
+
+    uint8_t *ring = sm + warp * (NST * F::STAGE);
+    // FULL: rows of HDP values, so that a block's offsets are constants
+    const int rowb = FULL ? F::RB : c.row * F::ESZ;
+    // this lane's pieces of a block: ch of rows lr, lr + STEP, ..  Piece
+    // positions within each 128 bytes of the ring: K's by row parity, V's by
+    // row pair, so that the fragments' reads touch every bank once.
+    constexpr int STEP = 32 / F::CPR;
+    const int ch = lane % F::CPR, lr = lane / F::CPR;
+    const bool col = FULL || ch * 16 < rowb;
+    const uint32_t src0 = lr * rowb + ch * 16;
+    auto ring_at = [&](int rr, int ch, bool v) {
+        const int pos = (F::RB == 64 ? (rr & 1) * 4 : 0) + ch;
+        const int line = rr * F::RB / 128 + (F::RB == 256 ? ch / 8 : 0);
+        const int sw = v ? ((rr >> 1) & 3) << 1 : F::RB == 64 ? 0 : (rr & 1) << 2;
+        return line * 128 + (((pos & 7) ^ sw) << 4);
+    };
+
+    // ---- loads of a part's blocks: this warp's are keys k0 + 16 (warp + 4 i)
+    int pbase = 0, pid = -1;  // page ids of pages pbase + lane of the part
+    auto pages_of = [&](const GdSeg &g, int p) {
+        return p + lane <= (g.k1 - 1) >> WB_PAGE_SHIFT ? __ldg(c.table + (long long)g.slot * c.max_pages + p + lane) : -1;
+    };
+    auto blocks_of = [&](const GdSeg &g) { return (((g.k1 - g.k0 + 15) >> 4) - warp + GD_WARPS - 1) / GD_WARPS; };
+    auto issue = [&](const GdSeg &g, int i, int stage) {
+        const int key0 = g.k0 + 16 * (warp + GD_WARPS * i);
+        const int p = key0 >> WB_PAGE_SHIFT;
+        if (p >= pbase + 32) {
+            pbase = p;
+            pid = pages_of(g, p);
+        }
+        const int pg = __shfl_sync(0xffffffffu, pid, p - pbase);
+        const bool ok = pg >= 0 && pg < c.n_pages;
+        const long long row0 = ok ? ((long long)pg * c.Hkv + g.hk) * WB_PAGE + (key0 & (WB_PAGE - 1)) : 0;
+        uint8_t *st = ring + stage * F::STAGE;
+        const uint8_t *kp = (const uint8_t *)c.k_pages + row0 * rowb, *vp = (const uint8_t *)c.v_pages + row0 * rowb;
+        if (ok && key0 + 16 <= g.k1) {
 #pragma unroll
             for (int x = 0; x < F::CPR / 2; x++) {
-                const int rr = lane / F::CPR + x * (32 / F::CPR);
-                const int n = ok && key0 + rr < k1 && ch * 16 < rowb ? 16 : 0;
-                const long long off = n ? (long long)rr * rowb + ch * 16 : 0;
-                // piece positions within each 128 bytes: K's by row parity, V's
-                // by row pair, so that the fragments' reads below touch every
-                // bank once
-                const int pos = (F::RB == 64 ? (rr & 1) * 4 : 0) + ch, line = rr * F::RB / 128 + (F::RB == 256 ? ch / 8 : 0);
-                const int kpos = F::RB == 64 ? pos : (pos & 7) ^ ((rr & 1) << 2);
-                const int vpos = (pos & 7) ^ (((rr >> 1) & 3) << 1);
-                cp_async16_or_zero(st + line * 128 + kpos * 16, kp + off, n);
-                cp_async16_or_zero(st + 16 * F::RB + line * 128 + vpos * 16, vp + off, n);
+                const int rr = lr + x * STEP;
+                if (FULL) {
+                    ptx::cp_async<16>(st + ring_at(rr, ch, false), kp + src0 + x * STEP * F::RB);
+                    ptx::cp_async<16>(st + 16 * F::RB + ring_at(rr, ch, true), vp + src0 + x * STEP * F::RB);
+                } else {
+                    const uint32_t off = col ? src0 + x * STEP * rowb : 0;
+                    cp_async16_or_zero(st + ring_at(rr, ch, false), kp + off, col ? 16 : 0);
+                    cp_async16_or_zero(st + 16 * F::RB + ring_at(rr, ch, true), vp + off, col ? 16 : 0);
+                }
             }
-            if (QUANT && lane < 8) {
-                const float *sp = (lane < 4 ? c.k_scale : c.v_scale) + row0 + (lane & 3) * 4;
-                cp_async16_or_zero(st + 32 * F::RB + lane * 16, sp, ok ? 16 : 0);
+        } else {
+#pragma unroll 1
+            for (int x = 0; x < F::CPR / 2; x++) {
+                const int rr = lr + x * STEP;
+                const int n = ok && col && key0 + rr < g.k1 ? 16 : 0;
+                const uint32_t off = n ? src0 + x * STEP * rowb : 0;
+                cp_async16_or_zero(st + ring_at(rr, ch, false), kp + off, n);
+                cp_async16_or_zero(st + 16 * F::RB + ring_at(rr, ch, true), vp + off, n);
             }
-            return ok;
-        };
-        uint32_t okbits = 0;  // bit i % NST: block i's page is mapped
-#pragma unroll
-        for (int i = 0; i < F::NST - 1; i++) {
-            if (i < cnt && issue(i)) okbits |= 1u << i;
-            ptx::cp_async_commit();
         }
-
-        // ---- queries: rows r and r + 8 of the 16, dims in the order of K's pieces
-        uint32_t qf[NK][4];
-        float fac[2];  // score factor of the two rows, log2 e included
-        {
-            float amax[2] = {0.0f, 0.0f};
-            float qv[2][NK * 4];
+        if (QUANT && lane < 8) {
+            const float *sp = (lane < 4 ? c.k_scale : c.v_scale) + row0 + (lane & 3) * 4;
+            cp_async16_or_zero(st + 32 * F::RB + lane * 16, sp, ok ? 16 : 0);
+        }
+        return ok;
+    };
+    // a part's queries as loaded: rows r and r + 8, dims in the order of K's pieces
+    const bool q8 = ((a.q_ss | a.q_hs | c.hd) & 3) == 0 && (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
+    auto q_dim = [&](int t) { return F::ESZ == 1 ? 16 * (cc + 4 * (t / 4)) + 4 * (t % 4) : 8 * (cc + 4 * (t / 2)) + 4 * (t % 2); };
+    uint32_t qf[NK][4];
+    auto load_q = [&](const GdSeg &g) {
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                const int row = r + 8 * hf;
-                const T *qp = (const T *)a.q + b * a.q_ss + (long long)(h0 + row) * a.q_hs;
-#pragma unroll
-                for (int t = 0; t < NK; t++) {
-                    const int d0 = F::ESZ == 1 ? 16 * (cc + 4 * (t / 4)) + 4 * (t % 4) : 8 * (cc + 4 * (t / 2)) + 4 * (t % 2);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float x = row < nrow && d0 + e < c.hd ? to_f(qp[d0 + e]) : 0.0f;
-                        qv[hf][t * 4 + e] = x;
-                        amax[hf] = fmaxf(amax[hf], fabsf(x));
-                    }
-                }
-                fac[hf] = a.scale * 1.4426950408889634f;
-                if (QUANT && !__is_same(T, __half)) {
-                    // bf16 queries meet fp16 keys: divided by a power of two
-                    // so that the row's largest is in [1, 2) (exact down to
-                    // 2^-14 of it)
-                    const int e = min(max((int)(__float_as_uint(quad_max(amax[hf])) >> 23), 1), 253);
-                    const float f = __uint_as_float((uint32_t)(254 - e) << 23);
-                    fac[hf] *= __uint_as_float((uint32_t)e << 23);
-#pragma unroll
-                    for (int i = 0; i < NK * 4; i++) qv[hf][i] *= f;
-                }
-            }
+        for (int hf = 0; hf < 2; hf++) {
+            const int row = r + 8 * hf;
+            const uint16_t *qp = (const uint16_t *)a.q + g.b * a.q_ss + (long long)(g.h0 + row) * a.q_hs;
 #pragma unroll
             for (int t = 0; t < NK; t++) {
-                qf[t][0] = pack2(qv[0][t * 4], qv[0][t * 4 + 1], BF);
-                qf[t][1] = pack2(qv[1][t * 4], qv[1][t * 4 + 1], BF);
-                qf[t][2] = pack2(qv[0][t * 4 + 2], qv[0][t * 4 + 3], BF);
-                qf[t][3] = pack2(qv[1][t * 4 + 2], qv[1][t * 4 + 3], BF);
+                const int d0 = q_dim(t);
+                uint2 w = make_uint2(0, 0);
+                if (row < g.nrow) {
+                    if (q8) {
+                        if (d0 < c.hd) w = __ldg(reinterpret_cast<const uint2 *>(qp + d0));
+                    } else {
+                        uint32_t e[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) e[i] = d0 + i < c.hd ? __ldg(qp + d0 + i) : 0;
+                        w = make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
+                    }
+                }
+                qf[t][hf] = w.x;
+                qf[t][2 + hf] = w.y;
+            }
+        }
+    };
+
+    if (s_seg[0].U == 0) return;
+    load_q(s_seg[0]);
+    pbase = s_seg[0].k0 >> WB_PAGE_SHIFT;
+    pid = pages_of(s_seg[0], pbase);
+    int stage = 0;  // ring stage of the part's first block
+    int cnt = blocks_of(s_seg[0]);
+    uint32_t okbits = 0;  // bit of a stage: its block's page is mapped
+#pragma unroll
+    for (int i = 0; i < NST - MST; i++) {
+        if (i < cnt && issue(s_seg[0], i, i)) okbits |= 1u << i;
+        ptx::cp_async_commit();
+    }
+    for (int part = 0;; part++) {
+        const GdSeg &g = s_seg[part % 3], &h = s_seg[(part + 1) % 3];
+        // ---- the rest of the first loads (the first NST - MST are under way)
+#pragma unroll
+        for (int i = NST - MST; i < NST - 1; i++) {
+            const int sg = (stage + i) % NST;
+            okbits &= ~(1u << sg);
+            if (i < cnt && issue(g, i, sg)) okbits |= 1u << sg;
+            ptx::cp_async_commit();
+        }
+        // the next part's page ids, long before they are needed
+        const bool more = h.U != 0;
+        const int hpid = more ? pages_of(h, h.k0 >> WB_PAGE_SHIFT) : -1;
+
+        float fac[2];  // score factor of the two rows, log2 e included
+        fac[0] = fac[1] = a.scale * 1.4426950408889634f;
+        if (QUANT && !__is_same(T, __half)) {
+            // bf16 queries meet fp16 keys: divided by a power of two so that
+            // the row's largest is in [1, 2) (exact down to 2^-14 of it)
+#pragma unroll
+            for (int hf = 0; hf < 2; hf++) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int t = 0; t < NK; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        top = max(top, max((qf[t][2 * e + hf] << 16) & 0x7fffffffu, qf[t][2 * e + hf] & 0x7fff0000u));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e = min(max((int)(top >> 23), 1), 253);
+                const float f = __uint_as_float((uint32_t)(254 - e) << 23);
+                fac[hf] *= __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+                for (int t = 0; t < NK; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t x = qf[t][2 * e + hf];
+                        qf[t][2 * e + hf] = pack2(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xffff0000u) * f, false);
+                    }
             }
         }
 
@@ -328,21 +434,23 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
         for (int j = 0; j < NV; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
         // finite stand-ins for -inf: the first visible score replaces them
         float m[2] = {-1e30f, -1e30f}, m2[2] = {-1e30f, -1e30f}, l[2] = {0.0f, 0.0f};
+        float off[2] = {1e30f, 1e30f}, e2[2] = {1.0f, 1.0f};  // 8 - m, 2^(m - m2)
         bool unmapped = false;
 
+        int stg = stage, nxs = (stage + NST - 1) % NST;
+        const int kbeg = g.k0, kend = g.k1;
         for (int i = 0; i < cnt; i++) {
-            ptx::cp_async_wait<F::NST - 2>();
+            ptx::cp_async_wait<NST - 2>();
             __syncwarp();
-            const int stg = i % F::NST;
             const bool ok = (okbits >> stg) & 1;
-            const int nx = i + F::NST - 1;
-            if (nx < cnt) {
-                okbits &= ~(1u << (nx % F::NST));
-                if (issue(nx)) okbits |= 1u << (nx % F::NST);
-            }
+            okbits &= ~(1u << nxs);
+            if (i + NST - 1 < cnt && issue(g, i + NST - 1, nxs)) okbits |= 1u << nxs;
             ptx::cp_async_commit();
             const uint8_t *st = ring + stg * F::STAGE;
-            const int key0 = k0 + 16 * (warp + GD_WARPS * i);
+            const int key0 = kbeg + 16 * (warp + GD_WARPS * i);
+            const int k1 = kend;
+            nxs = stg;
+            if (++stg == NST) stg = 0;
 
             // scores of keys 0-7 (s[0]) and 8-15 (s[1])
             float s[2][4] = {};
@@ -351,11 +459,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                 const int rr = r + 8 * g;
 #pragma unroll
                 for (int x = 0; x < F::CPR / 4; x++) {
-                    const int ch = cc + 4 * x;
-                    const int pos = (F::RB == 64 ? (rr & 1) * 4 : 0) + ch;
-                    const int line = rr * F::RB / 128 + (F::RB == 256 ? ch / 8 : 0);
-                    const int kpos = F::RB == 64 ? pos : (pos & 7) ^ ((rr & 1) << 2);
-                    const uint4 w = *reinterpret_cast<const uint4 *>(st + line * 128 + kpos * 16);
+                    const uint4 w = *reinterpret_cast<const uint4 *>(st + ring_at(rr, cc + 4 * x, false));
                     if constexpr (QUANT) {
                         mma16816<BF>(s[g], qf[4 * x], to_f16x2<KIND, 0>(w.x), to_f16x2<KIND, 1>(w.x));
                         mma16816<BF>(s[g], qf[4 * x + 1], to_f16x2<KIND, 0>(w.y), to_f16x2<KIND, 1>(w.y));
@@ -368,47 +472,65 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                 }
             }
             // this lane's keys: 2cc, 2cc+1 (g = 0) and 2cc+8, 2cc+9 (g = 1)
-            float lv[2][2];
+            float vs[2][2];
 #pragma unroll
             for (int g = 0; g < 2; g++) {
-                float2 ks = make_float2(1.0f, 1.0f), vs = ks;
                 if (QUANT) {
-                    ks = *reinterpret_cast<const float2 *>(st + 32 * F::RB + (2 * cc + 8 * g) * 4);
-                    vs = *reinterpret_cast<const float2 *>(st + 32 * F::RB + 64 + (2 * cc + 8 * g) * 4);
-                    lv[g][0] = lg2(vs.x);
-                    lv[g][1] = lg2(vs.y);
-                }
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const bool vis = ok && key0 + 2 * cc + 8 * g + e < k1;
-                    const float kf = e ? ks.y : ks.x;
-                    s[g][e] = vis ? s[g][e] * fac[0] * kf : -INFINITY;
-                    s[g][2 + e] = vis ? s[g][2 + e] * fac[1] * kf : -INFINITY;
-                    if (QUANT && !vis) lv[g][e] = 0.0f;
+                    const float2 ks = *reinterpret_cast<const float2 *>(st + 32 * F::RB + (2 * cc + 8 * g) * 4);
+                    const float2 v2 = *reinterpret_cast<const float2 *>(st + 32 * F::RB + 64 + (2 * cc + 8 * g) * 4);
+                    s[g][0] *= ks.x;
+                    s[g][1] *= ks.y;
+                    s[g][2] *= ks.x;
+                    s[g][3] *= ks.y;
+                    vs[g][0] = v2.x;
+                    vs[g][1] = v2.y;
                 }
             }
+            // keys past the end or on an unmapped page
+            const bool tail = !ok || key0 + 16 > k1;
+            auto dead = [&](int g, int e) { return tail && (!ok || key0 + 2 * cc + 8 * g + e >= k1); };
             unmapped |= !ok;
-            float mx[2], mx2[2];
+            float pr[2][4], wr[2][4];
+            auto weigh = [&]() {
+                float top = 0.0f;
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                mx[hf] = quad_max(fmaxf(fmaxf(s[0][2 * hf], s[0][2 * hf + 1]), fmaxf(s[1][2 * hf], s[1][2 * hf + 1])));
-                if (QUANT)
-                    mx2[hf] = quad_max(fmaxf(fmaxf(s[0][2 * hf] + lv[0][0], s[0][2 * hf + 1] + lv[0][1]),
-                                             fmaxf(s[1][2 * hf] + lv[1][0], s[1][2 * hf + 1] + lv[1][1])));
-                else mx2[hf] = mx[hf];
-            }
-            // the references follow the maxima when one is far ahead
-            const bool far = mx[0] > m[0] + GD_LAZY || mx[1] > m[1] + GD_LAZY ||
-                             (QUANT && (mx2[0] > m2[0] + GD_LAZY || mx2[1] > m2[1] + GD_LAZY));
-            if (__any_sync(0xffffffffu, far)) {
+                for (int g = 0; g < 2; g++)
+#pragma unroll
+                    for (int hf = 0; hf < 2; hf++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int i4 = 2 * hf + e;
+                            pr[g][i4] = ex2(fmaf(s[g][i4], fac[hf], off[hf]));
+                            if (QUANT) wr[g][i4] = pr[g][i4] * (vs[g][e] * e2[hf]);
+                            if (tail && dead(g, e)) pr[g][i4] = wr[g][i4] = 0.0f;
+                            top = fmaxf(top, pr[g][i4]);
+                            if (QUANT) top = fmaxf(top, wr[g][i4]);
+                        }
+                return top;
+            };
+            // The references m, m2 stay until a weight passes 2^14; then they
+            // follow the maxima.
+            if (__any_sync(0xffffffffu, !(weigh() <= GD_MOST))) {
                 float f2[2];
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
-                    const float mn = fmaxf(m[hf], mx[hf]), mn2 = fmaxf(m2[hf], mx2[hf]);
+                    float mx = -INFINITY, mx2 = -INFINITY;
+#pragma unroll
+                    for (int g = 0; g < 2; g++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            if (!dead(g, e)) {
+                                const float x = s[g][2 * hf + e] * fac[hf];
+                                mx = fmaxf(mx, x);
+                                if (QUANT) mx2 = fmaxf(mx2, x + lg2(vs[g][e]));
+                            }
+                    const float mn = fmaxf(m[hf], quad_max(mx)), mn2 = QUANT ? fmaxf(m2[hf], quad_max(mx2)) : mn;
                     l[hf] *= ex2(m[hf] - mn);
                     f2[hf] = ex2(m2[hf] - mn2);
                     m[hf] = mn;
                     m2[hf] = mn2;
+                    off[hf] = GD_SHIFT - mn;
+                    if (QUANT) e2[hf] = ex2(mn - mn2);
                 }
 #pragma unroll
                 for (int j = 0; j < NV; j++) {
@@ -417,18 +539,16 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                     acc[j][2] *= f2[1];
                     acc[j][3] *= f2[1];
                 }
+                weigh();
             }
             uint32_t pf[4], pl[4];
 #pragma unroll
             for (int g = 0; g < 2; g++)
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
-                    const float p0 = ex2(s[g][2 * hf] - m[hf] + GD_SHIFT), p1 = ex2(s[g][2 * hf + 1] - m[hf] + GD_SHIFT);
+                    const float p0 = pr[g][2 * hf], p1 = pr[g][2 * hf + 1];
                     l[hf] += p0 + p1;
-                    if (QUANT)
-                        pf[2 * g + hf] = pack2(ex2(s[g][2 * hf] + lv[g][0] - m2[hf] + GD_SHIFT),
-                                               ex2(s[g][2 * hf + 1] + lv[g][1] - m2[hf] + GD_SHIFT), BF);
-                    else pf[2 * g + hf] = pack2(p0, p1, BF);
+                    pf[2 * g + hf] = QUANT ? pack2(wr[g][2 * hf], wr[g][2 * hf + 1], BF) : pack2(p0, p1, BF);
                     if (BF) {
                         const uint32_t x = pf[2 * g + hf];
                         pl[2 * g + hf] = pack2(p0 - __uint_as_float(x << 16), p1 - __uint_as_float(x & 0xffff0000u), BF);
@@ -486,10 +606,28 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                 }
             }
         }
+        // every block of the part has been read: the next part's first loads
+        // and queries go out before this one's join
+        stage = stg;
         ptx::cp_async_wait<0>();
+        int hcnt = 0;
+        if (more) {
+            hcnt = blocks_of(h);
+            pbase = h.k0 >> WB_PAGE_SHIFT;
+            pid = hpid;
+            okbits = 0;
+#pragma unroll
+            for (int i = 0; i < NST - MST; i++) {
+                const int sg = (stage + i) % NST;
+                if (i < hcnt && issue(h, i, sg)) okbits |= 1u << sg;
+                ptx::cp_async_commit();
+            }
+            load_q(h);
+        }
         if (unmapped && lane == 0) atomicOr(c.dev_err, WB_DERR_BOUNDS);
 
-        // ---- the four warps' outputs into one
+        // ---- the four warps' outputs into one, through the MST ring stages
+        // (8 or 16 rows each) that hold none of the next part's blocks
         l[0] = quad_sum(l[0]);
         l[1] = quad_sum(l[1]);
         if (cc == 0) {
@@ -500,8 +638,13 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                 s_m2[warp][r + 8 * hf] = QUANT ? m2[hf] : m[hf];
             }
         }
-        __syncthreads();  // the rings have been read
-        float *buf = reinterpret_cast<float *>(sm);
+        // row's values of warp w (each warp has its own stage: s_stage)
+        if (lane == 0) s_stage[warp] = stage;
+        auto row_at = [&](int w, int stage_w, int row) {
+            const int sg = (stage_w + NST - MST + (MST == 2 ? row >> 3 : 0)) % NST;
+            return reinterpret_cast<float *>(sm + (w * NST + sg) * F::STAGE) + (MST == 2 ? row & 7 : row) * HDP;
+        };
+        __syncwarp();
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             // column n of product j is dim n * 16 + j (8-bit, 128 columns), n * 8 + j % 8 + 64 (j / 8) (else)
@@ -509,9 +652,11 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
             for (int e = 0; e < 4; e++) {
                 const int row = r + 8 * (e >> 1), n = 2 * cc + (e & 1);
                 const int d = F::ESZ == 1 && HDP == 128 ? n * 16 + j : n * 8 + (j & 7) + 64 * (j >> 3);
-                if (row < nrow) buf[(warp * 16 + row) * HDP + d] = acc[j][e];
+                if (row < g.nrow) row_at(warp, stage, row)[d] = acc[j][e];
             }
         }
+        __syncthreads();
+        if (tid == GD_THREADS - 1) next_seg(s_seg[(part + 2) % 3]);
         if (tid < 16) {
             float M = -1e30f, M2 = -1e30f, L = 0.0f;
             for (int w = 0; w < GD_WARPS; w++) {
@@ -524,24 +669,25 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
             s_row[tid] = L == 0.0f ? -INFINITY : M - GD_SHIFT + log2f(L);  // log2 sum exp
         }
         __syncthreads();
-        const bool whole = ua == 0 && ub == U;
-        float *piece = a.part + ((long long)blockIdx.x * 2 + (ua == 0 ? 1 : 0)) * gqa_piece(HDP);
-        for (int i = tid; i < nrow * c.hd; i += GD_THREADS) {
-            const int row = i / c.hd, d = i - row * c.hd;
+        const bool whole = g.ua == 0 && g.ub == g.U;
+        float *piece = a.part + ((long long)blockIdx.x * 2 + (g.ua == 0 ? 1 : 0)) * gqa_piece(HDP);
+        const long long row_out = (long long)g.b * a.H + g.h0;
+        for (int i = tid; i < g.nrow * HDP; i += GD_THREADS) {
+            const int row = i / HDP, d = i % HDP;
             float o = 0.0f;
 #pragma unroll
-            for (int w = 0; w < GD_WARPS; w++) o += buf[(w * 16 + row) * HDP + d] * s_f[w][row];
-            if (whole) ((T *)a.out)[((long long)b * a.H + h0 + row) * c.hd + d] = from_f<T>(o);
-            else __stcg(piece + 16 + row * HDP + d, o);
+            for (int w = 0; w < GD_WARPS; w++) o += row_at(w, s_stage[w], row)[d] * s_f[w][row];
+            if (whole) {
+                if (d < c.hd) ((T *)a.out)[(row_out + row) * c.hd + d] = from_f<T>(o);
+            } else __stcg(piece + 16 + i, o);
         }
-        if (tid < nrow) {
+        if (tid < g.nrow) {
             if (!whole) __stcg(piece + tid, s_row[tid]);
-            else if (a.lse) a.lse[(long long)b * a.H + h0 + tid] = s_row[tid] * 0.6931471805599453f;
+            else if (a.lse) a.lse[row_out + tid] = s_row[tid] * 0.6931471805599453f;
         }
         if (!whole) {
-            // ---- the last CTA of the item's joins the pieces
-            const long long i0 = pref + (long long)item * U;
-            const int c0 = (int)(((i0 + 1) * grid - 1) / total), c1 = (int)(((i0 + U) * grid - 1) / total);
+            // ---- the item's last CTA joins the pieces
+            const int c0 = (int)(((g.first + 1) * grid - 1) / total), c1 = (int)(((g.last + 1) * grid - 1) / total);
             __threadfence();
             __syncthreads();
             if (tid == 0) s_last = atomicAdd(a.counters + c0, 1) == (unsigned)(c1 - c0);
@@ -552,46 +698,40 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                 const int n = c1 - c0 + 1;
                 // piece x of the item: the first CTA's second slot, the others' first
                 auto at = [&](int x) { return a.part + ((long long)(c0 + x) * 2 + (x == 0 ? 1 : 0)) * gqa_piece(HDP); };
-                float *wt = reinterpret_cast<float *>(sm);  // [n][16] weights
-                for (int row = warp; row < nrow; row += GD_WARPS) {
+                for (int row = warp; row < g.nrow; row += GD_WARPS) {
                     float M = -INFINITY, L = 0.0f;
                     for (int x = lane; x < n; x += 32) M = fmaxf(M, __ldcg(at(x) + row));
                     M = warp_max(M);
                     const float M0 = M == -INFINITY ? 0.0f : M;
-                    for (int x = lane; x < n; x += 32) {
-                        const float w = ex2(__ldcg(at(x) + row) - M0);
-                        wt[x * 16 + row] = w;
-                        L += w;
-                    }
+                    for (int x = lane; x < n; x += 32) L += ex2(__ldcg(at(x) + row) - M0);
                     L = warp_sum(L);
                     if (lane == 0) {
+                        s_m[0][row] = M0;
                         s_f[0][row] = L == 0.0f ? 0.0f : 1.0f / L;
                         s_row[row] = L == 0.0f ? -INFINITY : M0 + log2f(L);
                     }
                 }
                 __syncthreads();
-                for (int i = tid; i < nrow * c.hd; i += GD_THREADS) {
-                    const int row = i / c.hd, d = i - row * c.hd;
+                for (int i = tid; i < g.nrow * HDP; i += GD_THREADS) {
+                    const int row = i / HDP, d = i % HDP;
+                    const float M0 = s_m[0][row];
                     float o = 0.0f;
-#pragma unroll 4
-                    for (int x = 0; x < n; x++) o += __ldcg(at(x) + 16 + row * HDP + d) * wt[x * 16 + row];
-                    ((T *)a.out)[((long long)b * a.H + h0 + row) * c.hd + d] = from_f<T>(o * s_f[0][row]);
+#pragma unroll 8
+                    for (int x = 0; x < n; x++) o += __ldcg(at(x) + 16 + i) * ex2(__ldcg(at(x) + row) - M0);
+                    if (d < c.hd) ((T *)a.out)[(row_out + row) * c.hd + d] = from_f<T>(o * s_f[0][row]);
                 }
-                if (tid < nrow && a.lse) a.lse[(long long)b * a.H + h0 + tid] = s_row[tid] * 0.6931471805599453f;
+                if (tid < g.nrow && a.lse) a.lse[row_out + tid] = s_row[tid] * 0.6931471805599453f;
             }
         }
-        __syncthreads();  // shared memory is free for the next item
-        u += ub - ua;
-        if (rel + (ub - ua) == (long long)U * ips) {
-            pref += (long long)U * ips;
-            b++;
-        }
+        if (!more) return;
+        __syncthreads();  // the join's stages are free
+        cnt = hcnt;
     }
 }
 
 static int gd_grid(const GqaCacheArgs &c, int H, int sm_count, int ctas) {
     const int G = H / c.Hkv;
-    const long long most = (long long)c.n_seq * c.Hkv * ((G + 15) / 16) * c.max_pages * (WB_PAGE / GD_UNIT);
+    const long long most = (long long)c.n_seq * c.Hkv * ((G + 15) / 16) * (c.max_pages * (WB_PAGE / GD_UNIT) + GD_ITEM);
     return (int)std::max(1LL, std::min(most, (long long)std::min(sm_count, 148) * ctas));
 }
 
@@ -599,18 +739,24 @@ size_t gqa_decode_scratch(const GqaCacheArgs &c, int H, int sm_count) {
     return (size_t)gd_grid(c, H, sm_count, 4) * 2 * gqa_piece(c.hd <= 64 ? 64 : 128) * sizeof(float);
 }
 
-template <class T, int KIND, int HDP>
-static int gd_launch(const GqaDecodeArgs &a, int sm_count, cudaStream_t st, std::string *msg) {
+template <class T, int KIND, int HDP, bool FULL>
+static int gd_launch_as(const GqaDecodeArgs &a, int sm_count, cudaStream_t st, std::string *msg) {
     using F = GdConf<KIND, HDP>;
     static const cudaError_t set =
-        cudaFuncSetAttribute(gqa_decode_kernel<T, KIND, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES);
+        cudaFuncSetAttribute(gqa_decode_kernel<T, KIND, HDP, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES);
     if (set != cudaSuccess) {
         *msg = std::string("decode kernel attributes: ") + cudaGetErrorString(set);
         return WB_ECUDA;
     }
     ProfScope ps("gqa_decode", st);
-    gqa_decode_kernel<T, KIND, HDP><<<gd_grid(a.c, a.H, sm_count, F::CTAS), GD_THREADS, F::BYTES, st>>>(a);
+    gqa_decode_kernel<T, KIND, HDP, FULL><<<gd_grid(a.c, a.H, sm_count, F::CTAS), GD_THREADS, F::BYTES, st>>>(a);
     return WB_OK;
+}
+
+template <class T, int KIND, int HDP>
+static int gd_launch(const GqaDecodeArgs &a, int sm_count, cudaStream_t st, std::string *msg) {
+    return a.c.row == HDP ? gd_launch_as<T, KIND, HDP, true>(a, sm_count, st, msg)
+                          : gd_launch_as<T, KIND, HDP, false>(a, sm_count, st, msg);
 }
 
 int launch_gqa_decode(const GqaCacheArgs &c, int dtype, int H, const void *q, long long q_ss, long long q_hs,
