@@ -38,6 +38,7 @@
 #include "wb_ptx.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace wb {
 
@@ -58,7 +59,6 @@ static constexpr int GD_UNIT = 64;      // keys per unit: one 16-key block for e
 static constexpr int GD_ITEM = 2;       // what an item's start and end cost, in units of the line
 static constexpr int GD_SEQS = 256;     // sequences of a CTA's share whose lengths it holds in shared memory
 static constexpr float GD_SHIFT = 8.0f; // weights are kept as 2^8 exp2(s - m): see above
-static constexpr float GD_MOST = 16384.0f;  // largest weight before m follows the maximum (fp16 ends at 65504)
 
 enum { GD_NATIVE = 0, GD_INT8 = 1, GD_E4M3 = 2 };
 
@@ -98,9 +98,11 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 }
 
 // 16 bytes global -> shared, the bytes past n (0 or 16) as zeros
-__device__ __forceinline__ void cp_async16_or_zero(void *dst, const void *src, int n) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(n)
-                 : "memory");
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf) {
@@ -285,28 +287,34 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
     uint8_t *ring = sm + warp * (NST * F::STAGE);
     // FULL: rows of HDP values, so that a block's offsets are constants
     const int rowb = FULL ? F::RB : c.row * F::ESZ;
-    // this lane's pieces of a block: ch of rows lr, lr + STEP, ..  Piece
-    // positions within each 128 bytes of the ring: K's by row parity, V's by
-    // row pair, so that the fragments' reads touch every bank once.
+    // This lane's pieces of a block: ch of rows lr, lr + STEP, ..  Piece
+    // positions within each 128 bytes of the ring are permuted, K's by row
+    // parity and V's by row pair, so that the fragments' reads touch every
+    // bank once; all of a lane's places are one base and constants.
     constexpr int STEP = 32 / F::CPR;
     const int ch = lane % F::CPR, lr = lane / F::CPR;
     const bool col = FULL || ch * 16 < rowb;
     const uint32_t src0 = lr * rowb + ch * 16;
-    auto ring_at = [&](int rr, int ch, bool v) {
+    const uint32_t ring0 = ptx::smem_u32(ring);
+    auto place = [&](int rr, int ch, int sw) {
         const int pos = (F::RB == 64 ? (rr & 1) * 4 : 0) + ch;
-        const int line = rr * F::RB / 128 + (F::RB == 256 ? ch / 8 : 0);
-        const int sw = v ? ((rr >> 1) & 3) << 1 : F::RB == 64 ? 0 : (rr & 1) << 2;
-        return line * 128 + (((pos & 7) ^ sw) << 4);
+        return (uint32_t)((rr * F::RB / 128 + (F::RB == 256 ? ch / 8 : 0)) * 128 + (((pos & 7) ^ sw) << 4));
     };
+    const uint32_t kdst = place(lr, ch, F::RB == 64 ? 0 : (lr & 1) << 2);  // row lr + x STEP: + 512 x
+    const uint32_t vdst = 16 * F::RB + place(lr, ch, ((lr >> 1) & 3) << 1);  // and ^ v_flip(x)
+    auto v_flip = [](int x) { return (uint32_t)(F::RB == 64 ? 0 : F::RB == 128 ? (x & 1) * 64 : (x & 3) * 32); };
+    // reads: piece cc of row r, and of rows 2cc (piece r) for the values
+    const uint32_t krd = place(r, cc, F::RB == 64 ? 0 : (r & 1) << 2);
+    const uint32_t vrd = 16 * F::RB + (F::RB == 64 ? place(2 * cc, r >> 1, cc << 1) + (r & 1) * 8 : place(2 * cc, r, cc << 1));
 
     // ---- loads of a part's blocks: this warp's are keys k0 + 16 (warp + 4 i)
     int pbase = 0, pid = -1;  // page ids of pages pbase + lane of the part
     auto pages_of = [&](const GdSeg &g, int p) {
         return p + lane <= (g.k1 - 1) >> WB_PAGE_SHIFT ? __ldg(c.table + (long long)g.slot * c.max_pages + p + lane) : -1;
     };
+    auto key_of = [&](int k0, int i) { return k0 + 16 * (warp + GD_WARPS * i); };
     auto blocks_of = [&](const GdSeg &g) { return (((g.k1 - g.k0 + 15) >> 4) - warp + GD_WARPS - 1) / GD_WARPS; };
-    auto issue = [&](const GdSeg &g, int i, int stage) {
-        const int key0 = g.k0 + 16 * (warp + GD_WARPS * i);
+    auto issue = [&](const GdSeg &g, int key0, int kend, int stage) {
         const int p = key0 >> WB_PAGE_SHIFT;
         if (p >= pbase + 32) {
             pbase = p;
@@ -315,29 +323,27 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
         const int pg = __shfl_sync(0xffffffffu, pid, p - pbase);
         const bool ok = pg >= 0 && pg < c.n_pages;
         const long long row0 = ok ? ((long long)pg * c.Hkv + g.hk) * WB_PAGE + (key0 & (WB_PAGE - 1)) : 0;
-        uint8_t *st = ring + stage * F::STAGE;
-        const uint8_t *kp = (const uint8_t *)c.k_pages + row0 * rowb, *vp = (const uint8_t *)c.v_pages + row0 * rowb;
-        if (ok && key0 + 16 <= g.k1) {
+        const uint32_t st = ring0 + stage * F::STAGE;
+        const uint8_t *kp = (const uint8_t *)c.k_pages + row0 * rowb + src0, *vp = (const uint8_t *)c.v_pages + row0 * rowb + src0;
+        if (ok && key0 + 16 <= kend) {
 #pragma unroll
             for (int x = 0; x < F::CPR / 2; x++) {
-                const int rr = lr + x * STEP;
+                const uint32_t kd = st + kdst + 512 * x, vd = st + (vdst ^ v_flip(x)) + 512 * x;
                 if (FULL) {
-                    ptx::cp_async<16>(st + ring_at(rr, ch, false), kp + src0 + x * STEP * F::RB);
-                    ptx::cp_async<16>(st + 16 * F::RB + ring_at(rr, ch, true), vp + src0 + x * STEP * F::RB);
+                    cp_async16(kd, kp + x * STEP * F::RB);
+                    cp_async16(vd, vp + x * STEP * F::RB);
                 } else {
-                    const uint32_t off = col ? src0 + x * STEP * rowb : 0;
-                    cp_async16_or_zero(st + ring_at(rr, ch, false), kp + off, col ? 16 : 0);
-                    cp_async16_or_zero(st + 16 * F::RB + ring_at(rr, ch, true), vp + off, col ? 16 : 0);
+                    cp_async16_or_zero(kd, col ? kp + x * STEP * rowb : kp, col ? 16 : 0);
+                    cp_async16_or_zero(vd, col ? vp + x * STEP * rowb : vp, col ? 16 : 0);
                 }
             }
         } else {
 #pragma unroll 1
             for (int x = 0; x < F::CPR / 2; x++) {
-                const int rr = lr + x * STEP;
-                const int n = ok && col && key0 + rr < g.k1 ? 16 : 0;
-                const uint32_t off = n ? src0 + x * STEP * rowb : 0;
-                cp_async16_or_zero(st + ring_at(rr, ch, false), kp + off, n);
-                cp_async16_or_zero(st + 16 * F::RB + ring_at(rr, ch, true), vp + off, n);
+                const int n = ok && col && key0 + lr + x * STEP < kend ? 16 : 0;
+                const long long o = n ? (long long)x * STEP * rowb : -(long long)src0;
+                cp_async16_or_zero(st + kdst + 512 * x, kp + o, n);
+                cp_async16_or_zero(st + (vdst ^ v_flip(x)) + 512 * x, vp + o, n);
             }
         }
         if (QUANT && lane < 8) {
@@ -384,7 +390,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
     uint32_t okbits = 0;  // bit of a stage: its block's page is mapped
 #pragma unroll
     for (int i = 0; i < NST - MST; i++) {
-        if (i < cnt && issue(s_seg[0], i, i)) okbits |= 1u << i;
+        if (i < cnt && issue(s_seg[0], key_of(s_seg[0].k0, i), s_seg[0].k1, i)) okbits |= 1u << i;
         ptx::cp_async_commit();
     }
     for (int part = 0;; part++) {
@@ -394,7 +400,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
         for (int i = NST - MST; i < NST - 1; i++) {
             const int sg = (stage + i) % NST;
             okbits &= ~(1u << sg);
-            if (i < cnt && issue(g, i, sg)) okbits |= 1u << sg;
+            if (i < cnt && issue(g, key_of(g.k0, i), g.k1, sg)) okbits |= 1u << sg;
             ptx::cp_async_commit();
         }
         // the next part's page ids, long before they are needed
@@ -437,29 +443,16 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
         float off[2] = {1e30f, 1e30f}, e2[2] = {1.0f, 1.0f};  // 8 - m, 2^(m - m2)
         bool unmapped = false;
 
-        int stg = stage, nxs = (stage + NST - 1) % NST;
-        const int kbeg = g.k0, kend = g.k1;
-        for (int i = 0; i < cnt; i++) {
-            ptx::cp_async_wait<NST - 2>();
-            __syncwarp();
-            const bool ok = (okbits >> stg) & 1;
-            okbits &= ~(1u << nxs);
-            if (i + NST - 1 < cnt && issue(g, i + NST - 1, nxs)) okbits |= 1u << nxs;
-            ptx::cp_async_commit();
-            const uint8_t *st = ring + stg * F::STAGE;
-            const int key0 = kbeg + 16 * (warp + GD_WARPS * i);
-            const int k1 = kend;
-            nxs = stg;
-            if (++stg == NST) stg = 0;
-
+        auto block = [&](const uint8_t *st, int n, auto tail) {
+            constexpr bool TAIL = decltype(tail)::value;
             // scores of keys 0-7 (s[0]) and 8-15 (s[1])
             float s[2][4] = {};
 #pragma unroll
             for (int g = 0; g < 2; g++) {
-                const int rr = r + 8 * g;
 #pragma unroll
                 for (int x = 0; x < F::CPR / 4; x++) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(st + ring_at(rr, cc + 4 * x, false));
+                    const uint4 w = *reinterpret_cast<const uint4 *>(
+                        st + (krd ^ (x & 1) * 64) + (x >> 1) * 128 + g * 8 * F::RB);
                     if constexpr (QUANT) {
                         mma16816<BF>(s[g], qf[4 * x], to_f16x2<KIND, 0>(w.x), to_f16x2<KIND, 1>(w.x));
                         mma16816<BF>(s[g], qf[4 * x + 1], to_f16x2<KIND, 0>(w.y), to_f16x2<KIND, 1>(w.y));
@@ -486,31 +479,39 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                     vs[g][1] = v2.y;
                 }
             }
-            // keys past the end or on an unmapped page
-            const bool tail = !ok || key0 + 16 > k1;
-            auto dead = [&](int g, int e) { return tail && (!ok || key0 + 2 * cc + 8 * g + e >= k1); };
-            unmapped |= !ok;
-            float pr[2][4], wr[2][4];
+            // weights of the part's first n keys (all 16 unless TAIL)
+            auto dead = [&](int g, int e) { return TAIL && 2 * cc + 8 * g + e >= n; };
+            float pr[2][4];
+            uint32_t pf[4];
+            float ps[2];  // sums of the rows' weights
             auto weigh = [&]() {
-                float top = 0.0f;
 #pragma unroll
-                for (int g = 0; g < 2; g++)
+                for (int hf = 0; hf < 2; hf++) {
 #pragma unroll
-                    for (int hf = 0; hf < 2; hf++)
+                    for (int g = 0; g < 2; g++) {
+                        float w[2];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            const int i4 = 2 * hf + e;
-                            pr[g][i4] = ex2(fmaf(s[g][i4], fac[hf], off[hf]));
-                            if (QUANT) wr[g][i4] = pr[g][i4] * (vs[g][e] * e2[hf]);
-                            if (tail && dead(g, e)) pr[g][i4] = wr[g][i4] = 0.0f;
-                            top = fmaxf(top, pr[g][i4]);
-                            if (QUANT) top = fmaxf(top, wr[g][i4]);
+                            float &p = pr[g][2 * hf + e];
+                            p = ex2(fmaf(s[g][2 * hf + e], fac[hf], off[hf]));
+                            w[e] = QUANT ? p * vs[g][e] * e2[hf] : p;  // in this order 0 stays 0
+                            if (dead(g, e)) p = w[e] = 0.0f;
                         }
-                return top;
+                        pf[2 * g + hf] = pack2(w[0], w[1], BF);
+                    }
+                    ps[hf] = (pr[0][2 * hf] + pr[0][2 * hf + 1]) + (pr[1][2 * hf] + pr[1][2 * hf + 1]);
+                }
+                // a weight above 2^14 (fp16), or sums that could leave fp32's range
+                bool far = ps[0] + ps[1] > 1.8e19f;
+                if (!BF) {
+                    auto h2 = [](uint32_t x) { return *reinterpret_cast<const __half2 *>(&x); };
+                    const __half2 top = __hmax2(__hmax2(h2(pf[0]), h2(pf[1])), __hmax2(h2(pf[2]), h2(pf[3])));
+                    far |= __hgt2_mask(top, __half2half2(__ushort_as_half(0x7400))) != 0;
+                }
+                return far;
             };
-            // The references m, m2 stay until a weight passes 2^14; then they
-            // follow the maxima.
-            if (__any_sync(0xffffffffu, !(weigh() <= GD_MOST))) {
+            // The references m, m2 stay until then; then they follow the maxima.
+            if (__any_sync(0xffffffffu, weigh())) {
                 float f2[2];
 #pragma unroll
                 for (int hf = 0; hf < 2; hf++) {
@@ -541,31 +542,29 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                 }
                 weigh();
             }
-            uint32_t pf[4], pl[4];
+            l[0] += ps[0];
+            l[1] += ps[1];
+            uint32_t pl[4];
+            if (BF) {
 #pragma unroll
-            for (int g = 0; g < 2; g++)
+                for (int g = 0; g < 2; g++)
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++) {
-                    const float p0 = pr[g][2 * hf], p1 = pr[g][2 * hf + 1];
-                    l[hf] += p0 + p1;
-                    pf[2 * g + hf] = QUANT ? pack2(wr[g][2 * hf], wr[g][2 * hf + 1], BF) : pack2(p0, p1, BF);
-                    if (BF) {
+                    for (int hf = 0; hf < 2; hf++) {
                         const uint32_t x = pf[2 * g + hf];
-                        pl[2 * g + hf] = pack2(p0 - __uint_as_float(x << 16), p1 - __uint_as_float(x & 0xffff0000u), BF);
+                        pl[2 * g + hf] = pack2(pr[g][2 * hf] - __uint_as_float(x << 16),
+                                               pr[g][2 * hf + 1] - __uint_as_float(x & 0xffff0000u), BF);
                     }
-                }
+            }
 
             // values: piece r of rows 2cc, 2cc+1, 2cc+8, 2cc+9
-            const uint8_t *sv = st + 16 * F::RB;
+            const uint8_t *sv = st + vrd;
             if constexpr (F::ESZ == 2) {
 #pragma unroll
                 for (int x = 0; x < HDP / 64; x++) {
                     uint4 w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const int rr = 2 * cc + (e & 1) + 8 * (e >> 1);
-                        w[e] = *reinterpret_cast<const uint4 *>(sv + (rr * F::RB / 128 + x) * 128 +
-                                                                ((r ^ (((rr >> 1) & 3) << 1)) * 16));
+                        w[e] = *reinterpret_cast<const uint4 *>(sv + ((e & 1) + 8 * (e >> 1)) * F::RB + x * 128);
                     }
                     const uint32_t *w0 = &w[0].x, *w1 = &w[1].x, *w2 = &w[2].x, *w3 = &w[3].x;
 #pragma unroll
@@ -584,13 +583,11 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                 uint32_t w[4][HDP / 32];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int rr = 2 * cc + (e & 1) + 8 * (e >> 1);
                     if constexpr (HDP == 128) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(sv + rr * 128 + ((r ^ (((rr >> 1) & 3) << 1)) * 16));
+                        const uint4 v = *reinterpret_cast<const uint4 *>(sv + ((e & 1) + 8 * (e >> 1)) * 128);
                         w[e][0] = v.x; w[e][1] = v.y; w[e][2] = v.z; w[e][3] = v.w;
                     } else {
-                        const int pos = ((rr & 1) * 4 + (r >> 1)) ^ (((rr >> 1) & 3) << 1);
-                        const uint2 v = *reinterpret_cast<const uint2 *>(sv + (rr >> 1) * 128 + pos * 16 + (r & 1) * 8);
+                        const uint2 v = *reinterpret_cast<const uint2 *>(st + (vrd ^ (e & 1) * 64) + (e >> 1) * 512);
                         w[e][0] = v.x; w[e][1] = v.y;
                     }
                 }
@@ -604,6 +601,27 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                     mma16816<BF>(acc[4 * d + 2], pf, to_f16x2<KIND, 0>(a23), to_f16x2<KIND, 0>(b23));
                     mma16816<BF>(acc[4 * d + 3], pf, to_f16x2<KIND, 1>(a23), to_f16x2<KIND, 1>(b23));
                 }
+            }
+        };
+
+        int stg = stage, nxs = (stage + NST - 1) % NST;
+        const int kbeg = g.k0, kend = g.k1;
+        for (int i = 0; i < cnt; i++) {
+            ptx::cp_async_wait<NST - 2>();
+            __syncwarp();
+            const bool ok = (okbits >> stg) & 1;
+            okbits &= ~(1u << nxs);
+            if (i + NST - 1 < cnt && issue(g, key_of(kbeg, i + NST - 1), kend, nxs)) okbits |= 1u << nxs;
+            ptx::cp_async_commit();
+            const uint8_t *st = ring + stg * F::STAGE;
+            const int key0 = key_of(kbeg, i);
+            nxs = stg;
+            if (++stg == NST) stg = 0;
+            if (ok && key0 + 16 <= kend) {
+                block(st, 16, std::false_type{});
+            } else {
+                unmapped |= !ok;
+                block(st, ok ? kend - key0 : 0, std::true_type{});
             }
         }
         // every block of the part has been read: the next part's first loads
@@ -619,7 +637,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
 #pragma unroll
             for (int i = 0; i < NST - MST; i++) {
                 const int sg = (stage + i) % NST;
-                if (i < hcnt && issue(h, i, sg)) okbits |= 1u << sg;
+                if (i < hcnt && issue(h, key_of(h.k0, i), h.k1, sg)) okbits |= 1u << sg;
                 ptx::cp_async_commit();
             }
             load_q(h);
