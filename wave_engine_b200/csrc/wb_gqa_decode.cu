@@ -5,7 +5,7 @@
 //
 // The call reads every cached K and V byte once and does little else with
 // it, so HBM bounds it.  All of the batch's keys are one line of 64-key
-// units (sequence, key-value head, group of 16 query heads, length), which
+// units (sequence, key-value head, 8 or 16 query heads, length), which
 // the CTAs of one resident wave share out evenly; a CTA's share may begin
 // and end inside an item, and the last CTA to finish an item joins its
 // pieces in the order of the keys (same bits every run).
@@ -13,18 +13,21 @@
 // In a CTA each of four warps takes every fourth 16-key block, with its own
 // running maximum, sum and output, through its own shared-memory ring filled
 // by cp.async; the four join at the end of the item.  The products run on
-// mma.sync m16n8k16 with the (up to 16) query heads of one key-value head as
-// the rows: each K and V byte is converted once for all of them.  tcgen05
-// would need every block converted to 16 bits and written back to shared
-// memory first, and its 128 rows would be mostly padding.
+// mma.sync m16n8k16 with the keys (then the dims) as the 16 rows and 8 query
+// heads of one key-value head as the columns, so each K and V byte is
+// converted once for all of them, and a group of 4 to 8 heads fills the
+// columns that it would half fill as rows.  tcgen05 would need every block
+// converted to 16 bits and written back to shared memory first, and its 128
+// rows would be mostly padding.
 //
-// Fragments without any transposition: the dims of q . k and the columns of
-// p v may be taken in any order as long as both sides use the same one, so
-//   - lane (r = lane / 4, c = lane % 4) feeds q . k with whole 16-byte
-//     pieces c, c + 4, .. of key r's row (and of key r + 8's), and
-//   - feeds p v with piece r of the rows of keys 2c, 2c+1, 2c+8, 2c+9, one
-//     product per dim of the piece -- the keys whose probabilities the lane
-//     already holds.
+// Fragments without any transposition of K or V: the dims of q . k and the
+// rows of v^T p may be taken in any order as long as both sides use the same
+// one, so
+//   - lane (r = lane / 4, cc = lane % 4) feeds k . q with whole 16-byte
+//     pieces cc, cc + 4, .. of the rows of keys r and r + 8, and
+//   - feeds v^T p with piece r of the rows of keys 2cc, 2cc+1, 2cc+8, 2cc+9,
+//     two of the piece's dims per product.
+// Only the 16 x 8 probabilities change sides (movmatrix).
 // 8-bit values become fp16 exactly (e4m3 by cvt, int8 by exponent insertion
 // and a subtraction); the K scale multiplies the finished score.  The V
 // scale joins the weight, w_j = p_j vscale_j 2^(m - m2), where m2 is a running
@@ -62,22 +65,23 @@ static constexpr float GD_SHIFT = 8.0f; // weights are kept as 2^8 exp2(s - m): 
 
 enum { GD_NATIVE = 0, GD_INT8 = 1, GD_E4M3 = 2 };
 
-// CTAs per SM and ring depth: three CTAs of 168 registers at 128 columns
-// (64 output + 32 query registers a thread), four at 64; the ring takes what
-// shared memory leaves.
-template <int KIND, int HDP>
+// CTAs per SM and ring depth: what registers (HDP / 4 NB output and HDP / 8
+// NB query registers a thread) and shared memory leave.
+template <int KIND, int HDP, int NB>
 struct GdConf {
     static constexpr int ESZ = KIND == GD_NATIVE ? 2 : 1;
     static constexpr int RB = HDP * ESZ;  // ring bytes of a row
     static constexpr int CPR = RB / 16;   // 16-byte pieces of a row
     static constexpr int SCALES = KIND == GD_NATIVE ? 0 : 128;
     static constexpr int STAGE = 2 * 16 * RB + SCALES;
-    static constexpr int CTAS = HDP == 64 ? 4 : (ESZ == 2 ? 2 : 3);
-    static constexpr int NST = HDP == 64 ? (ESZ == 2 ? 3 : 6) : (ESZ == 2 ? 3 : 4);
-    static constexpr int MST = 16 * HDP * 4 > STAGE ? 2 : 1;  // stages that hold a warp's 16 output rows
+    static constexpr int CTAS = NB == 1 ? (HDP == 64 || ESZ == 1 ? 4 : 2) : (HDP == 64 ? 4 : ESZ == 1 ? 3 : 2);
+    static constexpr int NST = HDP == 64 ? (ESZ == 2 ? 3 : 5) : (ESZ == 2 ? 3 : NB == 1 ? 3 : 4);
+    static constexpr int ROWS = 8 * NB;  // heads of an item
+    static constexpr int MST = (ROWS * HDP * 4 + STAGE - 1) / STAGE;  // stages that hold a warp's outputs
+    static constexpr int MROWS = ROWS / MST;
     static constexpr int BYTES = GD_WARPS * NST * STAGE;
     static_assert((BYTES + 4096) * CTAS <= 227 * 1024, "shared memory of the resident CTAs");
-    static_assert(16 * HDP * 4 <= MST * STAGE && NST - MST >= 1, "the join uses the ring");
+    static_assert(MROWS * MST == ROWS && MROWS * HDP * 4 <= STAGE && NST - MST >= 1, "the join uses the ring");
 };
 
 // Floats of one piece: 16 rows' log2 sum exp, then 16 rows of HDP values
@@ -138,13 +142,23 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float quad_max(float v) {
-    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+// over the 8 lanes of one cc
+__device__ __forceinline__ float oct_max(float v) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
 }
-__device__ __forceinline__ float quad_sum(float v) {
-    v += __shfl_xor_sync(0xffffffffu, v, 1);
-    return v + __shfl_xor_sync(0xffffffffu, v, 2);
+__device__ __forceinline__ float oct_sum(float v) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// 8 x 8 16-bit values: lane (r, cc) gives row r's columns 2cc, 2cc+1 and gets
+// column r's rows 2cc, 2cc+1
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 // The sequence's slot and length; a slot or length that does not fit counts
@@ -166,13 +180,14 @@ struct GdSeg {
     long long first, last;  // the item's first and last unit on the line
 };
 
-template <class T, int KIND, int HDP, bool FULL>
-__global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decode_kernel(GqaDecodeArgs a) {
-    using F = GdConf<KIND, HDP>;
+template <class T, int KIND, int HDP, int NB, bool FULL>
+__global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_decode_kernel(GqaDecodeArgs a) {
+    using F = GdConf<KIND, HDP, NB>;
     constexpr bool BF = KIND == GD_NATIVE && __is_same(T, __nv_bfloat16);  // product type
     constexpr bool QUANT = KIND != GD_NATIVE;
-    constexpr int NK = HDP / 16;  // q . k products per 8 keys
-    constexpr int NV = HDP / 8;   // p v products per 16 keys
+    constexpr int NK = HDP / 16;  // products of 16 keys and 8 heads over the dims ..
+    constexpr int NV = HDP / 16;  // .. and over the keys
+    constexpr int ROWS = F::ROWS;
     constexpr int NST = F::NST, MST = F::MST;
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ long long s_scan[GD_WARPS];
@@ -184,7 +199,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
     __shared__ int s_last, s_stage[GD_WARPS];
     const GqaCacheArgs &c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, cc = lane & 3;
-    const int G = a.H / c.Hkv, nch = (G + 15) / 16, ips = c.Hkv * nch;  // items of a sequence
+    const int G = a.H / c.Hkv, nch = (G + ROWS - 1) / ROWS, ips = c.Hkv * nch;  // items of a sequence
 
     // ---- the line of units and this CTA's share s0 .. s1-1
     auto line_len = [&](int n) { return n == 0 ? 0LL : (long long)((n + GD_UNIT - 1) / GD_UNIT + GD_ITEM) * ips; };
@@ -262,8 +277,8 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
             g.slot = slot;
             g.hk = item / nch;
             const int hc = item - g.hk * nch;
-            g.h0 = g.hk * G + hc * 16;
-            g.nrow = min(16, G - hc * 16);
+            g.h0 = g.hk * G + hc * ROWS;
+            g.nrow = min(ROWS, G - hc * ROWS);
             g.U = U;
             g.ua = max(0, o0 - GD_ITEM);
             g.ub = o1 - GD_ITEM;
@@ -352,14 +367,14 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
         }
         return ok;
     };
-    // a part's queries as loaded: rows r and r + 8, dims in the order of K's pieces
+    // a part's queries as loaded: head r of each eight, dims in the order of K's pieces
     const bool q8 = ((a.q_ss | a.q_hs | c.hd) & 3) == 0 && (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
     auto q_dim = [&](int t) { return F::ESZ == 1 ? 16 * (cc + 4 * (t / 4)) + 4 * (t % 4) : 8 * (cc + 4 * (t / 2)) + 4 * (t % 2); };
-    uint32_t qf[NK][4];
+    uint32_t qf[NB][NK][2];
     auto load_q = [&](const GdSeg &g) {
 #pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-            const int row = r + 8 * hf;
+        for (int nb = 0; nb < NB; nb++) {
+            const int row = r + 8 * nb;
             const uint16_t *qp = (const uint16_t *)a.q + g.b * a.q_ss + (long long)(g.h0 + row) * a.q_hs;
 #pragma unroll
             for (int t = 0; t < NK; t++) {
@@ -375,8 +390,8 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                         w = make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
                     }
                 }
-                qf[t][hf] = w.x;
-                qf[t][2 + hf] = w.y;
+                qf[nb][t][0] = w.x;
+                qf[nb][t][1] = w.y;
             }
         }
     };
@@ -407,177 +422,188 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
         const bool more = h.U != 0;
         const int hpid = more ? pages_of(h, h.k0 >> WB_PAGE_SHIFT) : -1;
 
-        float fac[2];  // score factor of the two rows, log2 e included
-        fac[0] = fac[1] = a.scale * 1.4426950408889634f;
-        if (QUANT && !__is_same(T, __half)) {
-            // bf16 queries meet fp16 keys: divided by a power of two so that
-            // the row's largest is in [1, 2) (exact down to 2^-14 of it)
+        float fac[NB][2];  // score factors of heads 2cc, 2cc+1, log2 e included
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
+        for (int nb = 0; nb < NB; nb++) {
+            float f = a.scale * 1.4426950408889634f;
+            if (QUANT && !__is_same(T, __half)) {
+                // bf16 queries meet fp16 keys: divided by a power of two so
+                // that the head's largest is in [1, 2) (exact down to 2^-14
+                // of it)
                 uint32_t top = 0;
 #pragma unroll
                 for (int t = 0; t < NK; t++)
 #pragma unroll
                     for (int e = 0; e < 2; e++)
-                        top = max(top, max((qf[t][2 * e + hf] << 16) & 0x7fffffffu, qf[t][2 * e + hf] & 0x7fff0000u));
+                        top = max(top, max((qf[nb][t][e] << 16) & 0x7fffffffu, qf[nb][t][e] & 0x7fff0000u));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = min(max((int)(top >> 23), 1), 253);
-                const float f = __uint_as_float((uint32_t)(254 - e) << 23);
-                fac[hf] *= __uint_as_float((uint32_t)e << 23);
+                const int e2 = min(max((int)(top >> 23), 1), 253);
+                const float down = __uint_as_float((uint32_t)(254 - e2) << 23);
+                f *= __uint_as_float((uint32_t)e2 << 23);
 #pragma unroll
                 for (int t = 0; t < NK; t++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const uint32_t x = qf[t][2 * e + hf];
-                        qf[t][2 * e + hf] = pack2(__uint_as_float(x << 16) * f, __uint_as_float(x & 0xffff0000u) * f, false);
+                        const uint32_t x = qf[nb][t][e];
+                        qf[nb][t][e] = pack2(__uint_as_float(x << 16) * down, __uint_as_float(x & 0xffff0000u) * down, false);
                     }
             }
+            fac[nb][0] = __shfl_sync(0xffffffffu, f, 8 * cc);
+            fac[nb][1] = __shfl_sync(0xffffffffu, f, 8 * cc + 4);
         }
 
-        float acc[NV][4];
-#pragma unroll
-        for (int j = 0; j < NV; j++) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+        // acc[nb][j]: dims of piece r (two per product), heads 2cc, 2cc+1
+        float acc[NB][NV][4] = {};
         // finite stand-ins for -inf: the first visible score replaces them
-        float m[2] = {-1e30f, -1e30f}, m2[2] = {-1e30f, -1e30f}, l[2] = {0.0f, 0.0f};
-        float off[2] = {1e30f, 1e30f}, e2[2] = {1.0f, 1.0f};  // 8 - m, 2^(m - m2)
+        float m[NB][2], m2[NB][2], l[NB][2], off[NB][2], e2[NB][2];  // off = 8 - m, e2 = 2^(m - m2)
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                m[nb][e] = m2[nb][e] = -1e30f;
+                l[nb][e] = 0.0f;
+                off[nb][e] = 1e30f;
+                e2[nb][e] = 1.0f;
+            }
         bool unmapped = false;
 
         auto block = [&](const uint8_t *st, int n, auto tail) {
             constexpr bool TAIL = decltype(tail)::value;
-            // scores of keys 0-7 (s[0]) and 8-15 (s[1])
-            float s[2][4] = {};
+            // s[nb]: scores of keys r (heads 2cc, 2cc+1) and r + 8 (the same)
+            float s[NB][4] = {};
 #pragma unroll
-            for (int g = 0; g < 2; g++) {
+            for (int x = 0; x < F::CPR / 4; x++) {
+                const uint8_t *kr = st + (krd ^ (x & 1) * 64) + (x >> 1) * 128;
+                const uint4 w0 = *reinterpret_cast<const uint4 *>(kr), w1 = *reinterpret_cast<const uint4 *>(kr + 8 * F::RB);
+                const uint32_t k0[4] = {w0.x, w0.y, w0.z, w0.w}, k1[4] = {w1.x, w1.y, w1.z, w1.w};
+                if constexpr (QUANT) {
 #pragma unroll
-                for (int x = 0; x < F::CPR / 4; x++) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(
-                        st + (krd ^ (x & 1) * 64) + (x >> 1) * 128 + g * 8 * F::RB);
-                    if constexpr (QUANT) {
-                        mma16816<BF>(s[g], qf[4 * x], to_f16x2<KIND, 0>(w.x), to_f16x2<KIND, 1>(w.x));
-                        mma16816<BF>(s[g], qf[4 * x + 1], to_f16x2<KIND, 0>(w.y), to_f16x2<KIND, 1>(w.y));
-                        mma16816<BF>(s[g], qf[4 * x + 2], to_f16x2<KIND, 0>(w.z), to_f16x2<KIND, 1>(w.z));
-                        mma16816<BF>(s[g], qf[4 * x + 3], to_f16x2<KIND, 0>(w.w), to_f16x2<KIND, 1>(w.w));
-                    } else {
-                        mma16816<BF>(s[g], qf[2 * x], w.x, w.y);
-                        mma16816<BF>(s[g], qf[2 * x + 1], w.z, w.w);
+                    for (int t = 0; t < 4; t++) {
+                        const uint32_t kf[4] = {to_f16x2<KIND, 0>(k0[t]), to_f16x2<KIND, 0>(k1[t]),
+                                                to_f16x2<KIND, 1>(k0[t]), to_f16x2<KIND, 1>(k1[t])};
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++) mma16816<BF>(s[nb], kf, qf[nb][4 * x + t][0], qf[nb][4 * x + t][1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        const uint32_t kf[4] = {k0[2 * t], k1[2 * t], k0[2 * t + 1], k1[2 * t + 1]};
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++) mma16816<BF>(s[nb], kf, qf[nb][2 * x + t][0], qf[nb][2 * x + t][1]);
                     }
                 }
             }
-            // this lane's keys: 2cc, 2cc+1 (g = 0) and 2cc+8, 2cc+9 (g = 1)
-            float vs[2][2];
+            float vs[2] = {1.0f, 1.0f};
+            if (QUANT) {
+                const float *sc = reinterpret_cast<const float *>(st + 32 * F::RB) + r;
+                vs[0] = sc[16];
+                vs[1] = sc[24];
 #pragma unroll
-            for (int g = 0; g < 2; g++) {
-                if (QUANT) {
-                    const float2 ks = *reinterpret_cast<const float2 *>(st + 32 * F::RB + (2 * cc + 8 * g) * 4);
-                    const float2 v2 = *reinterpret_cast<const float2 *>(st + 32 * F::RB + 64 + (2 * cc + 8 * g) * 4);
-                    s[g][0] *= ks.x;
-                    s[g][1] *= ks.y;
-                    s[g][2] *= ks.x;
-                    s[g][3] *= ks.y;
-                    vs[g][0] = v2.x;
-                    vs[g][1] = v2.y;
-                }
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[nb][i] *= sc[8 * (i >> 1)];
             }
-            // weights of the part's first n keys (all 16 unless TAIL)
-            auto dead = [&](int g, int e) { return TAIL && 2 * cc + 8 * g + e >= n; };
-            float pr[2][4];
-            uint32_t pf[4];
-            float ps[2];  // sums of the rows' weights
+            // weights of the first n keys (all 16 unless TAIL)
+            float pr[NB][4];
+            uint32_t pf[NB][2];  // fp16 or bf16: key r, key r + 8
             auto weigh = [&]() {
+                float most = 0.0f;
+                __half2 top = __half2half2(__ushort_as_half(0));
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++) {
+                for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
                         float w[2];
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            float &p = pr[g][2 * hf + e];
-                            p = ex2(fmaf(s[g][2 * hf + e], fac[hf], off[hf]));
-                            w[e] = QUANT ? p * vs[g][e] * e2[hf] : p;  // in this order 0 stays 0
-                            if (dead(g, e)) p = w[e] = 0.0f;
+                            float &p = pr[nb][2 * g + e];
+                            p = ex2(fmaf(s[nb][2 * g + e], fac[nb][e], off[nb][e]));
+                            w[e] = QUANT ? p * vs[g] * e2[nb][e] : p;  // in this order 0 stays 0
+                            if (TAIL && r + 8 * g >= n) p = w[e] = 0.0f;
                         }
-                        pf[2 * g + hf] = pack2(w[0], w[1], BF);
+                        pf[nb][g] = pack2(w[0], w[1], BF);
+                        if (!BF) top = __hmax2(top, *reinterpret_cast<const __half2 *>(&pf[nb][g]));
+                        most += pr[nb][2 * g] + pr[nb][2 * g + 1];
                     }
-                    ps[hf] = (pr[0][2 * hf] + pr[0][2 * hf + 1]) + (pr[1][2 * hf] + pr[1][2 * hf + 1]);
                 }
                 // a weight above 2^14 (fp16), or sums that could leave fp32's range
-                bool far = ps[0] + ps[1] > 1.8e19f;
-                if (!BF) {
-                    auto h2 = [](uint32_t x) { return *reinterpret_cast<const __half2 *>(&x); };
-                    const __half2 top = __hmax2(__hmax2(h2(pf[0]), h2(pf[1])), __hmax2(h2(pf[2]), h2(pf[3])));
-                    far |= __hgt2_mask(top, __half2half2(__ushort_as_half(0x7400))) != 0;
-                }
+                bool far = most > 1.8e19f;
+                if (!BF) far |= __hgt2_mask(top, __half2half2(__ushort_as_half(0x7400))) != 0;
                 return far;
             };
             // The references m, m2 stay until then; then they follow the maxima.
             if (__any_sync(0xffffffffu, weigh())) {
-                float f2[2];
 #pragma unroll
-                for (int hf = 0; hf < 2; hf++) {
-                    float mx = -INFINITY, mx2 = -INFINITY;
+                for (int nb = 0; nb < NB; nb++) {
+                    float f2[2];
 #pragma unroll
-                    for (int g = 0; g < 2; g++)
+                    for (int e = 0; e < 2; e++) {
+                        float mx = -INFINITY, mx2 = -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            if (!dead(g, e)) {
-                                const float x = s[g][2 * hf + e] * fac[hf];
+                        for (int g = 0; g < 2; g++)
+                            if (!TAIL || r + 8 * g < n) {
+                                const float x = s[nb][2 * g + e] * fac[nb][e];
                                 mx = fmaxf(mx, x);
-                                if (QUANT) mx2 = fmaxf(mx2, x + lg2(vs[g][e]));
+                                if (QUANT) mx2 = fmaxf(mx2, x + lg2(vs[g]));
                             }
-                    const float mn = fmaxf(m[hf], quad_max(mx)), mn2 = QUANT ? fmaxf(m2[hf], quad_max(mx2)) : mn;
-                    l[hf] *= ex2(m[hf] - mn);
-                    f2[hf] = ex2(m2[hf] - mn2);
-                    m[hf] = mn;
-                    m2[hf] = mn2;
-                    off[hf] = GD_SHIFT - mn;
-                    if (QUANT) e2[hf] = ex2(mn - mn2);
-                }
+                        const float mn = fmaxf(m[nb][e], oct_max(mx)), mn2 = QUANT ? fmaxf(m2[nb][e], oct_max(mx2)) : mn;
+                        l[nb][e] *= ex2(m[nb][e] - mn);
+                        f2[e] = ex2(m2[nb][e] - mn2);
+                        m[nb][e] = mn;
+                        m2[nb][e] = mn2;
+                        off[nb][e] = GD_SHIFT - mn;
+                        if (QUANT) e2[nb][e] = ex2(mn - mn2);
+                    }
 #pragma unroll
-                for (int j = 0; j < NV; j++) {
-                    acc[j][0] *= f2[0];
-                    acc[j][1] *= f2[0];
-                    acc[j][2] *= f2[1];
-                    acc[j][3] *= f2[1];
+                    for (int j = 0; j < NV; j++) {
+                        acc[nb][j][0] *= f2[0];
+                        acc[nb][j][1] *= f2[1];
+                        acc[nb][j][2] *= f2[0];
+                        acc[nb][j][3] *= f2[1];
+                    }
                 }
                 weigh();
             }
-            l[0] += ps[0];
-            l[1] += ps[1];
-            uint32_t pl[4];
-            if (BF) {
+            uint32_t pl[NB][2];
 #pragma unroll
-                for (int g = 0; g < 2; g++)
+            for (int nb = 0; nb < NB; nb++) {
+                l[nb][0] += pr[nb][0] + pr[nb][2];
+                l[nb][1] += pr[nb][1] + pr[nb][3];
 #pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {
-                        const uint32_t x = pf[2 * g + hf];
-                        pl[2 * g + hf] = pack2(pr[g][2 * hf] - __uint_as_float(x << 16),
-                                               pr[g][2 * hf + 1] - __uint_as_float(x & 0xffff0000u), BF);
+                for (int g = 0; g < 2; g++) {
+                    if (BF) {
+                        const uint32_t x = pf[nb][g];
+                        pl[nb][g] = transposed(pack2(pr[nb][2 * g] - __uint_as_float(x << 16),
+                                                     pr[nb][2 * g + 1] - __uint_as_float(x & 0xffff0000u), BF));
                     }
+                    pf[nb][g] = transposed(pf[nb][g]);
+                }
             }
+            auto product = [&](int j, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
+                const uint32_t vf[4] = {v0, v1, v2, v3};
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) {
+                    mma16816<BF>(acc[nb][j], vf, pf[nb][0], pf[nb][1]);
+                    if (BF) mma16816<BF>(acc[nb][j], vf, pl[nb][0], pl[nb][1]);
+                }
+            };
 
             // values: piece r of rows 2cc, 2cc+1, 2cc+8, 2cc+9
             const uint8_t *sv = st + vrd;
             if constexpr (F::ESZ == 2) {
 #pragma unroll
                 for (int x = 0; x < HDP / 64; x++) {
-                    uint4 w[4];
+                    uint32_t w[4][4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        w[e] = *reinterpret_cast<const uint4 *>(sv + ((e & 1) + 8 * (e >> 1)) * F::RB + x * 128);
+                        const uint4 v = *reinterpret_cast<const uint4 *>(sv + ((e & 1) + 8 * (e >> 1)) * F::RB + x * 128);
+                        w[e][0] = v.x; w[e][1] = v.y; w[e][2] = v.z; w[e][3] = v.w;
                     }
-                    const uint32_t *w0 = &w[0].x, *w1 = &w[1].x, *w2 = &w[2].x, *w3 = &w[3].x;
 #pragma unroll
-                    for (int d = 0; d < 4; d++) {
-                        const uint32_t a0 = __byte_perm(w0[d], w1[d], 0x5410), b0 = __byte_perm(w2[d], w3[d], 0x5410);
-                        const uint32_t a1 = __byte_perm(w0[d], w1[d], 0x7632), b1 = __byte_perm(w2[d], w3[d], 0x7632);
-                        mma16816<BF>(acc[8 * x + 2 * d], pf, a0, b0);
-                        mma16816<BF>(acc[8 * x + 2 * d + 1], pf, a1, b1);
-                        if (BF) {
-                            mma16816<BF>(acc[8 * x + 2 * d], pl, a0, b0);
-                            mma16816<BF>(acc[8 * x + 2 * d + 1], pl, a1, b1);
-                        }
-                    }
+                    for (int d = 0; d < 4; d++)
+                        product(4 * x + d, __byte_perm(w[0][d], w[1][d], 0x5410), __byte_perm(w[0][d], w[1][d], 0x7632),
+                                __byte_perm(w[2][d], w[3][d], 0x5410), __byte_perm(w[2][d], w[3][d], 0x7632));
                 }
             } else {
                 uint32_t w[4][HDP / 32];
@@ -596,10 +622,8 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
                     // (key a byte, key b byte) pairs of dims 4d, 4d+1 and 4d+2, 4d+3
                     const uint32_t a01 = __byte_perm(w[0][d], w[1][d], 0x5140), a23 = __byte_perm(w[0][d], w[1][d], 0x7362);
                     const uint32_t b01 = __byte_perm(w[2][d], w[3][d], 0x5140), b23 = __byte_perm(w[2][d], w[3][d], 0x7362);
-                    mma16816<BF>(acc[4 * d], pf, to_f16x2<KIND, 0>(a01), to_f16x2<KIND, 0>(b01));
-                    mma16816<BF>(acc[4 * d + 1], pf, to_f16x2<KIND, 1>(a01), to_f16x2<KIND, 1>(b01));
-                    mma16816<BF>(acc[4 * d + 2], pf, to_f16x2<KIND, 0>(a23), to_f16x2<KIND, 0>(b23));
-                    mma16816<BF>(acc[4 * d + 3], pf, to_f16x2<KIND, 1>(a23), to_f16x2<KIND, 1>(b23));
+                    product(2 * d, to_f16x2<KIND, 0>(a01), to_f16x2<KIND, 1>(a01), to_f16x2<KIND, 0>(b01), to_f16x2<KIND, 1>(b01));
+                    product(2 * d + 1, to_f16x2<KIND, 0>(a23), to_f16x2<KIND, 1>(a23), to_f16x2<KIND, 0>(b23), to_f16x2<KIND, 1>(b23));
                 }
             }
         };
@@ -645,37 +669,42 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP>::CTAS) gqa_decod
         if (unmapped && lane == 0) atomicOr(c.dev_err, WB_DERR_BOUNDS);
 
         // ---- the four warps' outputs into one, through the MST ring stages
-        // (8 or 16 rows each) that hold none of the next part's blocks
-        l[0] = quad_sum(l[0]);
-        l[1] = quad_sum(l[1]);
-        if (cc == 0) {
+        // that hold none of the next part's blocks
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++) {
-                s_m[warp][r + 8 * hf] = m[hf];
-                s_l[warp][r + 8 * hf] = l[hf];
-                s_m2[warp][r + 8 * hf] = QUANT ? m2[hf] : m[hf];
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                l[nb][e] = oct_sum(l[nb][e]);
+                if (r == 0) {
+                    s_m[warp][8 * nb + 2 * cc + e] = m[nb][e];
+                    s_l[warp][8 * nb + 2 * cc + e] = l[nb][e];
+                    s_m2[warp][8 * nb + 2 * cc + e] = QUANT ? m2[nb][e] : m[nb][e];
+                }
             }
-        }
-        // row's values of warp w (each warp has its own stage: s_stage)
         if (lane == 0) s_stage[warp] = stage;
         auto row_at = [&](int w, int stage_w, int row) {
-            const int sg = (stage_w + NST - MST + (MST == 2 ? row >> 3 : 0)) % NST;
-            return reinterpret_cast<float *>(sm + (w * NST + sg) * F::STAGE) + (MST == 2 ? row & 7 : row) * HDP;
+            const int sg = (stage_w + NST - F::MST + row / F::MROWS) % NST;
+            return reinterpret_cast<float *>(sm + (w * NST + sg) * F::STAGE) + row % F::MROWS * HDP;
         };
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            // column n of product j is dim n * 16 + j (8-bit, 128 columns), n * 8 + j % 8 + 64 (j / 8) (else)
+        for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int row = r + 8 * (e >> 1), n = 2 * cc + (e & 1);
-                const int d = F::ESZ == 1 && HDP == 128 ? n * 16 + j : n * 8 + (j & 7) + 64 * (j >> 3);
-                if (row < g.nrow) row_at(warp, stage, row)[d] = acc[j][e];
+            for (int e = 0; e < 2; e++) {
+                const int row = 8 * nb + 2 * cc + e;
+                if (row < g.nrow) {
+                    float *o = row_at(warp, stage, row);
+#pragma unroll
+                    for (int j = 0; j < NV; j++) {
+                        // product j holds dims 2j, 2j+1 of the lane's piece(s)
+                        const int d = F::ESZ == 2 ? 64 * (j >> 2) + r * 8 + 2 * (j & 3) : r * (HDP / 8) + 2 * j;
+                        *reinterpret_cast<float2 *>(o + d) = make_float2(acc[nb][j][e], acc[nb][j][2 + e]);
+                    }
+                }
             }
-        }
         __syncthreads();
         if (tid == GD_THREADS - 1) next_seg(s_seg[(part + 2) % 3]);
-        if (tid < 16) {
+        if (tid < ROWS) {
             float M = -1e30f, M2 = -1e30f, L = 0.0f;
             for (int w = 0; w < GD_WARPS; w++) {
                 M = fmaxf(M, s_m[w][tid]);
@@ -757,24 +786,29 @@ size_t gqa_decode_scratch(const GqaCacheArgs &c, int H, int sm_count) {
     return (size_t)gd_grid(c, H, sm_count, 4) * 2 * gqa_piece(c.hd <= 64 ? 64 : 128) * sizeof(float);
 }
 
-template <class T, int KIND, int HDP, bool FULL>
+template <class T, int KIND, int HDP, int NB, bool FULL>
 static int gd_launch_as(const GqaDecodeArgs &a, int sm_count, cudaStream_t st, std::string *msg) {
-    using F = GdConf<KIND, HDP>;
+    using F = GdConf<KIND, HDP, NB>;
     static const cudaError_t set =
-        cudaFuncSetAttribute(gqa_decode_kernel<T, KIND, HDP, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES);
+        cudaFuncSetAttribute(gqa_decode_kernel<T, KIND, HDP, NB, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES);
     if (set != cudaSuccess) {
         *msg = std::string("decode kernel attributes: ") + cudaGetErrorString(set);
         return WB_ECUDA;
     }
     ProfScope ps("gqa_decode", st);
-    gqa_decode_kernel<T, KIND, HDP, FULL><<<gd_grid(a.c, a.H, sm_count, F::CTAS), GD_THREADS, F::BYTES, st>>>(a);
+    gqa_decode_kernel<T, KIND, HDP, NB, FULL><<<gd_grid(a.c, a.H, sm_count, F::CTAS), GD_THREADS, F::BYTES, st>>>(a);
     return WB_OK;
 }
 
 template <class T, int KIND, int HDP>
 static int gd_launch(const GqaDecodeArgs &a, int sm_count, cudaStream_t st, std::string *msg) {
-    return a.c.row == HDP ? gd_launch_as<T, KIND, HDP, true>(a, sm_count, st, msg)
-                          : gd_launch_as<T, KIND, HDP, false>(a, sm_count, st, msg);
+    // up to 8 heads on a key-value head: one product's 8 columns; more: two
+    const bool full = a.c.row == HDP;
+    if (a.H / a.c.Hkv <= 8)
+        return full ? gd_launch_as<T, KIND, HDP, 1, true>(a, sm_count, st, msg)
+                    : gd_launch_as<T, KIND, HDP, 1, false>(a, sm_count, st, msg);
+    return full ? gd_launch_as<T, KIND, HDP, 2, true>(a, sm_count, st, msg)
+                : gd_launch_as<T, KIND, HDP, 2, false>(a, sm_count, st, msg);
 }
 
 int launch_gqa_decode(const GqaCacheArgs &c, int dtype, int H, const void *q, long long q_ss, long long q_hs,
