@@ -60,7 +60,9 @@ struct GqaDecodeArgs {
 static constexpr int GD_WARPS = 4, GD_THREADS = GD_WARPS * 32;
 static constexpr int GD_UNIT = 64;      // keys per unit: one 16-key block for each warp
 static constexpr int GD_ITEM = 2;       // what an item's start and end cost, in units of the line
-static constexpr int GD_SEQS = 256;     // sequences of a CTA's share whose lengths it holds in shared memory
+static constexpr int GD_FEW = 8;        // units per CTA below which items are cut into equal pieces ..
+static constexpr int GD_PIECE = 6;      // .. of this many units at least
+static constexpr int GD_SEQS = 256;     // sequences whose lengths a CTA holds in shared memory
 static constexpr float GD_SHIFT = 8.0f; // weights are kept as 2^8 exp2(s - m): see above
 
 enum { GD_NATIVE = 0, GD_INT8 = 1, GD_E4M3 = 2 };
@@ -142,6 +144,10 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// a / b, by a 32-bit division where that does
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
 // over the 8 lanes of one cc
 __device__ __forceinline__ float oct_max(float v) {
 #pragma unroll
@@ -177,7 +183,7 @@ __device__ __forceinline__ int gd_len(const GqaCacheArgs &c, int b, int *slot) {
 // The part of one item that a CTA takes: units ua .. ub-1 of U, keys k0 .. k1-1.
 struct GdSeg {
     int b, slot, hk, h0, nrow, ua, ub, U, k0, k1;
-    long long first, last;  // the item's first and last unit on the line
+    long long first, last;  // the item's first and last position with keys on the line
 };
 
 template <class T, int KIND, int HDP, int NB, bool FULL>
@@ -202,13 +208,16 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
     const int G = a.H / c.Hkv, nch = (G + ROWS - 1) / ROWS, ips = c.Hkv * nch;  // items of a sequence
 
     // ---- the line of units and this CTA's share s0 .. s1-1
-    auto line_len = [&](int n) { return n == 0 ? 0LL : (long long)((n + GD_UNIT - 1) / GD_UNIT + GD_ITEM) * ips; };
     const int per = (c.n_seq + GD_THREADS - 1) / GD_THREADS;
-    long long mine = 0;
+    long long sum = 0;  // units of a head in this thread's sequences, and how many have any (low 24 bits)
     for (int b = tid * per; b < min((tid + 1) * per, c.n_seq); b++) {
         int slot;
         const int n = gd_len(c, b, &slot);
-        mine += line_len(n);
+        if (b < GD_SEQS) {
+            s_len[b] = n;
+            s_slot[b] = slot;
+        }
+        sum += (long long)((n + GD_UNIT - 1) / GD_UNIT) << 24 | (n > 0);
         if (n == 0 && b % (int)gridDim.x == (int)blockIdx.x) {
             T *op = (T *)a.out + (long long)b * a.H * c.hd;
             for (int i = 0; i < a.H * c.hd; i++) op[i] = from_f<T>(0.0f);
@@ -216,38 +225,57 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                 for (int h = 0; h < a.H; h++) a.lse[(long long)b * a.H + h] = -INFINITY;
         }
     }
-    long long inc = mine;
+    // exclusive sum over the threads, and the total
+    auto scan = [&](long long x, long long *all) {
+        long long inc = x;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += x;
-    }
-    if (lane == 31) s_scan[warp] = inc;
-    __syncthreads();
-    long long total = 0, before = inc - mine;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        if (lane == 31) s_scan[warp] = inc;
+        __syncthreads();
+        long long before = inc - x;
+        *all = 0;
 #pragma unroll
-    for (int w = 0; w < GD_WARPS; w++) {
-        if (w < warp) before += s_scan[w];
-        total += s_scan[w];
+        for (int w = 0; w < GD_WARPS; w++) {
+            if (w < warp) before += s_scan[w];
+            *all += s_scan[w];
+        }
+        return before;
+    };
+    long long total;
+    const long long sums = scan(sum, &total);
+    const long long units = (total >> 24) * ips, items = (total & 0xffffff) * ips;
+    // Few units for the CTAs there are: every item in equal pieces of P
+    // units, one for each CTA (a piece that ends with its item has one join
+    // less).  Else positions of one unit, with W more for an item's start and
+    // end, in equal shares.
+    int P = 1, W = GD_ITEM;
+    if (2 * items <= gridDim.x && units <= (long long)gridDim.x * GD_FEW) {
+        W = 0;
+        P = max(GD_PIECE, (int)((units + (gridDim.x - items) - 1) / (gridDim.x - items)));
     }
+    auto item_len = [&](int n) { return n == 0 ? 0 : ((n + GD_UNIT - 1) / GD_UNIT + W + P - 1) / P; };
+    auto length = [&](int b, int *slot) {
+        if (b >= GD_SEQS) return gd_len(c, b, slot);
+        *slot = s_slot[b];
+        return s_len[b];
+    };
+
+    long long mine = ((sum >> 24) + W * (sum & 0xffffff)) * ips, before = ((sums >> 24) + W * (sums & 0xffffff)) * ips;
+    if (W == 0) {
+        mine = 0;
+        for (int b = tid * per; b < min((tid + 1) * per, c.n_seq); b++) {
+            int slot;
+            mine += (long long)item_len(length(b, &slot)) * ips;
+        }
+        __syncthreads();
+        before = scan(mine, &total);
+    } else total = units + W * items;
     const long long grid = min((long long)gridDim.x, total);
     if ((long long)blockIdx.x >= grid) return;
-    const long long s0 = blockIdx.x * total / grid, s1 = (blockIdx.x + 1) * total / grid;
-    if (s0 >= before && s0 < before + mine) {
-        int b = tid * per;
-        for (;; b++) {
-            int slot;
-            const long long n = line_len(gd_len(c, b, &slot));
-            if (s0 < before + n) break;
-            before += n;
-        }
-        s_seq = b;
-        s_pref = before;
-    }
-    __syncthreads();
-    const int b0 = s_seq;
-    for (int i = tid; i < GD_SEQS && b0 + i < c.n_seq; i += GD_THREADS) s_len[i] = gd_len(c, b0 + i, &s_slot[i]);
-    __syncthreads();
+    const long long s0 = quotient(blockIdx.x * total, grid), s1 = quotient((blockIdx.x + 1) * total, grid);
 
     // The share's parts with keys, one after another, U = 0 past its end.  One
     // thread finds part x + 2 while part x is joined.
@@ -256,23 +284,19 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
         long long pref = s_pref, u = s_at;
         g.U = 0;
         while (u < s1) {
-            int slot, len;
-            if (nb - b0 < GD_SEQS) {
-                len = s_len[nb - b0];
-                slot = s_slot[nb - b0];
-            } else len = gd_len(c, nb, &slot);
-            const long long n = line_len(len);
-            if (u >= pref + n) {
-                pref += n;
+            int slot;
+            const int len = length(nb, &slot);
+            const int il = item_len(len), U = (len + GD_UNIT - 1) / GD_UNIT;
+            if (u >= pref + (long long)il * ips) {
+                pref += (long long)il * ips;
                 nb++;
                 continue;
             }
-            const int U = (len + GD_UNIT - 1) / GD_UNIT, il = U + GD_ITEM;
             const long long rel = u - pref;
-            const int item = (int)(rel / il), o0 = (int)(rel - (long long)item * il);
+            const int item = (int)quotient(rel, il), o0 = (int)(rel - (long long)item * il);
             const int o1 = (int)min((long long)il, o0 + (s1 - u));
             u += o1 - o0;
-            if (o1 <= GD_ITEM) continue;
+            if (o1 * P <= W) continue;
             g.b = nb;
             g.slot = slot;
             g.hk = item / nch;
@@ -280,19 +304,21 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
             g.h0 = g.hk * G + hc * ROWS;
             g.nrow = min(ROWS, G - hc * ROWS);
             g.U = U;
-            g.ua = max(0, o0 - GD_ITEM);
-            g.ub = o1 - GD_ITEM;
+            g.ua = max(0, o0 * P - W);
+            g.ub = min(U, o1 * P - W);
             g.k0 = g.ua * GD_UNIT;
             g.k1 = min(g.ub * GD_UNIT, len);
-            g.first = pref + (long long)item * il + GD_ITEM;
-            g.last = g.first + U - 1;
+            g.first = pref + (long long)item * il + W;
+            g.last = pref + (long long)item * il + il - 1;
             break;
         }
         s_seq = nb;
         s_pref = pref;
         s_at = u;
     };
-    if (tid == 0) {
+    if (s0 >= before && s0 < before + mine) {  // in this thread's sequences
+        s_seq = tid * per;
+        s_pref = before;
         s_at = s0;
         next_seg(s_seg[0]);
         next_seg(s_seg[1]);
@@ -590,7 +616,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
             };
 
             // values: piece r of rows 2cc, 2cc+1, 2cc+8, 2cc+9
-            const uint8_t *sv = st + vrd;
+            [[maybe_unused]] const uint8_t *sv = st + vrd;
             if constexpr (F::ESZ == 2) {
 #pragma unroll
                 for (int x = 0; x < HDP / 64; x++) {
@@ -734,7 +760,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
         }
         if (!whole) {
             // ---- the item's last CTA joins the pieces
-            const int c0 = (int)(((g.first + 1) * grid - 1) / total), c1 = (int)(((g.last + 1) * grid - 1) / total);
+            const int c0 = (int)quotient((g.first + 1) * grid - 1, total), c1 = (int)quotient((g.last + 1) * grid - 1, total);
             __threadfence();
             __syncthreads();
             if (tid == 0) s_last = atomicAdd(a.counters + c0, 1) == (unsigned)(c1 - c0);
@@ -745,6 +771,29 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                 const int n = c1 - c0 + 1;
                 // piece x of the item: the first CTA's second slot, the others' first
                 auto at = [&](int x) { return a.part + ((long long)(c0 + x) * 2 + (x == 0 ? 1 : 0)) * gqa_piece(HDP); };
+                if (n <= 8) {  // all of a value's pieces in one round of loads
+                    for (int i = tid; i < g.nrow * HDP; i += GD_THREADS) {
+                        const int row = i / HDP, d = i % HDP;
+                        float z[8], v[8], M = -INFINITY, L = 0.0f, o = 0.0f;
+#pragma unroll
+                        for (int x = 0; x < 8; x++) {
+                            z[x] = x < n ? __ldcg(at(x) + row) : -INFINITY;
+                            v[x] = x < n ? __ldcg(at(x) + 16 + i) : 0.0f;
+                        }
+#pragma unroll
+                        for (int x = 0; x < 8; x++) M = fmaxf(M, z[x]);
+                        if (M == -INFINITY) M = 0.0f;
+#pragma unroll
+                        for (int x = 0; x < 8; x++) {
+                            const float w = ex2(z[x] - M);
+                            L += w;
+                            o += v[x] * w;
+                        }
+                        if (d < c.hd) ((T *)a.out)[(row_out + row) * c.hd + d] = from_f<T>(L == 0.0f ? 0.0f : o / L);
+                        if (d == 0 && a.lse)
+                            a.lse[row_out + row] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+                    }
+                } else {
                 for (int row = warp; row < g.nrow; row += GD_WARPS) {
                     float M = -INFINITY, L = 0.0f;
                     for (int x = lane; x < n; x += 32) M = fmaxf(M, __ldcg(at(x) + row));
@@ -768,6 +817,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                     if (d < c.hd) ((T *)a.out)[(row_out + row) * c.hd + d] = from_f<T>(o * s_f[0][row]);
                 }
                 if (tid < g.nrow && a.lse) a.lse[row_out + tid] = s_row[tid] * 0.6931471805599453f;
+                }
             }
         }
         if (!more) return;
