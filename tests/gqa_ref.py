@@ -9,8 +9,9 @@ rounded once to the type of its product with v, whose unit roundoff is u_p
 (at most u_p p_j |v_j| each, so u_p A with A = sum_j p_j |v_j|): T in the
 prompt attention; in the one-token attention fp16, or the sum of two bf16
 numbers with bf16 values.  An fp16 probability, kept as 2^8 times its ratio
-to the largest, is below its normal range off by up to 2^-25 2^-8 of the
-largest: ``floor``, 2^-33 n max|v| over the n keys.  Everything else is fp32: a score's sum of hd
+to the largest (2^5 in the prompt attention), is below its normal range off by
+up to 2^-25 2^-8 of the largest: ``floor``, 2^-33 (2^-30) n max|v| over the n
+keys.  Everything else is fp32: a score's sum of hd
 products is off by at most hd 2^-24 sum|q k| scale -- about 1e-4 at hd 128 and
 inputs of unit size, and computed where that is more -- which moves o by that
 times A, and the log sum exp by as much."""
@@ -50,9 +51,9 @@ def attention(q, k, v, cu_q, cu_k, causal, scale):
     return out, mag, (lse, off)
 
 
-def floor(n, v):
+def floor(n, v, shift=8):
     """What fp16 probabilities below their normal range may move an output of n keys by."""
-    return 2.0 ** -33 * n * v.abs().max().item() if n and v.numel() else 0.0
+    return 2.0 ** (-25 - shift) * n * v.abs().max().item() if n and v.numel() else 0.0
 
 
 def check(got, lse, ref, mag, ref_lse, u_p=None, floor=0.0):

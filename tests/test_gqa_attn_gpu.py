@@ -17,6 +17,11 @@ def _inputs(seed, dtype, H, Hkv, hd, Tq, Tk):
     return mk(Tq, H, hd), mk(Tk, Hkv, hd), mk(Tk, Hkv, hd)
 
 
+def _check(out, lse, want, v):
+    import torch
+    ref.check(out, lse, *want, floor=ref.floor(v.shape[0], v, 5) if out.dtype == torch.float16 else 0.0)
+
+
 def _run(dtype, H, Hkv, hd, lens, past=None, causal=True, scale=None, host=False, seed=0):
     import torch
     import wave_engine_b200 as wb
@@ -28,7 +33,7 @@ def _run(dtype, H, Hkv, hd, lens, past=None, causal=True, scale=None, host=False
     out, lse = wb.gqa_attention(q, k, v, ix(cq), None if past is None else ix(ck), causal=causal, scale=scale,
                                 return_lse=True)
     o, m, z = ref.attention(q, k, v, cq, ck, causal, hd ** -0.5 if scale is None else scale)
-    ref.check(out, lse, o, m, z)
+    _check(out, lse, (o, m, z), v)
     assert wb.default_context(0).take_device_error() == 0
 
 
@@ -85,7 +90,7 @@ def test_drifting_scores(rising):
     k[:, :, 0] = (ramp if rising else -ramp)[:, None]
     cu = [0, T]
     out, lse = wb.gqa_attention(q, k, v, cu, return_lse=True, scale=1.0)
-    ref.check(out, lse, *ref.attention(q, k, v, cu, cu, True, 1.0))
+    _check(out, lse, ref.attention(q, k, v, cu, cu, True, 1.0), v)
 
 
 @pytest.mark.parametrize("hd", [64, 128, 42])
@@ -117,7 +122,7 @@ def test_strides(layout, hd):
     cu = torch.tensor([0, 100, T], dtype=torch.int32, device="cuda")
     buf = torch.full((H, T, hd), 7.0, dtype=q.dtype, device="cuda")
     out, lse = wb.gqa_attention(q, k, v, cu, return_lse=True, out=buf.transpose(0, 1))
-    ref.check(out, lse, *ref.attention(q, k, v, [0, 100, T], [0, 100, T], True, hd ** -0.5))
+    _check(out, lse, ref.attention(q, k, v, [0, 100, T], [0, 100, T], True, hd ** -0.5), v)
     out2 = wb.gqa_attention(q, k, v, cu)
     assert torch.equal(out2, out)
 

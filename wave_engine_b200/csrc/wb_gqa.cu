@@ -4,67 +4,699 @@
 //   s_ij = scale q_i . k_j  over the keys j <= i + (n_k - n_q) of the
 //   query's own sequence (all of them when not causal);
 //   lse_i = log sum_j exp(s_ij); a query without keys gives 0 and -inf.
+//
+// One pass over the keys per query tile with the running maximum m and sum
+// l of the softmax: S = Q K^T on tcgen05 into TMEM, P = 2^(c S - m) in
+// registers (c = scale log2 e), P back to TMEM as the left operand of
+// O += P V, O in TMEM until the end.  m follows the row's maximum only when
+// that is more than 2^8 ahead (O and l are then rescaled), so most tiles
+// touch O on the tensor cores alone.
+//
+// Tiles.  The query heads that share a key-value head are rows of the same
+// tile: row = token * G + g, 128 / G tokens of G heads, which TMA gathers as
+// one box.  A CTA has two such tiles, one softmax warpgroup each: while the
+// tensor cores work for one, the other's warps take exponentials, and both
+// read the same K and V tiles (128 keys).  At head_dim 128 a pair of tiles
+// costs 2048 tensor cycles and, at 16 ex2 per cycle and SM, 2048 cycles of
+// the exponential unit; part of the exponentials therefore run on the FMA
+// pipe instead (a polynomial of degree 4).
 #include "wb_gqa.h"
+#include "wb_ptx.cuh"
+#include "wb_tc.h"
+
+#include <algorithm>
+#include <type_traits>
 
 namespace wb {
 
-// One warp per (query token, head): a running maximum m, sum l and weighted
-// values, one key at a time; the lanes hold 4 interleaved dims each.
-template <class T>
-__global__ void __launch_bounds__(128) gqa_attn_simple_kernel(GqaAttnArgs a) {
-    const long long wid = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (wid >= a.total_q * a.H) return;
-    const long long t = wid / a.H;
-    const int h = (int)(wid - t * a.H), hk = h / (a.H / a.Hkv);
-    const int b = gqa_find_seq(a.cu_q, a.n_seq, t);
-    const long long q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = a.cu_k[b], k1 = a.cu_k[b + 1];
-    if (q0 < 0 || t < q0 || t >= q1 || q1 > a.total_q || k0 < 0 || k1 < k0 || k1 > a.total_k) {
-        if (lane == 0) atomicOr(a.dev_err, WB_DERR_BOUNDS);
-        return;
+static constexpr int GA_ROWS = 128, GA_KEYS = 128;  // rows of a query tile, keys of a K/V tile
+static constexpr int GA_THREADS = 384;
+static constexpr int GA_W_TMA = 8, GA_W_MMA = 9, GA_W_FIX = 10;  // warps 0-7: softmax
+// pairs (of 16 in a row's 32 columns) whose exponentials run on the FMA pipe
+__device__ __forceinline__ constexpr bool GA_ON_FMA(int i) { return i % 4 == 3; }
+static constexpr int GA_EDGES = 4;  // most key tiles that some row of a CTA sees in part
+
+struct GaArgs {
+    GqaAttnArgs a;
+    float c;      // |scale| log2 e, at least 1e-30
+    int G, TT;    // heads per key-value head, tokens of a query tile
+    int vec;      // out rows take 16-byte stores
+};
+
+template <int HDP>
+struct GaConf {
+    static constexpr int NC = HDP / 64;              // 64-column swizzle atoms of a row
+    static constexpr int Q_BYTES = GA_ROWS * HDP * 2;
+    static constexpr int KV_BYTES = GA_KEYS * HDP * 2;
+    static constexpr int ST = HDP == 64 ? 4 : 2;     // K/V stages
+    static constexpr int OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + ST * KV_BYTES, OFF_BAR = OFF_V + ST * KV_BYTES;
+    static constexpr int NBAR = 6 * ST + 8;
+    static constexpr int BYTES = OFF_BAR + NBAR * 8 + 1024;
+    static_assert(BYTES <= 227 * 1024, "shared memory");
+};
+
+// Bounded mbarrier wait that also gives up once another role has: a timeout
+// then does not chain into one per barrier.
+__device__ __forceinline__ bool ga_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (true) {
+        if (ptx::mbar_try_wait_sleep(bar, parity, 20000)) return true;
+        if (*gave_up) return false;
+        if (clock64() - t0 > 4000000000LL) {
+            *gave_up = 1;
+            return false;
+        }
     }
-    const long long nk = k1 - k0;
-    long long vis = a.causal ? (t - q0) + nk - (q1 - q0) + 1 : nk;
-    vis = vis < nk ? vis : nk;
-    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-    const T *qp = (const T *)a.q + t * a.q_ts + (long long)h * a.q_hs;
-    for (int i = 0; i < 4; i++) q[i] = lane + 32 * i < a.hd ? to_f(qp[lane + 32 * i]) : 0.0f;
-    float m = -INFINITY, l = 0.0f, le = 0.0f;  // l's rounding so far in le
-    for (long long j = 0; j < vis; j++) {
-        const T *kp = (const T *)a.k + (k0 + j) * a.k_ts + (long long)hk * a.k_hs;
-        const T *vp = (const T *)a.v + (k0 + j) * a.v_ts + (long long)hk * a.v_hs;
-        float s = 0.0f;
-        for (int i = 0; i < 4; i++)
-            if (lane + 32 * i < a.hd) s = fmaf(q[i], to_f(kp[lane + 32 * i]), s);
-        s = warp_sum(s) * a.scale;
-        const float mn = fmaxf(m, s);
-        const float c = m == mn ? 1.0f : expf(m - mn), p = s == mn ? 1.0f : expf(s - mn);
-        const float y = p - le * c, ln = l * c + y;
-        le = (ln - l * c) - y;
-        l = ln;
-        for (int i = 0; i < 4; i++)
-            if (lane + 32 * i < a.hd) o[i] = o[i] * c + p * to_f(vp[lane + 32 * i]);
-        m = mn;
-    }
-    T *op = (T *)a.out + t * a.o_ts + (long long)h * a.o_hs;
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    for (int i = 0; i < 4; i++)
-        if (lane + 32 * i < a.hd) op[lane + 32 * i] = from_f<T>(o[i] * inv);
-    if (a.lse && lane == 0) a.lse[(long long)h * a.total_q + t] = m + logf(l);
 }
 
-size_t gqa_attention_scratch(const GqaAttnArgs &, int) { return 0; }
+__device__ __forceinline__ float ga_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
-int launch_gqa_attention(const GqaAttnArgs &a, int dtype, void *, int, cudaStream_t st, std::string *msg) {
-    const long long blocks = (a.total_q * a.H + 3) / 4;
-    if (blocks > 0x7fffffffLL) {
-        *msg = "too many query rows";
+// 2^x of two values <= 127 on the FMA pipe: x = n + f, |f| <= 1/2, by adding
+// 1.5 2^23; 2^f by a polynomial fitted to the relative error (2.7e-6 at
+// most); n into the exponent.  Below 2^-126 the result is 0 within 2^-146.
+// NaN must not come here.
+__device__ __forceinline__ void ga_ex2_fma(uint64_t x, float &e0, float &e1) {
+    float x0, x1;
+    ptx::f2_unpack(x, x0, x1);
+    x = ptx::f2_pack(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
+    const uint64_t big = ptx::f2_pack(12582912.0f, 12582912.0f), nbig = ptx::f2_pack(-12582912.0f, -12582912.0f);
+    const uint64_t n = ptx::f2_add(x, big);
+    const uint64_t f = ptx::f2_fma(ptx::f2_add(n, nbig), ptx::f2_pack(-1.0f, -1.0f), x);
+    uint64_t p = ptx::f2_pack(0.009570102207f, 0.009570102207f);
+    p = ptx::f2_fma(p, f, ptx::f2_pack(0.055917862803f, 0.055917862803f));
+    p = ptx::f2_fma(p, f, ptx::f2_pack(0.240247443318f, 0.240247443318f));
+    p = ptx::f2_fma(p, f, ptx::f2_pack(0.693121790886f, 0.693121790886f));
+    p = ptx::f2_fma(p, f, ptx::f2_pack(0.999999284744f, 0.999999284744f));
+    float n0, n1, p0, p1;
+    ptx::f2_unpack(n, n0, n1);
+    ptx::f2_unpack(p, p0, p1);
+    const float tiny = -1.17549435e-38f;  // takes back the 2^-126 that x was raised to
+    ptx::f2_unpack(ptx::f2_add(ptx::f2_pack(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23)),
+                                            __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23))),
+                               ptx::f2_pack(tiny, tiny)),
+                   e0, e1);
+}
+
+// the larger; NaN if either is
+__device__ __forceinline__ float ga_max(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t ga_pack(float lo, float hi) {
+    uint32_t r;
+    if (__is_same(T, __nv_bfloat16)) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ void ga_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+// Items (pairs of query tiles) of a sequence; 0, flagged, when its rows do
+// not lie inside the tensors.
+__device__ __forceinline__ int ga_items(const GqaAttnArgs &a, int b, int per_item) {
+    const int q0 = __ldg(a.cu_q + b), q1 = __ldg(a.cu_q + b + 1), k0 = __ldg(a.cu_k + b), k1 = __ldg(a.cu_k + b + 1);
+    if (q0 < 0 || q1 < q0 || q1 > a.total_q || k0 < 0 || k1 < k0 || k1 > a.total_k) {
+        atomicOr(a.dev_err, WB_DERR_BOUNDS);
+        return 0;
+    }
+    return (q1 - q0 + per_item - 1) / per_item;
+}
+
+// The sequence and tile pair of the `index`-th item; false past the last.
+// Up to 256 sequences: pairs late in their sequences (with the most keys)
+// first -- the largest t with more than `index` items at or behind pair t,
+// then by sequence -- so that the last CTAs to start are short.  More: in the
+// order of the sequences, in one pass.  Run by one warp.
+__device__ __forceinline__ bool ga_find(const GqaAttnArgs &a, int per_item, long long index, int lane, int *seq, int *pair) {
+    constexpr int N = 8;
+    if (a.n_seq > 32 * N) {
+        long long before = 0;
+        for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
+            const int n = b0 + lane < a.n_seq ? ga_items(a, b0 + lane, per_item) : 0;
+            int inc = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += y;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, before + inc > index);
+            if (past) {
+                const int at = __ffs(past) - 1;
+                *seq = b0 + at;
+                *pair = (int)(index - before) - __shfl_sync(0xffffffffu, inc - n, at);
+                return true;
+            }
+            before += __shfl_sync(0xffffffffu, inc, 31);
+        }
+        return false;
+    }
+    int n[N];
+    int hi = 0;
+#pragma unroll
+    for (int x = 0; x < N; x++) {
+        n[x] = lane + 32 * x < a.n_seq ? ga_items(a, lane + 32 * x, per_item) : 0;
+        hi = max(hi, n[x]);
+    }
+    auto behind = [&](int t) {  // items of pairs >= t
+        int sum = 0;
+#pragma unroll
+        for (int x = 0; x < N; x++) sum += max(0, n[x] - t);
+        return (long long)__reduce_add_sync(0xffffffffu, sum);
+    };
+    if (index >= behind(0)) return false;
+    int lo = 0;
+    hi = __reduce_max_sync(0xffffffffu, hi);  // behind(lo) > index >= behind(hi)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (behind(mid) > index) lo = mid;
+        else hi = mid;
+    }
+    int rank = (int)(index - behind(hi));
+#pragma unroll
+    for (int x = 0; x < N; x++) {
+        const uint32_t has = __ballot_sync(0xffffffffu, n[x] > lo);
+        if (rank < 0) continue;
+        if (rank < __popc(has)) {
+            *seq = 32 * x + (int)__fns(has, 0, rank + 1);
+            *pair = lo;
+            rank = -1;
+        } else {
+            rank -= __popc(has);
+        }
+    }
+    return true;
+}
+
+// Roles: warps 0-3 and 4-7 softmax and epilogue of tiles 0 and 1 (thread =
+// row); warp 8 loads; warp 9 issues the MMAs and owns TMEM; warps 10, 11 look
+// through the V tiles at the rows' edges (below).
+//
+// Edges.  A key that a row does not see gets probability 0, but 0 times an
+// infinity or NaN among its values would reach the row through the MMA.  So
+// in the tiles that some row sees in part (at the diagonal and at the
+// sequence's end) warps 10 and 11 set values that are not finite, and all
+// values past the sequence's last key, to 0 before the MMA may read them, and
+// note the key; the epilogue adds such values to the rows that do see them.
+template <class T, int HDP>
+__global__ void __launch_bounds__(GA_THREADS, 1)
+    gqa_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                    const __grid_constant__ CUtensorMap tm_v, const GaArgs ga) {
+    using F = GaConf<HDP>;
+    constexpr int ST = F::ST, NC = F::NC;
+    constexpr bool BF = __is_same(T, __nv_bfloat16);
+    const GqaAttnArgs &a = ga.a;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sm + F::OFF_BAR);
+    uint64_t *kfull = bars, *kfree = kfull + ST, *vfull = kfree + ST, *vfree = vfull + ST, *vok = vfree + ST;
+    uint64_t *vgo = vok + ST, *qfull = vgo + ST, *sfull = qfull + 1, *pready = sfull + 2, *ofull = pready + 2;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int s_gave_up, s_seq, s_pair;
+    __shared__ uint32_t s_bad[GA_EDGES][GA_KEYS / 32];  // keys with values that are not finite
+    volatile int *gave_up = &s_gave_up;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int G = ga.G, TT = ga.TT;
+
+    if (warp == 0) {
+        int seq = -1, pair = 0;
+        if (!ga_find(a, 2 * TT, blockIdx.x / a.Hkv, lane, &seq, &pair)) seq = -1;
+        if (lane == 0) {
+            s_seq = seq;
+            s_pair = pair;
+        }
+    }
+    if (tid == 32) {
+        for (int i = 0; i < F::NBAR; i++) {
+            uint64_t *b = bars + i;
+            ptx::mbar_init(b, b >= vok && b < vok + ST ? 2 : b >= pready && b < pready + 2 ? 4 : 1);
+        }
+        ptx::fence_mbar_init();
+        s_gave_up = 0;
+    }
+    if (tid >= 64 && tid < 64 + GA_EDGES * GA_KEYS / 32) (&s_bad[0][0])[tid - 64] = 0;
+    __syncthreads();
+    const int seq = s_seq;
+    if (seq < 0) return;
+    const int q0 = __ldg(a.cu_q + seq), nq = __ldg(a.cu_q + seq + 1) - q0;
+    const int k0 = __ldg(a.cu_k + seq), nk = __ldg(a.cu_k + seq + 1) - k0;
+    const int hk = blockIdx.x % a.Hkv;
+    const int tok0 = s_pair * 2 * TT;  // first token of tile 0
+    // keys that token t sees
+    auto visible = [&](int t) {
+        const long long n = a.causal ? (long long)t + 1 + nk - nq : nk;
+        return (int)max(0LL, min((long long)nk, n));
+    };
+    // key tiles of each query tile, and the first that some row sees in part
+    int nt[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+        nt[t] = tok0 + t * TT < nq ? (visible(min(tok0 + (t + 1) * TT, nq) - 1) + GA_KEYS - 1) / GA_KEYS : 0;
+    const int nmax = max(nt[0], nt[1]);
+    const int edge = visible(tok0) / GA_KEYS;
+
+    if (warp == GA_W_MMA) {
+        ptx::tmem_alloc(&tmem_slot, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    // columns: S of tile 0, S of tile 1, O of tile 0, O of tile 1
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        if (warp == GA_W_TMA) {
+            if (lane == 0 && nmax > 0) {
+                bool ok = true;
+                const int qrows = G * TT;
+                ptx::mbar_arrive_expect_tx(qfull, (uint32_t)((nt[0] > 0) + (nt[1] > 0)) * NC * qrows * 128);
+                for (int t = 0; t < 2; t++)
+                    for (int c = 0; nt[t] > 0 && c < NC; c++)
+                        ptx::tma_load_4d(sm + t * F::Q_BYTES + c * (GA_ROWS * 128), &tm_q, qfull, c * 64, 0, hk,
+                                         q0 + tok0 + t * TT);
+                int j = 0;
+                for (; j < nmax; j++) {
+                    const int st = j % ST;
+                    const uint32_t ph = (uint32_t)(j / ST - 1) & 1;
+                    if (j >= ST && !ga_wait(kfree + st, ph, gave_up)) {
+                        ok = false;
+                        break;
+                    }
+                    ptx::mbar_arrive_expect_tx(kfull + st, F::KV_BYTES);
+                    for (int c = 0; c < NC; c++)
+                        ptx::tma_load_3d(sm + F::OFF_K + st * F::KV_BYTES + c * (GA_KEYS * 128), &tm_k, kfull + st, c * 64,
+                                         hk, k0 + j * GA_KEYS);
+                    if (j >= ST && !ga_wait(vfree + st, ph, gave_up)) {
+                        ok = false;
+                        j++;
+                        break;
+                    }
+                    // warps 10, 11 come to a stage out of step with its
+                    // phases: this one lets them at the tile's own
+                    if (j >= edge) ptx::mbar_arrive(vgo + st);
+                    ptx::mbar_arrive_expect_tx(vfull + st, F::KV_BYTES);
+                    for (int c = 0; c < NC; c++)
+                        ptx::tma_load_3d(sm + F::OFF_V + st * F::KV_BYTES + c * (GA_KEYS * 128), &tm_v, vfull + st, c * 64,
+                                         hk, k0 + j * GA_KEYS);
+                }
+                if (!ok) {
+                    // copies in flight land before the CTA leaves
+                    atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
+                    ptx::mbar_wait(qfull, 0, 200000000LL);
+                    for (int i = max(0, j - ST); i < j; i++) {
+                        ptx::mbar_wait(kfull + i % ST, (uint32_t)(i / ST) & 1, 200000000LL);
+                        if (i < j - 1) ptx::mbar_wait(vfull + i % ST, (uint32_t)(i / ST) & 1, 200000000LL);
+                    }
+                }
+            }
+        } else if (warp == GA_W_MMA) {
+            if (lane == 0 && nmax > 0) {
+                constexpr uint32_t ID_QK = BF ? ptx::idesc_bf16(128, 128, 0, 0) : ptx::idesc_f16(128, 128, 0, 0);
+                constexpr uint32_t ID_PV = BF ? ptx::idesc_bf16(128, HDP, 0, 1) : ptx::idesc_f16(128, HDP, 0, 1);
+                auto qk = [&](int t, int j) {
+                    const uint64_t ad = ptx::smem_desc(ptx::smem_u32(sm + t * F::Q_BYTES), 16, 1024, ptx::UMMA_SW128);
+                    const uint64_t bd = ptx::smem_desc(ptx::smem_u32(sm + F::OFF_K + (j % ST) * F::KV_BYTES), 16, 1024,
+                                                       ptx::UMMA_SW128);
+#pragma unroll
+                    for (int kk = 0; kk < HDP / 16; kk++)
+                        ptx::mma_bf16(tmem + t * 128, ad + (uint64_t)((kk >> 2) * (GA_ROWS * 8) + (kk & 3) * 2),
+                                      bd + (uint64_t)((kk >> 2) * (GA_KEYS * 8) + (kk & 3) * 2), ID_QK, kk > 0);
+                    ptx::mma_commit(sfull + t);
+                };
+                auto pv = [&](int t, int j) {
+                    const uint64_t vd = ptx::smem_desc(ptx::smem_u32(sm + F::OFF_V + (j % ST) * F::KV_BYTES),
+                                                       GA_KEYS * 128, 1024, ptx::UMMA_SW128);
+#pragma unroll
+                    for (int kk = 0; kk < GA_KEYS / 16; kk++)
+                        ptx::mma_bf16_ta(tmem + 256 + t * HDP, tmem + t * 128 + kk * 8, vd + (uint64_t)(kk * 2048 >> 4), ID_PV,
+                                         j > 0 || kk > 0);
+                };
+                bool ok = ga_wait(qfull, 0, gave_up) && ga_wait(kfull, 0, gave_up);
+                if (ok) {
+                    ptx::tc_fence_after();
+                    if (nt[0] > 0) qk(0, 0);
+                    if (nt[1] > 0) qk(1, 0);
+                    ptx::mma_commit(kfree);
+                }
+                for (int j = 0; ok && j < nmax; j++) {
+                    const int st = j % ST;
+                    const bool more = j + 1 < nmax;
+                    ok = ga_wait(vfull + st, (uint32_t)(j / ST) & 1, gave_up) &&
+                         (j < edge || ga_wait(vok + st, (uint32_t)((j - edge) / ST) & 1, gave_up)) &&
+                         (!more || ga_wait(kfull + (j + 1) % ST, (uint32_t)((j + 1) / ST) & 1, gave_up));
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+                        if (ok && j < nt[t]) {
+                            ok = ga_wait(pready + t, (uint32_t)j & 1, gave_up);
+                            if (!ok) break;
+                            ptx::tc_fence_after();
+                            pv(t, j);
+                            if (j + 1 < nt[t]) qk(t, j + 1);  // in order behind the product that reads P from S's columns
+                            else ptx::mma_commit(ofull + t);
+                        }
+                    if (ok) {
+                        ptx::mma_commit(vfree + st);
+                        if (more) ptx::mma_commit(kfree + (j + 1) % ST);
+                    }
+                }
+                if (!ok) {
+                    atomicOr(a.dev_err, WB_DERR_TIMEOUT_MMA);
+                    // the MMAs issued have completed before TMEM is released
+                    ptx::mma_commit(bars + F::NBAR - 1);
+                    ptx::mbar_wait(bars + F::NBAR - 1, 0, 200000000LL);
+                }
+            }
+        } else {
+            // V tiles at the edges: 8 threads per row, one 16-byte piece of
+            // each swizzle atom each
+            const int x = tid - GA_W_FIX * 32;
+            const uint32_t step = BF ? 0x00800080u : 0x04000400u;  // carries out of a full exponent field
+            for (int j = edge; j < nmax; j++) {
+                const int st = j % ST, left = nk - j * GA_KEYS;
+                if (!ga_wait(vgo + st, (uint32_t)((j - edge) / ST) & 1, gave_up) ||
+                    !ga_wait(vfull + st, (uint32_t)(j / ST) & 1, gave_up)) {
+                    if (lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
+                    break;
+                }
+                for (int i = 0; i < NC * 16; i++) {
+                    const int row = (x >> 3) + 8 * (i & 15);
+                    uint4 *p = reinterpret_cast<uint4 *>(sm + F::OFF_V + st * F::KV_BYTES + (i >> 4) * (GA_KEYS * 128) +
+                                                         row * 128 + (x & 7) * 16);
+                    if (row >= left) {
+                        *p = make_uint4(0, 0, 0, 0);
+                        continue;
+                    }
+                    uint4 v = *p;
+                    auto bad = [&](uint32_t w) { return ((w & 0x7fff7fffu) + step) & 0x80008000u; };
+                    if (bad(v.x) | bad(v.y) | bad(v.z) | bad(v.w)) {
+                        auto clean = [&](uint32_t w) {
+                            const uint32_t m = bad(w);
+                            return w & ~((m & 0x8000u ? 0xffffu : 0u) | (m & 0x80000000u ? 0xffff0000u : 0u));
+                        };
+                        *p = make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
+                        atomicOr(&s_bad[j - edge][row >> 5], 1u << (row & 31));
+                    }
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(vok + st);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        // ---- softmax of tile t: thread = row
+        constexpr float SHIFT = BF ? 0.0f : 5.0f;  // fp16 probabilities: 2^5 times, up to 2^13, down to 2^-29
+        const int t = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(row & 96) << 16;
+        const uint32_t S = tmem + t * 128 + lanes, O = tmem + 256 + t * HDP + lanes;
+        const int tok = tok0 + t * TT + row / G, g = row % G;
+        const bool real = row < TT * G && tok < nq;
+        const int vis = real ? visible(tok) : 0;
+        float m = -INFINITY, off = 0.0f;  // reference of the exponents, and what is added to c s
+        uint64_t l2[2] = {0, 0};
+        const uint64_t c2 = ptx::f2_pack(ga.c, ga.c);
+        bool ok = true;
+        for (int j = 0; j < nt[t]; j++) {
+            if (!ga_wait(sfull + t, (uint32_t)j & 1, gave_up)) {
+                if (lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_SOFTMAX);
+                ok = false;
+                break;
+            }
+            ptx::tc_fence_after();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int x = 0; x < 4; x++) ptx::tmem_ld32(S + 32 * x, s[x]);
+            ptx::tmem_ld_wait();
+            const int lim = vis - j * GA_KEYS;
+            const bool part = __any_sync(0xffffffffu, lim < GA_KEYS);
+            if (part) {
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (32 * x + i >= lim) s[x][i] = 0xff800000u;
+            }
+            float mx[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                mx[x] = __uint_as_float(s[x][0]);
+#pragma unroll
+                for (int i = 1; i < 32; i++) mx[x] = ga_max(mx[x], __uint_as_float(s[x][i]));
+            }
+            // a row that sees a NaN or +infinity is NaN from here on
+            float top = ga_max(ga_max(mx[0], mx[1]), ga_max(mx[2], mx[3])) * ga.c;
+            const bool far = !(top <= m + 8.0f);
+            if (__any_sync(0xffffffffu, far)) {
+                if (!(top < INFINITY)) top = NAN;
+                const float mn = far ? top : m;
+                const float f = far ? (m == -INFINITY ? 0.0f : ga_ex2(m - mn)) : 1.0f;
+                m = mn;
+                off = m == -INFINITY ? 0.0f : SHIFT - m;
+                const uint64_t f2 = ptx::f2_pack(f, f);
+                l2[0] = ptx::f2_fma(l2[0], f2, 0);
+                l2[1] = ptx::f2_fma(l2[1], f2, 0);
+                if (j > 0) {
+                    // S of this tile is complete, so the product before it is
+#pragma unroll 1
+                    for (int x = 0; x < HDP / 32; x++) {
+                        uint32_t o[32];
+                        ptx::tmem_ld32(O + 32 * x, o);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        ga_st32(O + 32 * x, o);
+                    }
+                }
+            }
+            const uint64_t off2 = ptx::f2_pack(off, off);
+            auto weigh = [&](auto fma) {
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const uint64_t e = ptx::f2_fma(
+                            ptx::f2_pack(__uint_as_float(s[x][2 * i]), __uint_as_float(s[x][2 * i + 1])), c2, off2);
+                        float e0, e1;
+                        if (decltype(fma)::value && GA_ON_FMA(i)) {
+                            ga_ex2_fma(e, e0, e1);
+                        } else {
+                            ptx::f2_unpack(e, e0, e1);
+                            e0 = ga_ex2(e0);
+                            e1 = ga_ex2(e1);
+                        }
+                        l2[i & 1] = ptx::f2_add(l2[i & 1], ptx::f2_pack(e0, e1));
+                        p[i] = ga_pack<T>(e0, e1);
+                    }
+                    ptx::tmem_st16(S + 16 * x, p);
+                }
+            };
+            // hidden keys get exactly 0: ex2(-inf)
+            if (part) weigh(std::false_type{});
+            else weigh(std::true_type{});
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(pready + t);
+        }
+        // ---- epilogue: O / l
+        if (nt[t] > 0 && ok && !ga_wait(ofull + t, 0, gave_up)) {
+            if (lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_MMA);
+            ok = false;
+        }
+        ptx::tc_fence_after();
+        if (ok) {
+            float l, l0, l1;
+            ptx::f2_unpack(ptx::f2_add(l2[0], l2[1]), l0, l1);
+            l = l0 + l1;
+            const bool none = vis == 0;
+            const float inv = 1.0f / l;
+            const int h = hk * G + g;
+            T *out = (T *)a.out + (long long)(q0 + tok) * a.o_ts + (long long)h * a.o_hs;
+            // keys noted at the edges that this row sees
+            bool noted = false;
+            const int edges = max(0, nt[t] - edge);  // all of them multiplied by now
+            for (int e = max(0, edges - ST); e < edges; e++) ga_wait(vok + (edge + e) % ST, (uint32_t)(e / ST) & 1, gave_up);
+            for (int e = 0; e < edges; e++)
+                for (int w = 0; w < GA_KEYS / 32; w++) noted |= s_bad[e][w] != 0;
+#pragma unroll 1
+            for (int x = 0; x < HDP / 32 && nt[t] > 0; x++) {
+                uint32_t o[32];
+                __syncwarp();
+                ptx::tmem_ld32(O + 32 * x, o);
+                ptx::tmem_ld_wait();
+                if (noted && real) {
+                    for (int e = 0; e < edges; e++)
+                        for (int i = 0; i < GA_KEYS; i++) {
+                            const int key = (edge + e) * GA_KEYS + i;
+                            if (key >= vis || !(s_bad[e][i >> 5] >> (i & 31) & 1)) continue;
+                            const T *v = (const T *)a.v + (long long)(k0 + key) * a.v_ts + (long long)hk * a.v_hs;
+#pragma unroll
+                            for (int d = 0; d < 32; d++)
+                                if (32 * x + d < a.hd) {
+                                    const float y = to_f(v[32 * x + d]);
+                                    if (!isfinite(y)) o[d] = __float_as_uint(__uint_as_float(o[d]) + y);
+                                }
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[i] = none ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
+                if (!real) {
+                } else if (ga.vec) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (32 * x + 8 * i < a.hd) {
+                            uint4 w;
+                            w.x = ga_pack<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]));
+                            w.y = ga_pack<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
+                            w.z = ga_pack<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
+                            w.w = ga_pack<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
+                            *reinterpret_cast<uint4 *>(out + 32 * x + 8 * i) = w;
+                        }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (32 * x + i < a.hd) out[32 * x + i] = from_f<T>(__uint_as_float(o[i]));
+                }
+            }
+            if (real && nt[t] == 0)
+                for (int d = 0; d < a.hd; d++) out[d] = from_f<T>(0.0f);
+            if (real && a.lse)
+                a.lse[(long long)h * a.total_q + q0 + tok] = none ? -INFINITY : (log2f(l) - off) * 0.6931471805599453f;
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == GA_W_MMA) ptx::tmem_dealloc(tmem, 512);
+}
+
+// ---- rows that TMA cannot read --------------------------------------------
+// A tensor map wants a 16-byte aligned base and strides of whole 16 bytes.
+// Other rows (odd offsets, head_dim 42 back to back, heads spread by a zero
+// stride) are first copied to rows of 8-element multiples; a negative scale
+// is moved into the queries there.
+static bool ga_aligned(const void *p, long long ts, long long hs, int heads) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ts > 0 && ts % 8 == 0 && (heads == 1 || (hs > 0 && hs % 8 == 0));
+}
+static long long ga_copy_elems(long long rows, int heads, int hd) { return rows * heads * ((hd + 7) & ~7); }
+struct GaCopies {
+    bool q, k, v;
+    size_t oq, ok, ov, bytes;
+};
+static GaCopies ga_copies(const GqaAttnArgs &a) {
+    GaCopies c{};
+    c.q = a.scale < 0.0f || !ga_aligned(a.q, a.q_ts, a.q_hs, a.H);
+    c.k = a.total_k && !ga_aligned(a.k, a.k_ts, a.k_hs, a.Hkv);
+    c.v = a.total_k && !ga_aligned(a.v, a.v_ts, a.v_hs, a.Hkv);
+    Carve cv;
+    c.oq = c.q ? cv.take<uint16_t>(ga_copy_elems(a.total_q, a.H, a.hd)) : 0;
+    c.ok = c.k ? cv.take<uint16_t>(ga_copy_elems(a.total_k, a.Hkv, a.hd)) : 0;
+    c.ov = c.v ? cv.take<uint16_t>(ga_copy_elems(a.total_k, a.Hkv, a.hd)) : 0;
+    c.bytes = cv.off;
+    return c;
+}
+
+size_t gqa_attention_scratch(const GqaAttnArgs &a, int) { return ga_copies(a).bytes; }
+
+// One thread per 8 output elements; flip: 0x8000 changes the sign.
+__global__ void __launch_bounds__(256) gqa_rows_kernel(const uint16_t *src, long long ts, long long hs, long long rows,
+                                                       int heads, int hd, uint32_t flip, uint4 *dst) {
+    const int per = (hd + 7) / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * heads * per) return;
+    const int d0 = (int)(i % per) * 8;
+    const long long rh = i / per, row = rh / heads;
+    const uint16_t *p = src + row * ts + (rh - row * heads) * hs;
+    uint32_t w[4];
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+        const uint32_t lo = d0 + 2 * x < hd ? p[d0 + 2 * x] ^ flip : 0, hi = d0 + 2 * x + 1 < hd ? p[d0 + 2 * x + 1] ^ flip : 0;
+        w[x] = lo | hi << 16;
+    }
+    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <class T, int HDP>
+static int ga_launch(const GaArgs &ga, cudaStream_t st, std::string *msg) {
+    using F = GaConf<HDP>;
+    const GqaAttnArgs &a = ga.a;
+    const CUtensorMapDataType dt =
+        __is_same(T, __nv_bfloat16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap tq, tk, tv;
+    int rc;
+    const uint64_t q_hs = a.H == 1 ? 16 : (uint64_t)a.q_hs * 2, q_gs = ga.G == 1 ? 16 : q_hs;
+    const uint64_t qd[4] = {(uint64_t)a.hd, (uint64_t)ga.G, (uint64_t)a.Hkv, (uint64_t)a.total_q};
+    const uint64_t qs[3] = {q_gs, a.Hkv == 1 ? 16 : q_hs * ga.G, (uint64_t)a.q_ts * 2};
+    const uint32_t qb[4] = {64, (uint32_t)ga.G, 1, (uint32_t)ga.TT};
+    if ((rc = make_tmap(&tq, a.q, dt, 4, qd, qs, qb, CU_TENSOR_MAP_SWIZZLE_128B, msg))) return rc;
+    if (a.total_k) {
+        const uint64_t kd[3] = {(uint64_t)a.hd, (uint64_t)a.Hkv, (uint64_t)a.total_k};
+        const uint32_t kb[3] = {64, 1, GA_KEYS};
+        const uint64_t ks[2] = {a.Hkv == 1 ? 16 : (uint64_t)a.k_hs * 2, (uint64_t)a.k_ts * 2};
+        const uint64_t vs[2] = {a.Hkv == 1 ? 16 : (uint64_t)a.v_hs * 2, (uint64_t)a.v_ts * 2};
+        if ((rc = make_tmap(&tk, a.k, dt, 3, kd, ks, kb, CU_TENSOR_MAP_SWIZZLE_128B, msg))) return rc;
+        if ((rc = make_tmap(&tv, a.v, dt, 3, kd, vs, kb, CU_TENSOR_MAP_SWIZZLE_128B, msg))) return rc;
+    } else {  // never loaded from
+        tk = tv = tq;
+    }
+    static const cudaError_t set =
+        cudaFuncSetAttribute(gqa_attn_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES);
+    if (set != cudaSuccess) {
+        *msg = std::string("attention kernel attributes: ") + cudaGetErrorString(set);
+        return WB_ECUDA;
+    }
+    // at most this many tile pairs, whatever the sequences' lengths are
+    const long long items = std::min(a.total_q, a.total_q / (2 * ga.TT) + a.n_seq);
+    if (items * a.Hkv > 0x7fffffffLL) {
+        *msg = "too many query tiles";
         return WB_EINVAL;
     }
     ProfScope ps("gqa_attn", st);
-    if (dtype == WB_BF16) gqa_attn_simple_kernel<__nv_bfloat16><<<(unsigned)blocks, 128, 0, st>>>(a);
-    else gqa_attn_simple_kernel<__half><<<(unsigned)blocks, 128, 0, st>>>(a);
+    gqa_attn_kernel<T, HDP><<<(unsigned)(items * a.Hkv), GA_THREADS, F::BYTES, st>>>(tq, tk, tv, ga);
     return WB_OK;
+}
+
+int launch_gqa_attention(const GqaAttnArgs &args, int dtype, void *scratch, int, cudaStream_t st, std::string *msg) {
+    GaArgs ga{args, 0.0f, args.H / args.Hkv, 0, 0};
+    GqaAttnArgs &a = ga.a;
+    ga.TT = GA_ROWS / ga.G;
+    ga.c = std::max(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // 0 would turn a hidden key's -inf into NaN
+    ga.vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.o_ts % 8 == 0 && a.o_hs % 8 == 0 && a.hd % 8 == 0;
+    const GaCopies cp = ga_copies(args);
+    auto copy = [&](const void *&p, long long &ts, long long &hs, long long rows, int heads, uint32_t flip, size_t off) {
+        const long long n = ga_copy_elems(rows, heads, a.hd) / 8;
+        void *d = (char *)scratch + off;
+        ProfScope ps("gqa_rows", st);
+        gqa_rows_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>((const uint16_t *)p, ts, hs, rows, heads, a.hd, flip,
+                                                                     (uint4 *)d);
+        p = d;
+        hs = (a.hd + 7) & ~7;
+        ts = hs * heads;
+    };
+    if (cp.q) copy(a.q, a.q_ts, a.q_hs, a.total_q, a.H, a.scale < 0.0f ? 0x8000 : 0, cp.oq);
+    if (cp.k) copy(a.k, a.k_ts, a.k_hs, a.total_k, a.Hkv, 0, cp.ok);
+    if (cp.v) copy(a.v, a.v_ts, a.v_hs, a.total_k, a.Hkv, 0, cp.ov);
+    if (dtype == WB_BF16)
+        return a.hd <= 64 ? ga_launch<__nv_bfloat16, 64>(ga, st, msg) : ga_launch<__nv_bfloat16, 128>(ga, st, msg);
+    return a.hd <= 64 ? ga_launch<__half, 64>(ga, st, msg) : ga_launch<__half, 128>(ga, st, msg);
 }
 
 }  // namespace wb

@@ -77,8 +77,8 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-static int make_tmap(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int rank, const uint64_t *dims,
-                     const uint64_t *strides, const uint32_t *box, CUtensorMapSwizzle sw, std::string *msg) {
+int make_tmap(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int rank, const uint64_t *dims,
+              const uint64_t *strides, const uint32_t *box, CUtensorMapSwizzle sw, std::string *msg) {
     auto fn = encode_fn();
     if (!fn) {
         *msg = "cuTensorMapEncodeTiled unavailable";

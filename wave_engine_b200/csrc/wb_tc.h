@@ -5,9 +5,16 @@
 #include "wb_internal.h"
 #include "wb_proj.h"
 
+#include <cuda.h>
+
 #include <string>
 
 namespace wb {
+
+// A tiled tensor map (strides in bytes, innermost dimension contiguous; no
+// interleave, out-of-bounds elements read as zero).
+int make_tmap(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int rank, const uint64_t *dims,
+              const uint64_t *strides, const uint32_t *box, CUtensorMapSwizzle sw, std::string *msg);
 
 struct TcLayerWeights {
     int E = 0, H = 0, hd = 0, C = 0;
