@@ -30,10 +30,9 @@
 namespace wb {
 
 static constexpr int GA_ROWS = 128, GA_KEYS = 128;  // rows of a query tile, keys of a K/V tile
-static constexpr int GA_THREADS = 384;
-static constexpr int GA_W_TMA = 8, GA_W_MMA = 9, GA_W_FIX = 10;  // warps 0-7: softmax
 // pairs (of 16 in a row's 32 columns) whose exponentials run on the FMA pipe
 __device__ __forceinline__ constexpr bool GA_ON_FMA(int i) { return i % 4 == 3; }
+static constexpr bool GA_TWO = true;
 static constexpr int GA_EDGES = 4;  // most key tiles that some row of a CTA sees in part
 
 struct GaArgs {
@@ -43,16 +42,23 @@ struct GaArgs {
     int vec;      // out rows take 16-byte stores
 };
 
-template <int HDP>
+// NT query tiles per CTA.
+template <int HDP, int NT>
 struct GaConf {
+    static constexpr int W_TMA = 4 * NT, W_MMA = W_TMA + 1, W_FIX = W_TMA + 2;  // warps before: softmax
+    static constexpr int THREADS = (W_FIX + 2) * 32;
+    static constexpr int CTAS = NT == 2 ? 1 : 2;     // per SM
+    // registers: the softmax warps take what the other four give up
+    static constexpr int R_SOFTMAX = NT == 2 ? 200 : 192, R_OTHER = NT == 2 ? 104 : 64;
+    static constexpr int TMEM = NT * 256, O_COL = NT * 128;  // columns: S of each tile, then O of each
     static constexpr int NC = HDP / 64;              // 64-column swizzle atoms of a row
     static constexpr int Q_BYTES = GA_ROWS * HDP * 2;
     static constexpr int KV_BYTES = GA_KEYS * HDP * 2;
-    static constexpr int ST = HDP == 64 ? 4 : 2;     // K/V stages
-    static constexpr int OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + ST * KV_BYTES, OFF_BAR = OFF_V + ST * KV_BYTES;
-    static constexpr int NBAR = 6 * ST + 8;
+    static constexpr int ST = NT == 2 ? (HDP == 64 ? 4 : 2) : (HDP == 64 ? 2 : 1);  // K/V stages
+    static constexpr int OFF_K = NT * Q_BYTES, OFF_V = OFF_K + ST * KV_BYTES, OFF_BAR = OFF_V + ST * KV_BYTES;
+    static constexpr int NBAR = 6 * ST + 3 * NT + 2;
     static constexpr int BYTES = OFF_BAR + NBAR * 8 + 1024;
-    static_assert(BYTES <= 227 * 1024, "shared memory");
+    static_assert((BYTES + 1536) * CTAS <= 227 * 1024, "shared memory");
 };
 
 // Bounded mbarrier wait that also gives up once another role has: a timeout
@@ -128,7 +134,7 @@ __device__ __forceinline__ void ga_st32(uint32_t taddr, const uint32_t (&r)[32])
         : "memory");
 }
 
-// Items (pairs of query tiles) of a sequence; 0, flagged, when its rows do
+// Items (NT query tiles each) of a sequence; 0, flagged, when its rows do
 // not lie inside the tensors.
 __device__ __forceinline__ int ga_items(const GqaAttnArgs &a, int b, int per_item) {
     const int q0 = __ldg(a.cu_q + b), q1 = __ldg(a.cu_q + b + 1), k0 = __ldg(a.cu_k + b), k1 = __ldg(a.cu_k + b + 1);
@@ -214,11 +220,11 @@ __device__ __forceinline__ bool ga_find(const GqaAttnArgs &a, int per_item, long
 // sequence's end) warps 10 and 11 set values that are not finite, and all
 // values past the sequence's last key, to 0 before the MMA may read them, and
 // note the key; the epilogue adds such values to the rows that do see them.
-template <class T, int HDP>
-__global__ void __launch_bounds__(GA_THREADS, 1)
+template <class T, int HDP, int NT>
+__global__ void __launch_bounds__(GaConf<HDP, NT>::THREADS, GaConf<HDP, NT>::CTAS)
     gqa_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const GaArgs ga) {
-    using F = GaConf<HDP>;
+    using F = GaConf<HDP, NT>;
     constexpr int ST = F::ST, NC = F::NC;
     constexpr bool BF = __is_same(T, __nv_bfloat16);
     const GqaAttnArgs &a = ga.a;
@@ -226,69 +232,76 @@ __global__ void __launch_bounds__(GA_THREADS, 1)
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + F::OFF_BAR);
     uint64_t *kfull = bars, *kfree = kfull + ST, *vfull = kfree + ST, *vfree = vfull + ST, *vok = vfree + ST;
-    uint64_t *vgo = vok + ST, *qfull = vgo + ST, *sfull = qfull + 1, *pready = sfull + 2, *ofull = pready + 2;
+    uint64_t *vgo = vok + ST, *qfull = vgo + ST, *sfull = qfull + 1, *pready = sfull + NT, *ofull = pready + NT;
     __shared__ uint32_t tmem_slot;
-    __shared__ int s_gave_up, s_seq, s_pair;
+    __shared__ int s_gave_up, s_item[5];
     __shared__ uint32_t s_bad[GA_EDGES][GA_KEYS / 32];  // keys with values that are not finite
     volatile int *gave_up = &s_gave_up;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = ga.G, TT = ga.TT;
 
     if (warp == 0) {
-        int seq = -1, pair = 0;
-        if (!ga_find(a, 2 * TT, blockIdx.x / a.Hkv, lane, &seq, &pair)) seq = -1;
+        int seq = -1, group = 0;
+        const bool any = ga_find(a, NT * TT, blockIdx.x / a.Hkv, lane, &seq, &group);
         if (lane == 0) {
-            s_seq = seq;
-            s_pair = pair;
+            s_item[0] = any ? __ldg(a.cu_q + seq) : -1;
+            if (any) {
+                s_item[1] = __ldg(a.cu_q + seq + 1) - s_item[0];
+                s_item[2] = __ldg(a.cu_k + seq);
+                s_item[3] = __ldg(a.cu_k + seq + 1) - s_item[2];
+                s_item[4] = group * NT * TT;
+            }
         }
     }
     if (tid == 32) {
         for (int i = 0; i < F::NBAR; i++) {
             uint64_t *b = bars + i;
-            ptx::mbar_init(b, b >= vok && b < vok + ST ? 2 : b >= pready && b < pready + 2 ? 4 : 1);
+            ptx::mbar_init(b, b >= vok && b < vok + ST ? 2 : b >= pready && b < pready + NT ? 4 : 1);
         }
         ptx::fence_mbar_init();
         s_gave_up = 0;
     }
     if (tid >= 64 && tid < 64 + GA_EDGES * GA_KEYS / 32) (&s_bad[0][0])[tid - 64] = 0;
     __syncthreads();
-    const int seq = s_seq;
-    if (seq < 0) return;
-    const int q0 = __ldg(a.cu_q + seq), nq = __ldg(a.cu_q + seq + 1) - q0;
-    const int k0 = __ldg(a.cu_k + seq), nk = __ldg(a.cu_k + seq + 1) - k0;
+    const int q0 = s_item[0], nq = s_item[1], k0 = s_item[2], nk = s_item[3];
+    if (q0 < 0) return;
     const int hk = blockIdx.x % a.Hkv;
-    const int tok0 = s_pair * 2 * TT;  // first token of tile 0
+    const int tok0 = s_item[4];  // first token of tile 0
     // keys that token t sees
     auto visible = [&](int t) {
         const long long n = a.causal ? (long long)t + 1 + nk - nq : nk;
         return (int)max(0LL, min((long long)nk, n));
     };
     // key tiles of each query tile, and the first that some row sees in part
-    int nt[2];
+    int nt[NT], nmax = 0;
 #pragma unroll
-    for (int t = 0; t < 2; t++)
+    for (int t = 0; t < NT; t++) {
         nt[t] = tok0 + t * TT < nq ? (visible(min(tok0 + (t + 1) * TT, nq) - 1) + GA_KEYS - 1) / GA_KEYS : 0;
-    const int nmax = max(nt[0], nt[1]);
+        nmax = max(nmax, nt[t]);
+    }
     const int edge = visible(tok0) / GA_KEYS;
 
-    if (warp == GA_W_MMA) {
-        ptx::tmem_alloc(&tmem_slot, 512);
+    if (warp == F::W_MMA) {
+        ptx::tmem_alloc(&tmem_slot, F::TMEM);
         ptx::tmem_relinquish();
     }
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    // columns: S of tile 0, S of tile 1, O of tile 0, O of tile 1
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        if (warp == GA_W_TMA) {
+    if (warp >= F::W_TMA) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::R_OTHER));
+        if (warp == F::W_TMA) {
             if (lane == 0 && nmax > 0) {
                 bool ok = true;
                 const int qrows = G * TT;
-                ptx::mbar_arrive_expect_tx(qfull, (uint32_t)((nt[0] > 0) + (nt[1] > 0)) * NC * qrows * 128);
-                for (int t = 0; t < 2; t++)
+                int tiles = 0;
+#pragma unroll
+                for (int t = 0; t < NT; t++) tiles += nt[t] > 0;
+                ptx::mbar_arrive_expect_tx(qfull, (uint32_t)tiles * NC * qrows * 128);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
                     for (int c = 0; nt[t] > 0 && c < NC; c++)
                         ptx::tma_load_4d(sm + t * F::Q_BYTES + c * (GA_ROWS * 128), &tm_q, qfull, c * 64, 0, hk,
                                          q0 + tok0 + t * TT);
@@ -327,7 +340,7 @@ __global__ void __launch_bounds__(GA_THREADS, 1)
                     }
                 }
             }
-        } else if (warp == GA_W_MMA) {
+        } else if (warp == F::W_MMA) {
             if (lane == 0 && nmax > 0) {
                 constexpr uint32_t ID_QK = BF ? ptx::idesc_bf16(128, 128, 0, 0) : ptx::idesc_f16(128, 128, 0, 0);
                 constexpr uint32_t ID_PV = BF ? ptx::idesc_bf16(128, HDP, 0, 1) : ptx::idesc_f16(128, HDP, 0, 1);
@@ -346,31 +359,37 @@ __global__ void __launch_bounds__(GA_THREADS, 1)
                                                        GA_KEYS * 128, 1024, ptx::UMMA_SW128);
 #pragma unroll
                     for (int kk = 0; kk < GA_KEYS / 16; kk++)
-                        ptx::mma_bf16_ta(tmem + 256 + t * HDP, tmem + t * 128 + kk * 8, vd + (uint64_t)(kk * 2048 >> 4), ID_PV,
+                        ptx::mma_bf16_ta(tmem + F::O_COL + t * HDP, tmem + t * 128 + kk * 8, vd + (uint64_t)(kk * 2048 >> 4), ID_PV,
                                          j > 0 || kk > 0);
                 };
                 bool ok = ga_wait(qfull, 0, gave_up) && ga_wait(kfull, 0, gave_up);
                 if (ok) {
                     ptx::tc_fence_after();
-                    if (nt[0] > 0) qk(0, 0);
-                    if (nt[1] > 0) qk(1, 0);
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+                        if (nt[t] > 0) qk(t, 0);
                     ptx::mma_commit(kfree);
                 }
                 for (int j = 0; ok && j < nmax; j++) {
                     const int st = j % ST;
                     const bool more = j + 1 < nmax;
+                    bool next = false;  // the next K tile is here
                     ok = ga_wait(vfull + st, (uint32_t)(j / ST) & 1, gave_up) &&
-                         (j < edge || ga_wait(vok + st, (uint32_t)((j - edge) / ST) & 1, gave_up)) &&
-                         (!more || ga_wait(kfull + (j + 1) % ST, (uint32_t)((j + 1) / ST) & 1, gave_up));
+                         (j < edge || ga_wait(vok + st, (uint32_t)((j - edge) / ST) & 1, gave_up));
 #pragma unroll
-                    for (int t = 0; t < 2; t++)
+                    for (int t = 0; t < NT; t++)
                         if (ok && j < nt[t]) {
                             ok = ga_wait(pready + t, (uint32_t)j & 1, gave_up);
                             if (!ok) break;
                             ptx::tc_fence_after();
                             pv(t, j);
-                            if (j + 1 < nt[t]) qk(t, j + 1);  // in order behind the product that reads P from S's columns
-                            else ptx::mma_commit(ofull + t);
+                            if (j + 1 == nt[t]) {
+                                ptx::mma_commit(ofull + t);
+                                continue;
+                            }
+                            if (!next) ok = next = ga_wait(kfull + (j + 1) % ST, (uint32_t)((j + 1) / ST) & 1, gave_up);
+                            if (!ok) break;
+                            qk(t, j + 1);  // in order behind the product that reads P from S's columns
                         }
                     if (ok) {
                         ptx::mma_commit(vfree + st);
@@ -387,7 +406,7 @@ __global__ void __launch_bounds__(GA_THREADS, 1)
         } else {
             // V tiles at the edges: 8 threads per row, one 16-byte piece of
             // each swizzle atom each
-            const int x = tid - GA_W_FIX * 32;
+            const int x = tid - F::W_FIX * 32;
             const uint32_t step = BF ? 0x00800080u : 0x04000400u;  // carries out of a full exponent field
             for (int j = edge; j < nmax; j++) {
                 const int st = j % ST, left = nk - j * GA_KEYS;
@@ -421,20 +440,22 @@ __global__ void __launch_bounds__(GA_THREADS, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::R_SOFTMAX));
         // ---- softmax of tile t: thread = row
         constexpr float SHIFT = BF ? 0.0f : 5.0f;  // fp16 probabilities: 2^5 times, up to 2^13, down to 2^-29
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(row & 96) << 16;
-        const uint32_t S = tmem + t * 128 + lanes, O = tmem + 256 + t * HDP + lanes;
+        const uint32_t S = tmem + t * 128 + lanes, O = tmem + F::O_COL + t * HDP + lanes;
         const int tok = tok0 + t * TT + row / G, g = row % G;
         const bool real = row < TT * G && tok < nq;
         const int vis = real ? visible(tok) : 0;
+        int mine = nt[0];  // this tile's key tiles
+        if (NT == 2 && t == 1) mine = nt[NT - 1];
         float m = -INFINITY, off = 0.0f;  // reference of the exponents, and what is added to c s
         uint64_t l2[2] = {0, 0};
         const uint64_t c2 = ptx::f2_pack(ga.c, ga.c);
         bool ok = true;
-        for (int j = 0; j < nt[t]; j++) {
+        for (int j = 0; j < mine; j++) {
             if (!ga_wait(sfull + t, (uint32_t)j & 1, gave_up)) {
                 if (lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_SOFTMAX);
                 ok = false;
@@ -518,7 +539,7 @@ __global__ void __launch_bounds__(GA_THREADS, 1)
             if (lane == 0) ptx::mbar_arrive(pready + t);
         }
         // ---- epilogue: O / l
-        if (nt[t] > 0 && ok && !ga_wait(ofull + t, 0, gave_up)) {
+        if (mine > 0 && ok && !ga_wait(ofull + t, 0, gave_up)) {
             if (lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_MMA);
             ok = false;
         }
@@ -533,12 +554,12 @@ __global__ void __launch_bounds__(GA_THREADS, 1)
             T *out = (T *)a.out + (long long)(q0 + tok) * a.o_ts + (long long)h * a.o_hs;
             // keys noted at the edges that this row sees
             bool noted = false;
-            const int edges = max(0, nt[t] - edge);  // all of them multiplied by now
+            const int edges = max(0, mine - edge);  // all of them multiplied by now
             for (int e = max(0, edges - ST); e < edges; e++) ga_wait(vok + (edge + e) % ST, (uint32_t)(e / ST) & 1, gave_up);
             for (int e = 0; e < edges; e++)
                 for (int w = 0; w < GA_KEYS / 32; w++) noted |= s_bad[e][w] != 0;
 #pragma unroll 1
-            for (int x = 0; x < HDP / 32 && nt[t] > 0; x++) {
+            for (int x = 0; x < HDP / 32 && mine > 0; x++) {
                 uint32_t o[32];
                 __syncwarp();
                 ptx::tmem_ld32(O + 32 * x, o);
@@ -577,7 +598,7 @@ __global__ void __launch_bounds__(GA_THREADS, 1)
                         if (32 * x + i < a.hd) out[32 * x + i] = from_f<T>(__uint_as_float(o[i]));
                 }
             }
-            if (real && nt[t] == 0)
+            if (real && mine == 0)
                 for (int d = 0; d < a.hd; d++) out[d] = from_f<T>(0.0f);
             if (real && a.lse)
                 a.lse[(long long)h * a.total_q + q0 + tok] = none ? -INFINITY : (log2f(l) - off) * 0.6931471805599453f;
@@ -585,7 +606,7 @@ __global__ void __launch_bounds__(GA_THREADS, 1)
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == GA_W_MMA) ptx::tmem_dealloc(tmem, 512);
+    if (warp == F::W_MMA) ptx::tmem_dealloc(tmem, F::TMEM);
 }
 
 // ---- rows that TMA cannot read --------------------------------------------
@@ -634,9 +655,9 @@ __global__ void __launch_bounds__(256) gqa_rows_kernel(const uint16_t *src, long
     dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <class T, int HDP>
+template <class T, int HDP, int NT>
 static int ga_launch(const GaArgs &ga, cudaStream_t st, std::string *msg) {
-    using F = GaConf<HDP>;
+    using F = GaConf<HDP, NT>;
     const GqaAttnArgs &a = ga.a;
     const CUtensorMapDataType dt =
         __is_same(T, __nv_bfloat16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -658,19 +679,19 @@ static int ga_launch(const GaArgs &ga, cudaStream_t st, std::string *msg) {
         tk = tv = tq;
     }
     static const cudaError_t set =
-        cudaFuncSetAttribute(gqa_attn_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES);
+        cudaFuncSetAttribute(gqa_attn_kernel<T, HDP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES);
     if (set != cudaSuccess) {
         *msg = std::string("attention kernel attributes: ") + cudaGetErrorString(set);
         return WB_ECUDA;
     }
     // at most this many tile pairs, whatever the sequences' lengths are
-    const long long items = std::min(a.total_q, a.total_q / (2 * ga.TT) + a.n_seq);
+    const long long items = std::min(a.total_q, a.total_q / (NT * ga.TT) + a.n_seq);
     if (items * a.Hkv > 0x7fffffffLL) {
         *msg = "too many query tiles";
         return WB_EINVAL;
     }
     ProfScope ps("gqa_attn", st);
-    gqa_attn_kernel<T, HDP><<<(unsigned)(items * a.Hkv), GA_THREADS, F::BYTES, st>>>(tq, tk, tv, ga);
+    gqa_attn_kernel<T, HDP, NT><<<(unsigned)(items * a.Hkv), F::THREADS, F::BYTES, st>>>(tq, tk, tv, ga);
     return WB_OK;
 }
 
@@ -694,9 +715,13 @@ int launch_gqa_attention(const GqaAttnArgs &args, int dtype, void *scratch, int,
     if (cp.q) copy(a.q, a.q_ts, a.q_hs, a.total_q, a.H, a.scale < 0.0f ? 0x8000 : 0, cp.oq);
     if (cp.k) copy(a.k, a.k_ts, a.k_hs, a.total_k, a.Hkv, 0, cp.ok);
     if (cp.v) copy(a.v, a.v_ts, a.v_hs, a.total_k, a.Hkv, 0, cp.ov);
-    if (dtype == WB_BF16)
-        return a.hd <= 64 ? ga_launch<__nv_bfloat16, 64>(ga, st, msg) : ga_launch<__nv_bfloat16, 128>(ga, st, msg);
-    return a.hd <= 64 ? ga_launch<__half, 64>(ga, st, msg) : ga_launch<__half, 128>(ga, st, msg);
+    auto go = [&](auto t) {
+        using T = decltype(t);
+        const bool two = GA_TWO;
+        if (a.hd <= 64) return two ? ga_launch<T, 64, 2>(ga, st, msg) : ga_launch<T, 64, 1>(ga, st, msg);
+        return two ? ga_launch<T, 128, 2>(ga, st, msg) : ga_launch<T, 128, 1>(ga, st, msg);
+    };
+    return dtype == WB_BF16 ? go(__nv_bfloat16{}) : go(__half{});
 }
 
 }  // namespace wb
