@@ -18,21 +18,19 @@
 // tensor cores work for one, the other's warps take exponentials, and both
 // read the same K and V tiles (128 keys).  At head_dim 128 a pair of tiles
 // costs 2048 tensor cycles and, at 16 ex2 per cycle and SM, 2048 cycles of
-// the exponential unit; part of the exponentials therefore run on the FMA
-// pipe instead (a polynomial of degree 4).
+// the exponential unit; what a tile waits for is the chain S -> softmax ->
+// P V -> next S, so P is handed over in two halves.  (Exponentials by a
+// polynomial on the FMA pipe were measured and not kept: a quarter of them
+// cost 4% at 8192 tokens, three eighths 7%.)
 #include "wb_gqa.h"
 #include "wb_ptx.cuh"
 #include "wb_tc.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace wb {
 
 static constexpr int GA_ROWS = 128, GA_KEYS = 128;  // rows of a query tile, keys of a K/V tile
-// pairs (of 16 in a row's 32 columns) whose exponentials run on the FMA pipe
-__device__ __forceinline__ constexpr bool GA_ON_FMA(int i) { return i % 4 == 3; }
-static constexpr bool GA_TWO = true;
 static constexpr int GA_EDGES = 4;  // most key tiles that some row of a CTA sees in part
 
 struct GaArgs {
@@ -42,23 +40,22 @@ struct GaArgs {
     int vec;      // out rows take 16-byte stores
 };
 
-// NT query tiles per CTA.
-template <int HDP, int NT>
+template <int HDP>
 struct GaConf {
+    static constexpr int NT = 2;  // query tiles of a CTA
     static constexpr int W_TMA = 4 * NT, W_MMA = W_TMA + 1, W_FIX = W_TMA + 2;  // warps before: softmax
     static constexpr int THREADS = (W_FIX + 2) * 32;
-    static constexpr int CTAS = NT == 2 ? 1 : 2;     // per SM
     // registers: the softmax warps take what the other four give up
-    static constexpr int R_SOFTMAX = NT == 2 ? 200 : 192, R_OTHER = NT == 2 ? 104 : 64;
+    static constexpr int R_SOFTMAX = 200, R_OTHER = 104;
     static constexpr int TMEM = NT * 256, O_COL = NT * 128;  // columns: S of each tile, then O of each
     static constexpr int NC = HDP / 64;              // 64-column swizzle atoms of a row
     static constexpr int Q_BYTES = GA_ROWS * HDP * 2;
     static constexpr int KV_BYTES = GA_KEYS * HDP * 2;
-    static constexpr int ST = NT == 2 ? (HDP == 64 ? 4 : 2) : (HDP == 64 ? 2 : 1);  // K/V stages
+    static constexpr int ST = HDP == 64 ? 4 : 2;  // K/V stages
     static constexpr int OFF_K = NT * Q_BYTES, OFF_V = OFF_K + ST * KV_BYTES, OFF_BAR = OFF_V + ST * KV_BYTES;
-    static constexpr int NBAR = 6 * ST + 3 * NT + 2;
+    static constexpr int NBAR = 6 * ST + 4 * NT + 2;
     static constexpr int BYTES = OFF_BAR + NBAR * 8 + 1024;
-    static_assert((BYTES + 1536) * CTAS <= 227 * 1024, "shared memory");
+    static_assert(BYTES + 1536 <= 227 * 1024, "shared memory");
 };
 
 // Bounded mbarrier wait that also gives up once another role has: a timeout
@@ -82,36 +79,10 @@ __device__ __forceinline__ float ga_ex2(float x) {
     return y;
 }
 
-// 2^x of two values <= 127 on the FMA pipe: x = n + f, |f| <= 1/2, by adding
-// 1.5 2^23; 2^f by a polynomial fitted to the relative error (2.7e-6 at
-// most); n into the exponent.  Below 2^-126 the result is 0 within 2^-146.
-// NaN must not come here.
-__device__ __forceinline__ void ga_ex2_fma(uint64_t x, float &e0, float &e1) {
-    float x0, x1;
-    ptx::f2_unpack(x, x0, x1);
-    x = ptx::f2_pack(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
-    const uint64_t big = ptx::f2_pack(12582912.0f, 12582912.0f), nbig = ptx::f2_pack(-12582912.0f, -12582912.0f);
-    const uint64_t n = ptx::f2_add(x, big);
-    const uint64_t f = ptx::f2_fma(ptx::f2_add(n, nbig), ptx::f2_pack(-1.0f, -1.0f), x);
-    uint64_t p = ptx::f2_pack(0.009570102207f, 0.009570102207f);
-    p = ptx::f2_fma(p, f, ptx::f2_pack(0.055917862803f, 0.055917862803f));
-    p = ptx::f2_fma(p, f, ptx::f2_pack(0.240247443318f, 0.240247443318f));
-    p = ptx::f2_fma(p, f, ptx::f2_pack(0.693121790886f, 0.693121790886f));
-    p = ptx::f2_fma(p, f, ptx::f2_pack(0.999999284744f, 0.999999284744f));
-    float n0, n1, p0, p1;
-    ptx::f2_unpack(n, n0, n1);
-    ptx::f2_unpack(p, p0, p1);
-    const float tiny = -1.17549435e-38f;  // takes back the 2^-126 that x was raised to
-    ptx::f2_unpack(ptx::f2_add(ptx::f2_pack(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23)),
-                                            __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23))),
-                               ptx::f2_pack(tiny, tiny)),
-                   e0, e1);
-}
-
-// the larger; NaN if either is
-__device__ __forceinline__ float ga_max(float a, float b) {
+// the largest; NaN if one is
+__device__ __forceinline__ float ga_max(float a, float b, float c) {
     float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
 
@@ -220,19 +191,19 @@ __device__ __forceinline__ bool ga_find(const GqaAttnArgs &a, int per_item, long
 // sequence's end) warps 10 and 11 set values that are not finite, and all
 // values past the sequence's last key, to 0 before the MMA may read them, and
 // note the key; the epilogue adds such values to the rows that do see them.
-template <class T, int HDP, int NT>
-__global__ void __launch_bounds__(GaConf<HDP, NT>::THREADS, GaConf<HDP, NT>::CTAS)
+template <class T, int HDP>
+__global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
     gqa_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const GaArgs ga) {
-    using F = GaConf<HDP, NT>;
-    constexpr int ST = F::ST, NC = F::NC;
+    using F = GaConf<HDP>;
+    constexpr int ST = F::ST, NC = F::NC, NT = F::NT;
     constexpr bool BF = __is_same(T, __nv_bfloat16);
     const GqaAttnArgs &a = ga.a;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + F::OFF_BAR);
     uint64_t *kfull = bars, *kfree = kfull + ST, *vfull = kfree + ST, *vfree = vfull + ST, *vok = vfree + ST;
-    uint64_t *vgo = vok + ST, *qfull = vgo + ST, *sfull = qfull + 1, *pready = sfull + NT, *ofull = pready + NT;
+    uint64_t *vgo = vok + ST, *qfull = vgo + ST, *sfull = qfull + 1, *pready = sfull + NT, *ofull = pready + 2 * NT;
     __shared__ uint32_t tmem_slot;
     __shared__ int s_gave_up, s_item[5];
     __shared__ uint32_t s_bad[GA_EDGES][GA_KEYS / 32];  // keys with values that are not finite
@@ -256,7 +227,7 @@ __global__ void __launch_bounds__(GaConf<HDP, NT>::THREADS, GaConf<HDP, NT>::CTA
     if (tid == 32) {
         for (int i = 0; i < F::NBAR; i++) {
             uint64_t *b = bars + i;
-            ptx::mbar_init(b, b >= vok && b < vok + ST ? 2 : b >= pready && b < pready + NT ? 4 : 1);
+            ptx::mbar_init(b, b >= vok && b < vok + ST ? 2 : b >= pready && b < pready + 2 * NT ? 4 : 1);
         }
         ptx::fence_mbar_init();
         s_gave_up = 0;
@@ -354,11 +325,11 @@ __global__ void __launch_bounds__(GaConf<HDP, NT>::THREADS, GaConf<HDP, NT>::CTA
                                       bd + (uint64_t)((kk >> 2) * (GA_KEYS * 8) + (kk & 3) * 2), ID_QK, kk > 0);
                     ptx::mma_commit(sfull + t);
                 };
-                auto pv = [&](int t, int j) {
+                auto pv = [&](int t, int j, int part) {  // keys 64 part ..
                     const uint64_t vd = ptx::smem_desc(ptx::smem_u32(sm + F::OFF_V + (j % ST) * F::KV_BYTES),
                                                        GA_KEYS * 128, 1024, ptx::UMMA_SW128);
 #pragma unroll
-                    for (int kk = 0; kk < GA_KEYS / 16; kk++)
+                    for (int kk = 4 * part; kk < 4 * part + 4; kk++)
                         ptx::mma_bf16_ta(tmem + F::O_COL + t * HDP, tmem + t * 128 + kk * 8, vd + (uint64_t)(kk * 2048 >> 4), ID_PV,
                                          j > 0 || kk > 0);
                 };
@@ -379,10 +350,14 @@ __global__ void __launch_bounds__(GaConf<HDP, NT>::THREADS, GaConf<HDP, NT>::CTA
 #pragma unroll
                     for (int t = 0; t < NT; t++)
                         if (ok && j < nt[t]) {
-                            ok = ga_wait(pready + t, (uint32_t)j & 1, gave_up);
+                            ok = ga_wait(pready + 2 * t, (uint32_t)j & 1, gave_up);
                             if (!ok) break;
                             ptx::tc_fence_after();
-                            pv(t, j);
+                            pv(t, j, 0);
+                            ok = ga_wait(pready + 2 * t + 1, (uint32_t)j & 1, gave_up);
+                            if (!ok) break;
+                            ptx::tc_fence_after();
+                            pv(t, j, 1);
                             if (j + 1 == nt[t]) {
                                 ptx::mma_commit(ofull + t);
                                 continue;
@@ -449,8 +424,7 @@ __global__ void __launch_bounds__(GaConf<HDP, NT>::THREADS, GaConf<HDP, NT>::CTA
         const int tok = tok0 + t * TT + row / G, g = row % G;
         const bool real = row < TT * G && tok < nq;
         const int vis = real ? visible(tok) : 0;
-        int mine = nt[0];  // this tile's key tiles
-        if (NT == 2 && t == 1) mine = nt[NT - 1];
+        const int mine = t ? nt[1] : nt[0];  // this tile's key tiles
         float m = -INFINITY, off = 0.0f;  // reference of the exponents, and what is added to c s
         uint64_t l2[2] = {0, 0};
         const uint64_t c2 = ptx::f2_pack(ga.c, ga.c);
@@ -467,8 +441,7 @@ __global__ void __launch_bounds__(GaConf<HDP, NT>::THREADS, GaConf<HDP, NT>::CTA
             for (int x = 0; x < 4; x++) ptx::tmem_ld32(S + 32 * x, s[x]);
             ptx::tmem_ld_wait();
             const int lim = vis - j * GA_KEYS;
-            const bool part = __any_sync(0xffffffffu, lim < GA_KEYS);
-            if (part) {
+            if (__any_sync(0xffffffffu, lim < GA_KEYS)) {
 #pragma unroll
                 for (int x = 0; x < 4; x++)
 #pragma unroll
@@ -477,13 +450,14 @@ __global__ void __launch_bounds__(GaConf<HDP, NT>::THREADS, GaConf<HDP, NT>::CTA
             }
             float mx[4];
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                mx[x] = __uint_as_float(s[x][0]);
+            for (int i = 0; i < 32; i += 2)
 #pragma unroll
-                for (int i = 1; i < 32; i++) mx[x] = ga_max(mx[x], __uint_as_float(s[x][i]));
-            }
+                for (int x = 0; x < 4; x++) {
+                    const float u = __uint_as_float(s[x][i]), v = __uint_as_float(s[x][i + 1]);
+                    mx[x] = i == 0 ? ga_max(u, u, v) : ga_max(mx[x], u, v);
+                }
             // a row that sees a NaN or +infinity is NaN from here on
-            float top = ga_max(ga_max(mx[0], mx[1]), ga_max(mx[2], mx[3])) * ga.c;
+            float top = ga_max(ga_max(mx[0], mx[1], mx[2]), mx[3], mx[3]) * ga.c;
             const bool far = !(top <= m + 8.0f);
             if (__any_sync(0xffffffffu, far)) {
                 if (!(top < INFINITY)) top = NAN;
@@ -508,35 +482,28 @@ __global__ void __launch_bounds__(GaConf<HDP, NT>::THREADS, GaConf<HDP, NT>::CTA
                 }
             }
             const uint64_t off2 = ptx::f2_pack(off, off);
-            auto weigh = [&](auto fma) {
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    uint32_t p[16];
+            for (int x = 0; x < 4; x++) {
+                uint32_t p[16];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const uint64_t e = ptx::f2_fma(
-                            ptx::f2_pack(__uint_as_float(s[x][2 * i]), __uint_as_float(s[x][2 * i + 1])), c2, off2);
-                        float e0, e1;
-                        if (decltype(fma)::value && GA_ON_FMA(i)) {
-                            ga_ex2_fma(e, e0, e1);
-                        } else {
-                            ptx::f2_unpack(e, e0, e1);
-                            e0 = ga_ex2(e0);
-                            e1 = ga_ex2(e1);
-                        }
-                        l2[i & 1] = ptx::f2_add(l2[i & 1], ptx::f2_pack(e0, e1));
-                        p[i] = ga_pack<T>(e0, e1);
-                    }
-                    ptx::tmem_st16(S + 16 * x, p);
+                for (int i = 0; i < 16; i++) {
+                    float e0, e1;
+                    ptx::f2_unpack(ptx::f2_fma(ptx::f2_pack(__uint_as_float(s[x][2 * i]), __uint_as_float(s[x][2 * i + 1])),
+                                               c2, off2),
+                                   e0, e1);
+                    e0 = ga_ex2(e0);
+                    e1 = ga_ex2(e1);
+                    l2[i & 1] = ptx::f2_add(l2[i & 1], ptx::f2_pack(e0, e1));
+                    p[i] = ga_pack<T>(e0, e1);
                 }
-            };
-            // hidden keys get exactly 0: ex2(-inf)
-            if (part) weigh(std::false_type{});
-            else weigh(std::true_type{});
-            ptx::tmem_st_wait();
-            ptx::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(pready + t);
+                ptx::tmem_st16(S + 16 * x, p);
+                if (x & 1) {  // half of the keys: their product may begin
+                    ptx::tmem_st_wait();
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(pready + 2 * t + (x >> 1));
+                }
+            }
         }
         // ---- epilogue: O / l
         if (mine > 0 && ok && !ga_wait(ofull + t, 0, gave_up)) {
@@ -655,9 +622,9 @@ __global__ void __launch_bounds__(256) gqa_rows_kernel(const uint16_t *src, long
     dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <class T, int HDP, int NT>
+template <class T, int HDP>
 static int ga_launch(const GaArgs &ga, cudaStream_t st, std::string *msg) {
-    using F = GaConf<HDP, NT>;
+    using F = GaConf<HDP>;
     const GqaAttnArgs &a = ga.a;
     const CUtensorMapDataType dt =
         __is_same(T, __nv_bfloat16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -679,19 +646,19 @@ static int ga_launch(const GaArgs &ga, cudaStream_t st, std::string *msg) {
         tk = tv = tq;
     }
     static const cudaError_t set =
-        cudaFuncSetAttribute(gqa_attn_kernel<T, HDP, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES);
+        cudaFuncSetAttribute(gqa_attn_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES);
     if (set != cudaSuccess) {
         *msg = std::string("attention kernel attributes: ") + cudaGetErrorString(set);
         return WB_ECUDA;
     }
     // at most this many tile pairs, whatever the sequences' lengths are
-    const long long items = std::min(a.total_q, a.total_q / (NT * ga.TT) + a.n_seq);
+    const long long items = std::min(a.total_q, a.total_q / (F::NT * ga.TT) + a.n_seq);
     if (items * a.Hkv > 0x7fffffffLL) {
         *msg = "too many query tiles";
         return WB_EINVAL;
     }
     ProfScope ps("gqa_attn", st);
-    gqa_attn_kernel<T, HDP, NT><<<(unsigned)(items * a.Hkv), F::THREADS, F::BYTES, st>>>(tq, tk, tv, ga);
+    gqa_attn_kernel<T, HDP><<<(unsigned)(items * a.Hkv), F::THREADS, F::BYTES, st>>>(tq, tk, tv, ga);
     return WB_OK;
 }
 
@@ -715,13 +682,9 @@ int launch_gqa_attention(const GqaAttnArgs &args, int dtype, void *scratch, int,
     if (cp.q) copy(a.q, a.q_ts, a.q_hs, a.total_q, a.H, a.scale < 0.0f ? 0x8000 : 0, cp.oq);
     if (cp.k) copy(a.k, a.k_ts, a.k_hs, a.total_k, a.Hkv, 0, cp.ok);
     if (cp.v) copy(a.v, a.v_ts, a.v_hs, a.total_k, a.Hkv, 0, cp.ov);
-    auto go = [&](auto t) {
-        using T = decltype(t);
-        const bool two = GA_TWO;
-        if (a.hd <= 64) return two ? ga_launch<T, 64, 2>(ga, st, msg) : ga_launch<T, 64, 1>(ga, st, msg);
-        return two ? ga_launch<T, 128, 2>(ga, st, msg) : ga_launch<T, 128, 1>(ga, st, msg);
-    };
-    return dtype == WB_BF16 ? go(__nv_bfloat16{}) : go(__half{});
+    if (dtype == WB_BF16)
+        return a.hd <= 64 ? ga_launch<__nv_bfloat16, 64>(ga, st, msg) : ga_launch<__nv_bfloat16, 128>(ga, st, msg);
+    return a.hd <= 64 ? ga_launch<__half, 64>(ga, st, msg) : ga_launch<__half, 128>(ga, st, msg);
 }
 
 }  // namespace wb
