@@ -53,7 +53,7 @@ struct GaConf {
     static constexpr int KV_BYTES = GA_KEYS * HDP * 2;
     static constexpr int ST = HDP == 64 ? 4 : 2;  // K/V stages
     static constexpr int OFF_K = NT * Q_BYTES, OFF_V = OFF_K + ST * KV_BYTES, OFF_BAR = OFF_V + ST * KV_BYTES;
-    static constexpr int NBAR = 6 * ST + 4 * NT + 2;
+    static constexpr int NBAR = 4 * ST + 4 * NT + 2;
     static constexpr int BYTES = OFF_BAR + NBAR * 8 + 1024;
     static_assert(BYTES + 1536 <= 227 * 1024, "shared memory");
 };
@@ -157,6 +157,12 @@ __device__ __forceinline__ bool ga_find(const GqaAttnArgs &a, int per_item, long
         for (int x = 0; x < N; x++) sum += max(0, n[x] - t);
         return (long long)__reduce_add_sync(0xffffffffu, sum);
     };
+    if (a.n_seq == 1) {
+        hi = __shfl_sync(0xffffffffu, n[0], 0);
+        *seq = 0;
+        *pair = hi - 1 - (int)index;
+        return index < hi;
+    }
     if (index >= behind(0)) return false;
     int lo = 0;
     hi = __reduce_max_sync(0xffffffffu, hi);  // behind(lo) > index >= behind(hi)
@@ -202,16 +208,23 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + F::OFF_BAR);
-    uint64_t *kfull = bars, *kfree = kfull + ST, *vfull = kfree + ST, *vfree = vfull + ST, *vok = vfree + ST;
-    uint64_t *vgo = vok + ST, *qfull = vgo + ST, *sfull = qfull + 1, *pready = sfull + NT, *ofull = pready + 2 * NT;
+    uint64_t *full = bars, *free_ = full + ST, *vok = free_ + ST, *vgo = vok + ST;
+    uint64_t *qfull = vgo + ST, *sfull = qfull + 1, *pready = sfull + NT, *ofull = pready + 2 * NT;
     __shared__ uint32_t tmem_slot;
-    __shared__ int s_gave_up, s_item[5];
+    __shared__ int s_gave_up, s_any_bad, s_item[5];
     __shared__ uint32_t s_bad[GA_EDGES][GA_KEYS / 32];  // keys with values that are not finite
     volatile int *gave_up = &s_gave_up;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = ga.G, TT = ga.TT;
 
-    if (warp == 0) {
+    // one barrier before the work: the loading warp finds the item, others set
+    // up TMEM and the mbarriers meanwhile
+    if (warp == F::W_TMA) {
+        if (lane == 0) {
+            ptx::prefetch_tmap(&tm_q);
+            ptx::prefetch_tmap(&tm_k);
+            ptx::prefetch_tmap(&tm_v);
+        }
         int seq = -1, group = 0;
         const bool any = ga_find(a, NT * TT, blockIdx.x / a.Hkv, lane, &seq, &group);
         if (lane == 0) {
@@ -223,19 +236,29 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                 s_item[4] = group * NT * TT;
             }
         }
-    }
-    if (tid == 32) {
-        for (int i = 0; i < F::NBAR; i++) {
+    } else if (warp == F::W_MMA) {
+        ptx::tmem_alloc(&tmem_slot, F::TMEM);
+        ptx::tmem_relinquish();
+    } else if (warp == 0) {
+        for (int i = lane; i < F::NBAR; i += 32) {
             uint64_t *b = bars + i;
             ptx::mbar_init(b, b >= vok && b < vok + ST ? 2 : b >= pready && b < pready + 2 * NT ? 4 : 1);
         }
         ptx::fence_mbar_init();
-        s_gave_up = 0;
+        if (lane == 0) s_gave_up = 0;
+    } else if (warp == 1) {
+        if (lane < GA_EDGES * GA_KEYS / 32) (&s_bad[0][0])[lane] = 0;
+        if (lane == 31) s_any_bad = 0;
     }
-    if (tid >= 64 && tid < 64 + GA_EDGES * GA_KEYS / 32) (&s_bad[0][0])[tid - 64] = 0;
+    ptx::tc_fence_before();
     __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = tmem_slot;
     const int q0 = s_item[0], nq = s_item[1], k0 = s_item[2], nk = s_item[3];
-    if (q0 < 0) return;
+    if (q0 < 0) {  // no such item
+        if (warp == F::W_MMA) ptx::tmem_dealloc(tmem, F::TMEM);
+        return;
+    }
     const int hk = blockIdx.x % a.Hkv;
     const int tok0 = s_item[4];  // first token of tile 0
     // keys that token t sees
@@ -252,15 +275,6 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
     }
     const int edge = visible(tok0) / GA_KEYS;
 
-    if (warp == F::W_MMA) {
-        ptx::tmem_alloc(&tmem_slot, F::TMEM);
-        ptx::tmem_relinquish();
-    }
-    ptx::tc_fence_before();
-    __syncthreads();
-    ptx::tc_fence_after();
-    const uint32_t tmem = tmem_slot;
-
     if (warp >= F::W_TMA) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::R_OTHER));
         if (warp == F::W_TMA) {
@@ -270,45 +284,39 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                 int tiles = 0;
 #pragma unroll
                 for (int t = 0; t < NT; t++) tiles += nt[t] > 0;
+                // Stage x % ST of the ring holds K of tile x and V of tile
+                // x - 1, what one round of the products needs.
+                auto load = [&](const CUtensorMap *tm, int base, int x, int tile) {
+                    for (int c = 0; c < NC; c++)
+                        ptx::tma_load_3d(sm + base + (x % ST) * F::KV_BYTES + c * (GA_KEYS * 128), tm, full + x % ST, c * 64,
+                                         hk, k0 + tile * GA_KEYS);
+                };
                 ptx::mbar_arrive_expect_tx(qfull, (uint32_t)tiles * NC * qrows * 128);
+                ptx::mbar_arrive_expect_tx(full, F::KV_BYTES);
+                load(&tm_k, F::OFF_K, 0, 0);
 #pragma unroll
                 for (int t = 0; t < NT; t++)
                     for (int c = 0; nt[t] > 0 && c < NC; c++)
                         ptx::tma_load_4d(sm + t * F::Q_BYTES + c * (GA_ROWS * 128), &tm_q, qfull, c * 64, 0, hk,
                                          q0 + tok0 + t * TT);
-                int j = 0;
-                for (; j < nmax; j++) {
-                    const int st = j % ST;
-                    const uint32_t ph = (uint32_t)(j / ST - 1) & 1;
-                    if (j >= ST && !ga_wait(kfree + st, ph, gave_up)) {
+                int x = 1;
+                for (; x <= nmax; x++) {
+                    if (x >= ST && !ga_wait(free_ + x % ST, (uint32_t)(x / ST - 1) & 1, gave_up)) {
                         ok = false;
-                        break;
-                    }
-                    ptx::mbar_arrive_expect_tx(kfull + st, F::KV_BYTES);
-                    for (int c = 0; c < NC; c++)
-                        ptx::tma_load_3d(sm + F::OFF_K + st * F::KV_BYTES + c * (GA_KEYS * 128), &tm_k, kfull + st, c * 64,
-                                         hk, k0 + j * GA_KEYS);
-                    if (j >= ST && !ga_wait(vfree + st, ph, gave_up)) {
-                        ok = false;
-                        j++;
                         break;
                     }
                     // warps 10, 11 come to a stage out of step with its
                     // phases: this one lets them at the tile's own
-                    if (j >= edge) ptx::mbar_arrive(vgo + st);
-                    ptx::mbar_arrive_expect_tx(vfull + st, F::KV_BYTES);
-                    for (int c = 0; c < NC; c++)
-                        ptx::tma_load_3d(sm + F::OFF_V + st * F::KV_BYTES + c * (GA_KEYS * 128), &tm_v, vfull + st, c * 64,
-                                         hk, k0 + j * GA_KEYS);
+                    if (x - 1 >= edge) ptx::mbar_arrive(vgo + x % ST);
+                    ptx::mbar_arrive_expect_tx(full + x % ST, (x < nmax ? 2 : 1) * F::KV_BYTES);
+                    if (x < nmax) load(&tm_k, F::OFF_K, x, x);
+                    load(&tm_v, F::OFF_V, x, x - 1);
                 }
                 if (!ok) {
                     // copies in flight land before the CTA leaves
                     atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
                     ptx::mbar_wait(qfull, 0, 200000000LL);
-                    for (int i = max(0, j - ST); i < j; i++) {
-                        ptx::mbar_wait(kfull + i % ST, (uint32_t)(i / ST) & 1, 200000000LL);
-                        if (i < j - 1) ptx::mbar_wait(vfull + i % ST, (uint32_t)(i / ST) & 1, 200000000LL);
-                    }
+                    for (int i = max(0, x - ST); i < x; i++) ptx::mbar_wait(full + i % ST, (uint32_t)(i / ST) & 1, 200000000LL);
                 }
             }
         } else if (warp == F::W_MMA) {
@@ -326,26 +334,24 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                     ptx::mma_commit(sfull + t);
                 };
                 auto pv = [&](int t, int j, int part) {  // keys 64 part ..
-                    const uint64_t vd = ptx::smem_desc(ptx::smem_u32(sm + F::OFF_V + (j % ST) * F::KV_BYTES),
+                    const uint64_t vd = ptx::smem_desc(ptx::smem_u32(sm + F::OFF_V + ((j + 1) % ST) * F::KV_BYTES),
                                                        GA_KEYS * 128, 1024, ptx::UMMA_SW128);
 #pragma unroll
                     for (int kk = 4 * part; kk < 4 * part + 4; kk++)
                         ptx::mma_bf16_ta(tmem + F::O_COL + t * HDP, tmem + t * 128 + kk * 8, vd + (uint64_t)(kk * 2048 >> 4), ID_PV,
                                          j > 0 || kk > 0);
                 };
-                bool ok = ga_wait(qfull, 0, gave_up) && ga_wait(kfull, 0, gave_up);
+                bool ok = ga_wait(qfull, 0, gave_up) && ga_wait(full, 0, gave_up);
                 if (ok) {
                     ptx::tc_fence_after();
 #pragma unroll
                     for (int t = 0; t < NT; t++)
                         if (nt[t] > 0) qk(t, 0);
-                    ptx::mma_commit(kfree);
+                    ptx::mma_commit(free_);
                 }
                 for (int j = 0; ok && j < nmax; j++) {
-                    const int st = j % ST;
-                    const bool more = j + 1 < nmax;
-                    bool next = false;  // the next K tile is here
-                    ok = ga_wait(vfull + st, (uint32_t)(j / ST) & 1, gave_up) &&
+                    const int st = (j + 1) % ST;
+                    ok = ga_wait(full + st, (uint32_t)((j + 1) / ST) & 1, gave_up) &&
                          (j < edge || ga_wait(vok + st, (uint32_t)((j - edge) / ST) & 1, gave_up));
 #pragma unroll
                     for (int t = 0; t < NT; t++)
@@ -358,18 +364,10 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                             if (!ok) break;
                             ptx::tc_fence_after();
                             pv(t, j, 1);
-                            if (j + 1 == nt[t]) {
-                                ptx::mma_commit(ofull + t);
-                                continue;
-                            }
-                            if (!next) ok = next = ga_wait(kfull + (j + 1) % ST, (uint32_t)((j + 1) / ST) & 1, gave_up);
-                            if (!ok) break;
-                            qk(t, j + 1);  // in order behind the product that reads P from S's columns
+                            if (j + 1 == nt[t]) ptx::mma_commit(ofull + t);
+                            else qk(t, j + 1);  // in order behind the product that reads P from S's columns
                         }
-                    if (ok) {
-                        ptx::mma_commit(vfree + st);
-                        if (more) ptx::mma_commit(kfree + (j + 1) % ST);
-                    }
+                    if (ok) ptx::mma_commit(free_ + st);
                 }
                 if (!ok) {
                     atomicOr(a.dev_err, WB_DERR_TIMEOUT_MMA);
@@ -383,30 +381,36 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
             // each swizzle atom each
             const int x = tid - F::W_FIX * 32;
             const uint32_t step = BF ? 0x00800080u : 0x04000400u;  // carries out of a full exponent field
+            auto bad = [&](uint32_t w) { return ((w & 0x7fff7fffu) + step) & 0x80008000u; };
+            auto clean = [&](uint32_t w) {
+                const uint32_t m = bad(w);
+                return w & ~((m & 0x8000u ? 0xffffu : 0u) | (m & 0x80000000u ? 0xffff0000u : 0u));
+            };
             for (int j = edge; j < nmax; j++) {
-                const int st = j % ST, left = nk - j * GA_KEYS;
+                const int st = (j + 1) % ST, left = nk - j * GA_KEYS;
                 if (!ga_wait(vgo + st, (uint32_t)((j - edge) / ST) & 1, gave_up) ||
-                    !ga_wait(vfull + st, (uint32_t)(j / ST) & 1, gave_up)) {
+                    !ga_wait(full + st, (uint32_t)((j + 1) / ST) & 1, gave_up)) {
                     if (lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
                     break;
                 }
-                for (int i = 0; i < NC * 16; i++) {
-                    const int row = (x >> 3) + 8 * (i & 15);
-                    uint4 *p = reinterpret_cast<uint4 *>(sm + F::OFF_V + st * F::KV_BYTES + (i >> 4) * (GA_KEYS * 128) +
-                                                         row * 128 + (x & 7) * 16);
-                    if (row >= left) {
-                        *p = make_uint4(0, 0, 0, 0);
-                        continue;
-                    }
-                    uint4 v = *p;
-                    auto bad = [&](uint32_t w) { return ((w & 0x7fff7fffu) + step) & 0x80008000u; };
-                    if (bad(v.x) | bad(v.y) | bad(v.z) | bad(v.w)) {
-                        auto clean = [&](uint32_t w) {
-                            const uint32_t m = bad(w);
-                            return w & ~((m & 0x8000u ? 0xffffu : 0u) | (m & 0x80000000u ? 0xffff0000u : 0u));
-                        };
-                        *p = make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
-                        atomicOr(&s_bad[j - edge][row >> 5], 1u << (row & 31));
+                uint8_t *v0 = sm + F::OFF_V + st * F::KV_BYTES + (x >> 3) * 128 + (x & 7) * 16;
+                for (int i0 = 0; i0 < NC * 16; i0 += 8) {  // rows x / 8 + 8 i of an atom
+                    uint4 v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = *reinterpret_cast<const uint4 *>(v0 + (i0 + i) * 1024);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int row = (x >> 3) + 8 * ((i0 + i) & 15);
+                        const bool past = row >= left;
+                        if (past || (bad(v[i].x) | bad(v[i].y) | bad(v[i].z) | bad(v[i].w))) {
+                            *reinterpret_cast<uint4 *>(v0 + (i0 + i) * 1024) =
+                                past ? make_uint4(0, 0, 0, 0)
+                                     : make_uint4(clean(v[i].x), clean(v[i].y), clean(v[i].z), clean(v[i].w));
+                            if (!past) {
+                                atomicOr(&s_bad[j - edge][row >> 5], 1u << (row & 31));
+                                s_any_bad = 1;
+                            }
+                        }
                     }
                 }
                 ptx::fence_proxy_async_smem();
@@ -518,19 +522,27 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
             const bool none = vis == 0;
             const float inv = 1.0f / l;
             const int h = hk * G + g;
-            T *out = (T *)a.out + (long long)(q0 + tok) * a.o_ts + (long long)h * a.o_hs;
+            const long long at = (long long)(q0 + tok) * a.o_ts + (long long)h * a.o_hs;  // the row's place in out
             // keys noted at the edges that this row sees
-            bool noted = false;
             const int edges = max(0, mine - edge);  // all of them multiplied by now
-            for (int e = max(0, edges - ST); e < edges; e++) ga_wait(vok + (edge + e) % ST, (uint32_t)(e / ST) & 1, gave_up);
-            for (int e = 0; e < edges; e++)
-                for (int w = 0; w < GA_KEYS / 32; w++) noted |= s_bad[e][w] != 0;
+            for (int e = max(0, edges - ST); e < edges; e++)
+                if (!ga_wait(vok + (edge + e + 1) % ST, (uint32_t)(e / ST) & 1, gave_up) && lane == 0)
+                    atomicOr(a.dev_err, WB_DERR_TIMEOUT_SOFTMAX);
+            const bool noted = s_any_bad;
+            // Through shared memory, so that a store instruction writes whole
+            // rows (a thread per row took 4.5 us): this tile's query rows
+            // are not read any more.  16-byte piece c of a row at place
+            // c ^ (row & 7) of its 128 bytes.
+            constexpr int RB = HDP * 2, PPR = HDP / 8;
+            uint8_t *stage = sm + t * F::Q_BYTES + (row & 96) * RB;
 #pragma unroll 1
-            for (int x = 0; x < HDP / 32 && mine > 0; x++) {
+            for (int x = 0; x < HDP / 32; x++) {
                 uint32_t o[32];
                 __syncwarp();
-                ptx::tmem_ld32(O + 32 * x, o);
-                ptx::tmem_ld_wait();
+                if (mine > 0) {
+                    ptx::tmem_ld32(O + 32 * x, o);
+                    ptx::tmem_ld_wait();
+                }
                 if (noted && real) {
                     for (int e = 0; e < edges; e++)
                         for (int i = 0; i < GA_KEYS; i++) {
@@ -547,26 +559,35 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                 }
 #pragma unroll
                 for (int i = 0; i < 32; i++) o[i] = none ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
-                if (!real) {
-                } else if (ga.vec) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (32 * x + 8 * i < a.hd) {
-                            uint4 w;
-                            w.x = ga_pack<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]));
-                            w.y = ga_pack<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
-                            w.z = ga_pack<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
-                            w.w = ga_pack<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
-                            *reinterpret_cast<uint4 *>(out + 32 * x + 8 * i) = w;
-                        }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (32 * x + i < a.hd) out[32 * x + i] = from_f<T>(__uint_as_float(o[i]));
+                for (int i = 0; i < 4; i++) {
+                    uint4 w;
+                    w.x = ga_pack<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]));
+                    w.y = ga_pack<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
+                    w.z = ga_pack<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
+                    w.w = ga_pack<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
+                    *reinterpret_cast<uint4 *>(stage + lane * RB + ((4 * x + i) ^ (lane & 7)) * 16) = w;
                 }
             }
-            if (real && mine == 0)
-                for (int d = 0; d < a.hd; d++) out[d] = from_f<T>(0.0f);
+            __syncwarp();
+            const uint32_t rows = __ballot_sync(0xffffffffu, real);
+            if (ga.vec) {
+                const int c = lane % PPR;
+#pragma unroll
+                for (int i = 0; i < PPR; i++) {
+                    const int r = i * (32 / PPR) + lane / PPR;
+                    const long long to = __shfl_sync(0xffffffffu, at, r);
+                    if ((rows >> r & 1) && 8 * c < a.hd)
+                        *reinterpret_cast<uint4 *>((T *)a.out + to + 8 * c) =
+                            *reinterpret_cast<const uint4 *>(stage + r * RB + (c ^ (r & 7)) * 16);
+                }
+            } else {
+                for (int r = 0; r < 32; r++) {
+                    const long long to = __shfl_sync(0xffffffffu, at, r);
+                    for (int d = lane; (rows >> r & 1) && d < a.hd; d += 32)
+                        ((T *)a.out)[to + d] = *reinterpret_cast<const T *>(stage + r * RB + ((d >> 3) ^ (r & 7)) * 16 + (d & 7) * 2);
+                }
+            }
             if (real && a.lse)
                 a.lse[(long long)h * a.total_q + q0 + tok] = none ? -INFINITY : (log2f(l) - off) * 0.6931471805599453f;
         }
