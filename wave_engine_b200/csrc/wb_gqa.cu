@@ -38,12 +38,22 @@ struct GaArgs {
     float c;      // |scale| log2 e, at least 1e-30
     int G, TT;    // heads per key-value head, tokens of a query tile
     int vec;      // out rows take 16-byte stores
+    long long items;  // no more than this many (sequence, tiles) items
 };
+
+// A work item: two query tiles of one key-value head.
+struct GaItem {
+    int q0, nq, k0, nk;      // the sequence's rows; q0 < 0: no more work
+    int tok0, hk;            // first token of the first tile, key-value head
+    int nt[2], edge;         // key tiles of each query tile, the first that some row sees in part
+    uint32_t any_bad, bad[GA_EDGES][GA_KEYS / 32];  // keys from tile `edge` on with values that are not finite
+};
+static constexpr int GA_SLOTS = 4;  // items known to the CTA's roles at a time
 
 template <int HDP>
 struct GaConf {
     static constexpr int NT = 2;  // query tiles of a CTA
-    static constexpr int W_TMA = 4 * NT, W_MMA = W_TMA + 1, W_FIX = W_TMA + 2;  // warps before: softmax
+    static constexpr int W_TMA = 4 * NT, W_MMA = W_TMA + 1, W_FIX = W_MMA + 1;  // warps before: softmax
     static constexpr int THREADS = (W_FIX + 2) * 32;
     // registers: the softmax warps take what the other four give up
     static constexpr int R_SOFTMAX = 200, R_OTHER = 104;
@@ -52,10 +62,14 @@ struct GaConf {
     static constexpr int Q_BYTES = GA_ROWS * HDP * 2;
     static constexpr int KV_BYTES = GA_KEYS * HDP * 2;
     static constexpr int ST = HDP == 64 ? 4 : 2;  // K/V stages
-    static constexpr int OFF_K = NT * Q_BYTES, OFF_V = OFF_K + ST * KV_BYTES, OFF_BAR = OFF_V + ST * KV_BYTES;
-    static constexpr int NBAR = 4 * ST + 4 * NT + 2;
-    static constexpr int BYTES = OFF_BAR + NBAR * 8 + 1024;
-    static_assert(BYTES + 1536 <= 227 * 1024, "shared memory");
+    static constexpr int OFF_K = NT * Q_BYTES, OFF_V = OFF_K + ST * KV_BYTES;
+    static constexpr int OFF_OUT = OFF_V + ST * KV_BYTES, OUT_WARP = 32 * 64;  // a warp's 32 rows of 32 outputs
+    static constexpr int OFF_BAR = OFF_OUT + 4 * NT * OUT_WARP;
+    static constexpr int NBAR = 4 * ST + 4 * NT + 3 + 3 * GA_SLOTS;
+    static constexpr int OFF_ITEM = OFF_BAR + NBAR * 8;
+    static constexpr int BYTES = OFF_ITEM + GA_SLOTS * (int)sizeof(GaItem) + 1024;
+    static_assert(BYTES + 1280 <= 227 * 1024, "shared memory");
+    static_assert(OFF_OUT % 128 == 0 && OFF_BAR % 16 == 0, "alignment");
 };
 
 // Bounded mbarrier wait that also gives up once another role has: a timeout
@@ -105,6 +119,24 @@ __device__ __forceinline__ void ga_st32(uint32_t taddr, const uint32_t (&r)[32])
         : "memory");
 }
 
+// tcgen05.mma with A from shared memory or TMEM; descriptors as low and high
+// words
+template <bool ACC>
+__device__ __forceinline__ void ga_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc) {
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "n"(ACC ? 1 : 0)
+        : "memory");
+}
+__device__ __forceinline__ void ga_mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 b;\n mov.b64 b, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+        "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
+
 // Items (NT query tiles each) of a sequence; 0, flagged, when its rows do
 // not lie inside the tensors.
 __device__ __forceinline__ int ga_items(const GqaAttnArgs &a, int b, int per_item) {
@@ -116,80 +148,81 @@ __device__ __forceinline__ int ga_items(const GqaAttnArgs &a, int b, int per_ite
     return (q1 - q0 + per_item - 1) / per_item;
 }
 
-// The sequence and tile pair of the `index`-th item; false past the last.
-// Up to 256 sequences: pairs late in their sequences (with the most keys)
-// first -- the largest t with more than `index` items at or behind pair t,
-// then by sequence -- so that the last CTAs to start are short.  More: in the
-// order of the sequences, in one pass.  Run by one warp.
-__device__ __forceinline__ bool ga_find(const GqaAttnArgs &a, int per_item, long long index, int lane, int *seq, int *pair) {
-    constexpr int N = 8;
-    if (a.n_seq > 32 * N) {
-        long long before = 0;
-        for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
-            const int n = b0 + lane < a.n_seq ? ga_items(a, b0 + lane, per_item) : 0;
-            int inc = n;
+// Finds the sequence and tiles of ascending item indexes; one warp.  Up to
+// 256 sequences: tiles late in their sequences (with the most keys) first --
+// the largest t with more than `index` items at or behind place t, then by
+// sequence -- so that long items are dealt out first.  More: in the order of
+// the sequences, one pass over them for all items of the CTA.
+struct GaFinder {
+    static constexpr int N = 8;
+    int n[N];                // items of sequences lane + 32 x (or of sequences b0 + lane, in n[0])
+    int top = 0, b0 = 0;
+    long long before = 0;    // items of sequences before b0
+    __device__ __forceinline__ void start(const GqaAttnArgs &a, int per_item, int lane) {
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += y;
-            }
-            const uint32_t past = __ballot_sync(0xffffffffu, before + inc > index);
-            if (past) {
-                const int at = __ffs(past) - 1;
-                *seq = b0 + at;
-                *pair = (int)(index - before) - __shfl_sync(0xffffffffu, inc - n, at);
-                return true;
-            }
-            before += __shfl_sync(0xffffffffu, inc, 31);
+        for (int x = 0; x < N; x++) {
+            n[x] = lane + 32 * x < a.n_seq ? ga_items(a, lane + 32 * x, per_item) : 0;
+            top = max(top, n[x]);
         }
-        return false;
+        top = __reduce_max_sync(0xffffffffu, top);
     }
-    int n[N];
-    int hi = 0;
-#pragma unroll
-    for (int x = 0; x < N; x++) {
-        n[x] = lane + 32 * x < a.n_seq ? ga_items(a, lane + 32 * x, per_item) : 0;
-        hi = max(hi, n[x]);
-    }
-    auto behind = [&](int t) {  // items of pairs >= t
+    __device__ __forceinline__ int behind(int t) const {  // items at places >= t
         int sum = 0;
 #pragma unroll
         for (int x = 0; x < N; x++) sum += max(0, n[x] - t);
-        return (long long)__reduce_add_sync(0xffffffffu, sum);
-    };
-    if (a.n_seq == 1) {
-        hi = __shfl_sync(0xffffffffu, n[0], 0);
-        *seq = 0;
-        *pair = hi - 1 - (int)index;
-        return index < hi;
+        return __reduce_add_sync(0xffffffffu, sum);
     }
-    if (index >= behind(0)) return false;
-    int lo = 0;
-    hi = __reduce_max_sync(0xffffffffu, hi);  // behind(lo) > index >= behind(hi)
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (behind(mid) > index) lo = mid;
-        else hi = mid;
-    }
-    int rank = (int)(index - behind(hi));
+    __device__ __forceinline__ bool find(const GqaAttnArgs &a, int per_item, long long index, int lane, int *seq, int *place) {
+        if (a.n_seq > 32 * N) {
+            for (;;) {
+                int inc = n[0];
 #pragma unroll
-    for (int x = 0; x < N; x++) {
-        const uint32_t has = __ballot_sync(0xffffffffu, n[x] > lo);
-        if (rank < 0) continue;
-        if (rank < __popc(has)) {
-            *seq = 32 * x + (int)__fns(has, 0, rank + 1);
-            *pair = lo;
-            rank = -1;
-        } else {
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += y;
+                }
+                const uint32_t past = __ballot_sync(0xffffffffu, before + inc > index);
+                if (past) {
+                    const int at = __ffs(past) - 1;
+                    *seq = b0 + at;
+                    *place = (int)(index - before) - __shfl_sync(0xffffffffu, inc - n[0], at);
+                    return true;
+                }
+                before += __shfl_sync(0xffffffffu, inc, 31);
+                b0 += 32;
+                if (b0 >= a.n_seq) return false;
+                n[0] = b0 + lane < a.n_seq ? ga_items(a, b0 + lane, per_item) : 0;
+            }
+        }
+        if (a.n_seq == 1) {
+            *place = top - 1 - (int)index;
+            return index < top;
+        }
+        if (index >= behind(0)) return false;
+        int lo = 0, hi = top;  // behind(lo) > index >= behind(hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (behind(mid) > index) lo = mid;
+            else hi = mid;
+        }
+        int rank = (int)(index - behind(hi));
+        *place = lo;
+#pragma unroll
+        for (int x = 0; x < N; x++) {
+            const uint32_t has = __ballot_sync(0xffffffffu, n[x] > lo);
+            if (rank >= 0 && rank < __popc(has)) *seq = 32 * x + (int)__fns(has, 0, rank + 1);
             rank -= __popc(has);
         }
+        return true;
     }
-    return true;
-}
+};
 
-// Roles: warps 0-3 and 4-7 softmax and epilogue of tiles 0 and 1 (thread =
-// row); warp 8 loads; warp 9 issues the MMAs and owns TMEM; warps 10, 11 look
-// through the V tiles at the rows' edges (below).
+// Persistent: one CTA per SM takes the items in rounds, every second round
+// backwards (the items come largest first), and its roles run ahead of each
+// other from item to item: warps 0-3 and 4-7 softmax and epilogue of tiles 0
+// and 1 (thread = row); warp 8 finds the items and loads; warp 9 issues the
+// MMAs and owns TMEM; warps 10, 11 look through the V tiles at the rows'
+// edges.
 //
 // Edges.  A key that a row does not see gets probability 0, but 0 times an
 // infinity or NaN among its values would reach the row through the MMA.  So
@@ -209,176 +242,247 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + F::OFF_BAR);
     uint64_t *full = bars, *free_ = full + ST, *vok = free_ + ST, *vgo = vok + ST;
-    uint64_t *qfull = vgo + ST, *sfull = qfull + 1, *pready = sfull + NT, *ofull = pready + 2 * NT;
+    uint64_t *qfull = vgo + ST, *qfree = qfull + 1, *done = qfree + 1;
+    uint64_t *sfull = done + 1, *pready = sfull + NT, *ofull = pready + 2 * NT;
+    uint64_t *itemfull = ofull + NT, *itemfree = itemfull + GA_SLOTS, *fixed = itemfree + GA_SLOTS;
+    GaItem *items = reinterpret_cast<GaItem *>(sm + F::OFF_ITEM);
     __shared__ uint32_t tmem_slot;
-    __shared__ int s_gave_up, s_any_bad, s_item[5];
-    __shared__ uint32_t s_bad[GA_EDGES][GA_KEYS / 32];  // keys with values that are not finite
+    __shared__ int s_gave_up;
     volatile int *gave_up = &s_gave_up;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = ga.G, TT = ga.TT;
 
-    // one barrier before the work: the loading warp finds the item, others set
-    // up TMEM and the mbarriers meanwhile
+    GaFinder finder;  // warp W_TMA's
+    int seq = 0, place = 0;
+    bool any = false;
     if (warp == F::W_TMA) {
         if (lane == 0) {
             ptx::prefetch_tmap(&tm_q);
             ptx::prefetch_tmap(&tm_k);
             ptx::prefetch_tmap(&tm_v);
         }
-        int seq = -1, group = 0;
-        const bool any = ga_find(a, NT * TT, blockIdx.x / a.Hkv, lane, &seq, &group);
-        if (lane == 0) {
-            s_item[0] = any ? __ldg(a.cu_q + seq) : -1;
-            if (any) {
-                s_item[1] = __ldg(a.cu_q + seq + 1) - s_item[0];
-                s_item[2] = __ldg(a.cu_k + seq);
-                s_item[3] = __ldg(a.cu_k + seq + 1) - s_item[2];
-                s_item[4] = group * NT * TT;
-            }
-        }
-    } else if (warp == F::W_MMA) {
-        ptx::tmem_alloc(&tmem_slot, F::TMEM);
-        ptx::tmem_relinquish();
-    } else if (warp == 0) {
+        finder.start(a, NT * TT, lane);
+        any = finder.find(a, NT * TT, blockIdx.x / a.Hkv, lane, &seq, &place);
+    }
+    if (warp == 0) {
         for (int i = lane; i < F::NBAR; i += 32) {
             uint64_t *b = bars + i;
-            ptx::mbar_init(b, b >= vok && b < vok + ST ? 2 : b >= pready && b < pready + 2 * NT ? 4 : 1);
+            int n = 1;
+            if (b >= vok && b < vok + ST) n = 2;
+            else if (b >= pready && b < pready + 2 * NT) n = 4;
+            else if (b >= itemfree && b < itemfree + GA_SLOTS) n = 4 * NT + 3;
+            else if (b >= fixed) n = 2;
+            ptx::mbar_init(b, n);
         }
         ptx::fence_mbar_init();
         if (lane == 0) s_gave_up = 0;
-    } else if (warp == 1) {
-        if (lane < GA_EDGES * GA_KEYS / 32) (&s_bad[0][0])[lane] = 0;
-        if (lane == 31) s_any_bad = 0;
+    }
+    if (warp == F::W_MMA) {
+        ptx::tmem_alloc(&tmem_slot, F::TMEM);
+        ptx::tmem_relinquish();
     }
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    const int q0 = s_item[0], nq = s_item[1], k0 = s_item[2], nk = s_item[3];
-    if (q0 < 0) {  // no such item
-        if (warp == F::W_MMA) ptx::tmem_dealloc(tmem, F::TMEM);
-        return;
-    }
-    const int hk = blockIdx.x % a.Hkv;
-    const int tok0 = s_item[4];  // first token of tile 0
-    // keys that token t sees
-    auto visible = [&](int t) {
+    // keys that token t of an item's sequence sees
+    auto visible = [&](int nq, int nk, int t) {
         const long long n = a.causal ? (long long)t + 1 + nk - nq : nk;
         return (int)max(0LL, min((long long)nk, n));
     };
-    // key tiles of each query tile, and the first that some row sees in part
-    int nt[NT], nmax = 0;
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        nt[t] = tok0 + t * TT < nq ? (visible(min(tok0 + (t + 1) * TT, nq) - 1) + GA_KEYS - 1) / GA_KEYS : 0;
-        nmax = max(nmax, nt[t]);
-    }
-    const int edge = visible(tok0) / GA_KEYS;
 
     if (warp >= F::W_TMA) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::R_OTHER));
         if (warp == F::W_TMA) {
-            if (lane == 0 && nmax > 0) {
-                bool ok = true;
-                const int qrows = G * TT;
-                int tiles = 0;
+            // ---- items and loads
+            uint32_t g = 0, nq_loads = 0;  // ring stages and Q pairs loaded
+            bool ok = true;
+            for (int k = 0;; k++) {
+                const long long index = (long long)k * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                if (k > 0) any = index < ga.items * a.Hkv && finder.find(a, NT * TT, index / a.Hkv, lane, &seq, &place);
+                GaItem *it = items + k % GA_SLOTS;
+                if (k >= GA_SLOTS && !ga_wait(itemfree + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS - 1) & 1, gave_up)) {
+                    if (lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
+                    ok = false;
+                    break;
+                }
+                if (lane <= GA_EDGES * GA_KEYS / 32) (&it->any_bad)[lane] = 0;
+                const int q0 = any ? __ldg(a.cu_q + seq) : -1, nq = any ? __ldg(a.cu_q + seq + 1) - q0 : 0;
+                const int k0 = any ? __ldg(a.cu_k + seq) : 0, nk = any ? __ldg(a.cu_k + seq + 1) - k0 : 0;
+                const int hk = (int)(index % a.Hkv), tok0 = place * NT * TT;
+                int nt[NT], nmax = 0;
 #pragma unroll
-                for (int t = 0; t < NT; t++) tiles += nt[t] > 0;
-                // Stage x % ST of the ring holds K of tile x and V of tile
-                // x - 1, what one round of the products needs.
-                auto load = [&](const CUtensorMap *tm, int base, int x, int tile) {
-                    for (int c = 0; c < NC; c++)
-                        ptx::tma_load_3d(sm + base + (x % ST) * F::KV_BYTES + c * (GA_KEYS * 128), tm, full + x % ST, c * 64,
-                                         hk, k0 + tile * GA_KEYS);
-                };
-                ptx::mbar_arrive_expect_tx(qfull, (uint32_t)tiles * NC * qrows * 128);
-                ptx::mbar_arrive_expect_tx(full, F::KV_BYTES);
-                load(&tm_k, F::OFF_K, 0, 0);
+                for (int t = 0; t < NT; t++) {
+                    const int last = min(tok0 + (t + 1) * TT, nq) - 1;
+                    nt[t] = tok0 + t * TT < nq ? (visible(nq, nk, last) + GA_KEYS - 1) / GA_KEYS : 0;
+                    nmax = max(nmax, nt[t]);
+                }
+                const int edge = visible(nq, nk, tok0) / GA_KEYS;
+                __syncwarp();
+                if (lane == 0) {
+                    it->q0 = q0;
+                    it->nq = nq;
+                    it->k0 = k0;
+                    it->nk = nk;
+                    it->tok0 = tok0;
+                    it->hk = hk;
+                    it->nt[0] = nt[0];
+                    it->nt[1] = nt[1];
+                    it->edge = edge;
+                    ptx::mbar_arrive(itemfull + k % GA_SLOTS);
+                }
+                if (!any) break;
+                if (lane == 0 && nmax > 0) {
+                    // Stage g of the ring holds K of the item's tile x and V
+                    // of tile x - 1, what one round of the products needs.
+                    for (int x = 0; ok && x <= nmax; x++) {
+                        const int st = (int)(g % ST);
+                        if (g >= ST && !ga_wait(free_ + st, (g / ST - 1) & 1, gave_up)) {
+                            ok = false;
+                            break;
+                        }
+                        // warps 10, 11 come to a stage out of step with its
+                        // phases: this one lets them at the tile's own
+                        if (x > edge) ptx::mbar_arrive(vgo + st);
+                        ptx::mbar_arrive_expect_tx(full + st, ((x < nmax) + (x > 0)) * F::KV_BYTES);
+                        g++;
+                        for (int c = 0; x < nmax && c < NC; c++)
+                            ptx::tma_load_3d(sm + F::OFF_K + st * F::KV_BYTES + c * (GA_KEYS * 128), &tm_k, full + st,
+                                             c * 64, hk, k0 + x * GA_KEYS);
+                        for (int c = 0; x > 0 && c < NC; c++)
+                            ptx::tma_load_3d(sm + F::OFF_V + st * F::KV_BYTES + c * (GA_KEYS * 128), &tm_v, full + st,
+                                             c * 64, hk, k0 + (x - 1) * GA_KEYS);
+                        if (x > 0) continue;
+                        if (nq_loads > 0) ok = ga_wait(qfree, (nq_loads - 1) & 1, gave_up);
+                        if (!ok) break;
+                        int tiles = 0;
 #pragma unroll
-                for (int t = 0; t < NT; t++)
-                    for (int c = 0; nt[t] > 0 && c < NC; c++)
-                        ptx::tma_load_4d(sm + t * F::Q_BYTES + c * (GA_ROWS * 128), &tm_q, qfull, c * 64, 0, hk,
-                                         q0 + tok0 + t * TT);
-                int x = 1;
-                for (; x <= nmax; x++) {
-                    if (x >= ST && !ga_wait(free_ + x % ST, (uint32_t)(x / ST - 1) & 1, gave_up)) {
-                        ok = false;
-                        break;
+                        for (int t = 0; t < NT; t++) tiles += nt[t] > 0;
+                        ptx::mbar_arrive_expect_tx(qfull, (uint32_t)(tiles * NC * G * TT * 128));
+#pragma unroll
+                        for (int t = 0; t < NT; t++)
+                            for (int c = 0; nt[t] > 0 && c < NC; c++)
+                                ptx::tma_load_4d(sm + t * F::Q_BYTES + c * (GA_ROWS * 128), &tm_q, qfull, c * 64, 0, hk,
+                                                 q0 + tok0 + t * TT);
+                        nq_loads++;
                     }
-                    // warps 10, 11 come to a stage out of step with its
-                    // phases: this one lets them at the tile's own
-                    if (x - 1 >= edge) ptx::mbar_arrive(vgo + x % ST);
-                    ptx::mbar_arrive_expect_tx(full + x % ST, (x < nmax ? 2 : 1) * F::KV_BYTES);
-                    if (x < nmax) load(&tm_k, F::OFF_K, x, x);
-                    load(&tm_v, F::OFF_V, x, x - 1);
+                    if (!ok) {
+                        // copies in flight land before the CTA leaves
+                        atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
+                        if (nq_loads > 0) ptx::mbar_wait(qfull, (nq_loads - 1) & 1, 200000000LL);
+                        for (uint32_t i = g > ST ? g - ST : 0; i < g; i++)
+                            ptx::mbar_wait(full + i % ST, (i / ST) & 1, 200000000LL);
+                    }
                 }
-                if (!ok) {
-                    // copies in flight land before the CTA leaves
-                    atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
-                    ptx::mbar_wait(qfull, 0, 200000000LL);
-                    for (int i = max(0, x - ST); i < x; i++) ptx::mbar_wait(full + i % ST, (uint32_t)(i / ST) & 1, 200000000LL);
-                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
             }
         } else if (warp == F::W_MMA) {
-            if (lane == 0 && nmax > 0) {
+            // ---- products.  The whole warp goes through the loop, one lane
+            // issues: counters and stages then stay in uniform registers,
+            // where the MMAs want their descriptors.
+            {
                 constexpr uint32_t ID_QK = BF ? ptx::idesc_bf16(128, 128, 0, 0) : ptx::idesc_f16(128, 128, 0, 0);
                 constexpr uint32_t ID_PV = BF ? ptx::idesc_bf16(128, HDP, 0, 1) : ptx::idesc_f16(128, HDP, 0, 1);
-                auto qk = [&](int t, int j) {
-                    const uint64_t ad = ptx::smem_desc(ptx::smem_u32(sm + t * F::Q_BYTES), 16, 1024, ptx::UMMA_SW128);
-                    const uint64_t bd = ptx::smem_desc(ptx::smem_u32(sm + F::OFF_K + (j % ST) * F::KV_BYTES), 16, 1024,
-                                                       ptx::UMMA_SW128);
+                // Descriptors: the low words change, by constants within a
+                // product; few instructions stand between a barrier and the
+                // first product behind it.
+                const uint32_t hi = 1024 / 16 | 1u << 14 | ptx::UMMA_SW128 << 29;
+                const uint32_t q_lo = ptx::smem_u32(sm) >> 4 | 1u << 16, k_lo = ptx::smem_u32(sm + F::OFF_K) >> 4 | 1u << 16;
+                const uint32_t v_lo = ptx::smem_u32(sm + F::OFF_V) >> 4 | (GA_KEYS * 128 / 16) << 16;
+                auto qk = [&](int t, int st) {
+                    const uint32_t q = q_lo + t * (F::Q_BYTES / 16), kd = k_lo + st * (F::KV_BYTES / 16);
+                    if (lane == 0) {
 #pragma unroll
-                    for (int kk = 0; kk < HDP / 16; kk++)
-                        ptx::mma_bf16(tmem + t * 128, ad + (uint64_t)((kk >> 2) * (GA_ROWS * 8) + (kk & 3) * 2),
-                                      bd + (uint64_t)((kk >> 2) * (GA_KEYS * 8) + (kk & 3) * 2), ID_QK, kk > 0);
-                    ptx::mma_commit(sfull + t);
+                        for (int kk = 0; kk < HDP / 16; kk++) {
+                            const uint32_t o = (kk >> 2) * (GA_ROWS * 8) + (kk & 3) * 2;
+                            if (kk == 0) ga_mma_ss<false>(tmem + t * 128, q + o, kd + o, hi, ID_QK);
+                            else ga_mma_ss<true>(tmem + t * 128, q + o, kd + o, hi, ID_QK);
+                        }
+                        ptx::mma_commit(sfull + t);
+                    }
+                    __syncwarp();
                 };
-                auto pv = [&](int t, int j, int part) {  // keys 64 part ..
-                    const uint64_t vd = ptx::smem_desc(ptx::smem_u32(sm + F::OFF_V + ((j + 1) % ST) * F::KV_BYTES),
-                                                       GA_KEYS * 128, 1024, ptx::UMMA_SW128);
+                auto pv = [&](int t, int st, int part, bool first) {  // keys 64 part ..
+                    const uint32_t v = v_lo + st * (F::KV_BYTES / 16), S = tmem + t * 128, O = tmem + F::O_COL + t * HDP;
+                    if (lane == 0) {
 #pragma unroll
-                    for (int kk = 4 * part; kk < 4 * part + 4; kk++)
-                        ptx::mma_bf16_ta(tmem + F::O_COL + t * HDP, tmem + t * 128 + kk * 8, vd + (uint64_t)(kk * 2048 >> 4), ID_PV,
-                                         j > 0 || kk > 0);
+                        for (int kk = 4 * part; kk < 4 * part + 4; kk++) {
+                            if (kk == 0) ga_mma_ts(O, S, v, hi, ID_PV, !first);
+                            else ga_mma_ts(O, S + kk * 8, v + kk * (2048 / 16), hi, ID_PV, true);
+                        }
+                    }
+                    __syncwarp();
                 };
-                bool ok = ga_wait(qfull, 0, gave_up) && ga_wait(full, 0, gave_up);
-                if (ok) {
+                auto commit = [&](uint64_t *bar) {
+                    if (lane == 0) ptx::mma_commit(bar);
+                    __syncwarp();
+                };
+                auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+                uint32_t g = 0, n_q = 0, n_p[NT] = {}, vok_ph = 0;
+                bool ok = true;
+                for (int k = 0;; k++) {
+                    ok = __all_sync(0xffffffffu, ok && ga_wait(itemfull + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS) & 1, gave_up));
+                    if (!ok) break;
+                    const GaItem *it = items + k % GA_SLOTS;
+                    if ((int)uniform(it->q0) < 0) break;
+                    const int nt[NT] = {(int)uniform(it->nt[0]), (int)uniform(it->nt[1])};
+                    const int nmax = max(nt[0], nt[1]), edge = uniform(it->edge);
+                    if (lane == 0) ptx::mbar_arrive(itemfree + k % GA_SLOTS);
+                    __syncwarp();
+                    if (nmax == 0) continue;
+                    g = uniform(g);
+                    vok_ph = uniform(vok_ph);
+                    ok = ga_wait(qfull, n_q++ & 1, gave_up) && ga_wait(full + g % ST, (g / ST) & 1, gave_up);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) n_p[t] = uniform(n_p[t]);
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        ok = false;
+                        continue;  // and out
+                    }
                     ptx::tc_fence_after();
 #pragma unroll
                     for (int t = 0; t < NT; t++)
-                        if (nt[t] > 0) qk(t, 0);
-                    ptx::mma_commit(free_);
-                }
-                for (int j = 0; ok && j < nmax; j++) {
-                    const int st = (j + 1) % ST;
-                    ok = ga_wait(full + st, (uint32_t)((j + 1) / ST) & 1, gave_up) &&
-                         (j < edge || ga_wait(vok + st, (uint32_t)((j - edge) / ST) & 1, gave_up));
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-                        if (ok && j < nt[t]) {
-                            ok = ga_wait(pready + 2 * t, (uint32_t)j & 1, gave_up);
-                            if (!ok) break;
-                            ptx::tc_fence_after();
-                            pv(t, j, 0);
-                            ok = ga_wait(pready + 2 * t + 1, (uint32_t)j & 1, gave_up);
-                            if (!ok) break;
-                            ptx::tc_fence_after();
-                            pv(t, j, 1);
-                            if (j + 1 == nt[t]) ptx::mma_commit(ofull + t);
-                            else qk(t, j + 1);  // in order behind the product that reads P from S's columns
+                        if (nt[t] > 0) qk(t, (int)(g % ST));
+                    commit(free_ + g % ST);
+                    g++;
+                    if (nmax == 1) commit(qfree);
+                    for (int j = 0; j < nmax; j++, g++) {
+                        const int st = (int)(g % ST);
+                        ok = ok && ga_wait(full + st, (g / ST) & 1, gave_up);
+                        if (j >= edge) {
+                            ok = ok && ga_wait(vok + st, (vok_ph >> st) & 1, gave_up);
+                            vok_ph ^= 1u << st;
                         }
-                    if (ok) ptx::mma_commit(free_ + st);
+                        // after a timeout the products go on for nothing to
+                        // the item's end: every wait returns at once
+#pragma unroll
+                        for (int t = 0; t < NT; t++)
+                            if (j < nt[t]) {
+                                ok = ok && ga_wait(pready + 2 * t, n_p[t] & 1, gave_up);
+                                ptx::tc_fence_after();
+                                pv(t, st, 0, j == 0);  // the warps that gave P have read the item's before O
+                                ok = ok && ga_wait(pready + 2 * t + 1, n_p[t]++ & 1, gave_up);
+                                ptx::tc_fence_after();
+                                pv(t, st, 1, j == 0);
+                                if (j + 1 == nt[t]) commit(ofull + t);
+                                else qk(t, st);  // in order behind the product that reads P from S's columns
+                            }
+                        commit(free_ + st);
+                        if (j + 2 == nmax) commit(qfree);
+                    }
                 }
-                if (!ok) {
+                if (!ok && lane == 0) {
                     atomicOr(a.dev_err, WB_DERR_TIMEOUT_MMA);
                     // the MMAs issued have completed before TMEM is released
-                    ptx::mma_commit(bars + F::NBAR - 1);
-                    ptx::mbar_wait(bars + F::NBAR - 1, 0, 200000000LL);
+                    ptx::mma_commit(done);
+                    ptx::mbar_wait(done, 0, 200000000LL);
                 }
+                __syncwarp();
             }
         } else {
-            // V tiles at the edges: 8 threads per row, one 16-byte piece of
-            // each swizzle atom each
+            // ---- V tiles at the edges: 8 threads per row, one 16-byte piece
+            // of each swizzle atom each
             const int x = tid - F::W_FIX * 32;
             const uint32_t step = BF ? 0x00800080u : 0x04000400u;  // carries out of a full exponent field
             auto bad = [&](uint32_t w) { return ((w & 0x7fff7fffu) + step) & 0x80008000u; };
@@ -386,37 +490,51 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                 const uint32_t m = bad(w);
                 return w & ~((m & 0x8000u ? 0xffffu : 0u) | (m & 0x80000000u ? 0xffff0000u : 0u));
             };
-            for (int j = edge; j < nmax; j++) {
-                const int st = (j + 1) % ST, left = nk - j * GA_KEYS;
-                if (!ga_wait(vgo + st, (uint32_t)((j - edge) / ST) & 1, gave_up) ||
-                    !ga_wait(full + st, (uint32_t)((j + 1) / ST) & 1, gave_up)) {
-                    if (lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
-                    break;
-                }
-                uint8_t *v0 = sm + F::OFF_V + st * F::KV_BYTES + (x >> 3) * 128 + (x & 7) * 16;
-                for (int i0 = 0; i0 < NC * 16; i0 += 8) {  // rows x / 8 + 8 i of an atom
-                    uint4 v[8];
+            uint32_t g = 0, vgo_ph = 0;
+            bool ok = true;
+            for (int k = 0; ok; k++) {
+                GaItem *it = items + k % GA_SLOTS;
+                ok = ga_wait(itemfull + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS) & 1, gave_up);
+                if (!ok || it->q0 < 0) break;
+                const int nmax = max(it->nt[0], it->nt[1]), edge = it->edge, nk = it->nk;
+                for (int j = edge; j < nmax; j++) {
+                    const uint32_t gj = g + 1 + j;
+                    const int st = (int)(gj % ST), left = nk - j * GA_KEYS;
+                    ok = ga_wait(vgo + st, (vgo_ph >> st) & 1, gave_up) && ga_wait(full + st, (gj / ST) & 1, gave_up);
+                    if (!ok) break;
+                    vgo_ph ^= 1u << st;
+                    uint8_t *v0 = sm + F::OFF_V + st * F::KV_BYTES + (x >> 3) * 128 + (x & 7) * 16;
+                    for (int i0 = 0; i0 < NC * 16; i0 += 8) {  // rows x / 8 + 8 i of an atom
+                        uint4 v[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = *reinterpret_cast<const uint4 *>(v0 + (i0 + i) * 1024);
+                        for (int i = 0; i < 8; i++) v[i] = *reinterpret_cast<const uint4 *>(v0 + (i0 + i) * 1024);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int row = (x >> 3) + 8 * ((i0 + i) & 15);
-                        const bool past = row >= left;
-                        if (past || (bad(v[i].x) | bad(v[i].y) | bad(v[i].z) | bad(v[i].w))) {
-                            *reinterpret_cast<uint4 *>(v0 + (i0 + i) * 1024) =
-                                past ? make_uint4(0, 0, 0, 0)
-                                     : make_uint4(clean(v[i].x), clean(v[i].y), clean(v[i].z), clean(v[i].w));
-                            if (!past) {
-                                atomicOr(&s_bad[j - edge][row >> 5], 1u << (row & 31));
-                                s_any_bad = 1;
+                        for (int i = 0; i < 8; i++) {
+                            const int row = (x >> 3) + 8 * ((i0 + i) & 15);
+                            const bool past = row >= left;
+                            if (past || (bad(v[i].x) | bad(v[i].y) | bad(v[i].z) | bad(v[i].w))) {
+                                *reinterpret_cast<uint4 *>(v0 + (i0 + i) * 1024) =
+                                    past ? make_uint4(0, 0, 0, 0)
+                                         : make_uint4(clean(v[i].x), clean(v[i].y), clean(v[i].z), clean(v[i].w));
+                                if (!past) {
+                                    atomicOr(&it->bad[j - edge][row >> 5], 1u << (row & 31));
+                                    it->any_bad = 1;
+                                }
                             }
                         }
                     }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(vok + st);
                 }
-                ptx::fence_proxy_async_smem();
+                if (nmax > 0) g += nmax + 1;
                 __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(vok + st);
+                if (lane == 0) {
+                    ptx::mbar_arrive(fixed + k % GA_SLOTS);
+                    ptx::mbar_arrive(itemfree + k % GA_SLOTS);
+                }
             }
+            if (!ok && lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::R_SOFTMAX));
@@ -425,118 +543,118 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(row & 96) << 16;
         const uint32_t S = tmem + t * 128 + lanes, O = tmem + F::O_COL + t * HDP + lanes;
-        const int tok = tok0 + t * TT + row / G, g = row % G;
-        const bool real = row < TT * G && tok < nq;
-        const int vis = real ? visible(tok) : 0;
-        const int mine = t ? nt[1] : nt[0];  // this tile's key tiles
-        float m = -INFINITY, off = 0.0f;  // reference of the exponents, and what is added to c s
-        uint64_t l2[2] = {0, 0};
+        const int row_tok = t * TT + row / G, row_g = row % G;
         const uint64_t c2 = ptx::f2_pack(ga.c, ga.c);
+        uint32_t n_s = 0, n_o = 0;
         bool ok = true;
-        for (int j = 0; j < mine; j++) {
-            if (!ga_wait(sfull + t, (uint32_t)j & 1, gave_up)) {
-                if (lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_SOFTMAX);
+        for (int k = 0; ok; k++) {
+            const GaItem *it = items + k % GA_SLOTS;
+            if (!ga_wait(itemfull + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS) & 1, gave_up)) {
                 ok = false;
                 break;
             }
-            ptx::tc_fence_after();
-            uint32_t s[4][32];
+            const int q0 = it->q0;
+            if (q0 < 0) break;
+            const int mine = it->nt[t], edge = it->edge, nq = it->nq, k0 = it->k0, hk = it->hk, tok = it->tok0 + row_tok;
+            const bool real = row < TT * G && tok < nq;
+            const int vis = real ? visible(nq, it->nk, tok) : 0;
+            float m = -INFINITY, off = 0.0f;  // reference of the exponents, and what is added to c s
+            uint64_t l2[2] = {0, 0};
+            for (int j = 0; j < mine; j++, n_s++) {
+                ok = ga_wait(sfull + t, n_s & 1, gave_up);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                uint32_t s[4][32];
 #pragma unroll
-            for (int x = 0; x < 4; x++) ptx::tmem_ld32(S + 32 * x, s[x]);
-            ptx::tmem_ld_wait();
-            const int lim = vis - j * GA_KEYS;
-            if (__any_sync(0xffffffffu, lim < GA_KEYS)) {
+                for (int x = 0; x < 4; x++) ptx::tmem_ld32(S + 32 * x, s[x]);
+                ptx::tmem_ld_wait();
+                const int lim = vis - j * GA_KEYS;
+                if (__any_sync(0xffffffffu, lim < GA_KEYS)) {
 #pragma unroll
-                for (int x = 0; x < 4; x++)
+                    for (int x = 0; x < 4; x++)
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (32 * x + i >= lim) s[x][i] = 0xff800000u;
-            }
-            float mx[4];
+                        for (int i = 0; i < 32; i++)
+                            if (32 * x + i >= lim) s[x][i] = 0xff800000u;
+                }
+                float mx[4];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2)
+                for (int i = 0; i < 32; i += 2)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const float u = __uint_as_float(s[x][i]), v = __uint_as_float(s[x][i + 1]);
+                        mx[x] = i == 0 ? ga_max(u, u, v) : ga_max(mx[x], u, v);
+                    }
+                // a row that sees a NaN or +infinity is NaN from here on
+                float top = ga_max(ga_max(mx[0], mx[1], mx[2]), mx[3], mx[3]) * ga.c;
+                const bool far = !(top <= m + 8.0f);
+                if (__any_sync(0xffffffffu, far)) {
+                    if (!(top < INFINITY)) top = NAN;
+                    const float mn = far ? top : m;
+                    const float f = far ? (m == -INFINITY ? 0.0f : ga_ex2(m - mn)) : 1.0f;
+                    m = mn;
+                    off = m == -INFINITY ? 0.0f : SHIFT - m;
+                    const uint64_t f2 = ptx::f2_pack(f, f);
+                    l2[0] = ptx::f2_fma(l2[0], f2, 0);
+                    l2[1] = ptx::f2_fma(l2[1], f2, 0);
+                    if (j > 0) {
+                        // S of this tile is complete, so the product before it is
+#pragma unroll 1
+                        for (int x = 0; x < HDP / 16; x++) {
+                            uint32_t o[16];
+                            ptx::tmem_ld16(O + 16 * x, o);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            ptx::tmem_st16(O + 16 * x, o);
+                        }
+                    }
+                }
+                const uint64_t off2 = ptx::f2_pack(off, off);
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
-                    const float u = __uint_as_float(s[x][i]), v = __uint_as_float(s[x][i + 1]);
-                    mx[x] = i == 0 ? ga_max(u, u, v) : ga_max(mx[x], u, v);
-                }
-            // a row that sees a NaN or +infinity is NaN from here on
-            float top = ga_max(ga_max(mx[0], mx[1], mx[2]), mx[3], mx[3]) * ga.c;
-            const bool far = !(top <= m + 8.0f);
-            if (__any_sync(0xffffffffu, far)) {
-                if (!(top < INFINITY)) top = NAN;
-                const float mn = far ? top : m;
-                const float f = far ? (m == -INFINITY ? 0.0f : ga_ex2(m - mn)) : 1.0f;
-                m = mn;
-                off = m == -INFINITY ? 0.0f : SHIFT - m;
-                const uint64_t f2 = ptx::f2_pack(f, f);
-                l2[0] = ptx::f2_fma(l2[0], f2, 0);
-                l2[1] = ptx::f2_fma(l2[1], f2, 0);
-                if (j > 0) {
-                    // S of this tile is complete, so the product before it is
-#pragma unroll 1
-                    for (int x = 0; x < HDP / 32; x++) {
-                        uint32_t o[32];
-                        ptx::tmem_ld32(O + 32 * x, o);
-                        ptx::tmem_ld_wait();
+                    uint32_t p[16];
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        ga_st32(O + 32 * x, o);
+                    for (int i = 0; i < 16; i++) {
+                        float e0, e1;
+                        ptx::f2_unpack(
+                            ptx::f2_fma(ptx::f2_pack(__uint_as_float(s[x][2 * i]), __uint_as_float(s[x][2 * i + 1])), c2, off2),
+                            e0, e1);
+                        e0 = ga_ex2(e0);
+                        e1 = ga_ex2(e1);
+                        l2[i & 1] = ptx::f2_add(l2[i & 1], ptx::f2_pack(e0, e1));
+                        p[i] = ga_pack<T>(e0, e1);
+                    }
+                    ptx::tmem_st16(S + 16 * x, p);
+                    if (x & 1) {  // half of the keys: their product may begin
+                        ptx::tmem_st_wait();
+                        ptx::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive(pready + 2 * t + (x >> 1));
                     }
                 }
             }
-            const uint64_t off2 = ptx::f2_pack(off, off);
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                uint32_t p[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float e0, e1;
-                    ptx::f2_unpack(ptx::f2_fma(ptx::f2_pack(__uint_as_float(s[x][2 * i]), __uint_as_float(s[x][2 * i + 1])),
-                                               c2, off2),
-                                   e0, e1);
-                    e0 = ga_ex2(e0);
-                    e1 = ga_ex2(e1);
-                    l2[i & 1] = ptx::f2_add(l2[i & 1], ptx::f2_pack(e0, e1));
-                    p[i] = ga_pack<T>(e0, e1);
-                }
-                ptx::tmem_st16(S + 16 * x, p);
-                if (x & 1) {  // half of the keys: their product may begin
-                    ptx::tmem_st_wait();
-                    ptx::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(pready + 2 * t + (x >> 1));
-                }
-            }
-        }
-        // ---- epilogue: O / l
-        if (mine > 0 && ok && !ga_wait(ofull + t, 0, gave_up)) {
-            if (lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_MMA);
-            ok = false;
-        }
-        ptx::tc_fence_after();
-        if (ok) {
-            float l, l0, l1;
+            if (!ok) break;
+            // ---- epilogue: O / l
+            float l0, l1;
             ptx::f2_unpack(ptx::f2_add(l2[0], l2[1]), l0, l1);
-            l = l0 + l1;
+            const float l = l0 + l1, inv = 1.0f / l;
             const bool none = vis == 0;
-            const float inv = 1.0f / l;
-            const int h = hk * G + g;
+            const int h = hk * G + row_g;
             const long long at = (long long)(q0 + tok) * a.o_ts + (long long)h * a.o_hs;  // the row's place in out
-            // keys noted at the edges that this row sees
-            const int edges = max(0, mine - edge);  // all of them multiplied by now
-            for (int e = max(0, edges - ST); e < edges; e++)
-                if (!ga_wait(vok + (edge + e + 1) % ST, (uint32_t)(e / ST) & 1, gave_up) && lane == 0)
-                    atomicOr(a.dev_err, WB_DERR_TIMEOUT_SOFTMAX);
-            const bool noted = s_any_bad;
-            // Through shared memory, so that a store instruction writes whole
-            // rows (a thread per row took 4.5 us): this tile's query rows
-            // are not read any more.  16-byte piece c of a row at place
-            // c ^ (row & 7) of its 128 bytes.
-            constexpr int RB = HDP * 2, PPR = HDP / 8;
-            uint8_t *stage = sm + t * F::Q_BYTES + (row & 96) * RB;
+            const uint32_t rows = __ballot_sync(0xffffffffu, real);
+            // keys noted at the edges that this row may see
+            ok = ga_wait(fixed + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS) & 1, gave_up);
+            if (ok && mine > 0) ok = ga_wait(ofull + t, n_o++ & 1, gave_up);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            const bool noted = it->any_bad;
+            const int edges = max(0, mine - edge);
+            // 32 columns at a time through shared memory, so that a store
+            // instruction writes 64 bytes of eight rows (a thread per row
+            // took 4 us): 16-byte piece c of a row at place c ^ (row / 2 & 3)
+            uint8_t *stage = sm + F::OFF_OUT + warp * F::OUT_WARP;
 #pragma unroll 1
-            for (int x = 0; x < HDP / 32; x++) {
+            for (int x = 0; x < HDP / 32 && 32 * x < a.hd; x++) {
                 uint32_t o[32];
                 __syncwarp();
                 if (mine > 0) {
@@ -547,7 +665,7 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                     for (int e = 0; e < edges; e++)
                         for (int i = 0; i < GA_KEYS; i++) {
                             const int key = (edge + e) * GA_KEYS + i;
-                            if (key >= vis || !(s_bad[e][i >> 5] >> (i & 31) & 1)) continue;
+                            if (key >= vis || !(it->bad[e][i >> 5] >> (i & 31) & 1)) continue;
                             const T *v = (const T *)a.v + (long long)(k0 + key) * a.v_ts + (long long)hk * a.v_hs;
 #pragma unroll
                             for (int d = 0; d < 32; d++)
@@ -566,32 +684,36 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                     w.y = ga_pack<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
                     w.z = ga_pack<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
                     w.w = ga_pack<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
-                    *reinterpret_cast<uint4 *>(stage + lane * RB + ((4 * x + i) ^ (lane & 7)) * 16) = w;
+                    *reinterpret_cast<uint4 *>(stage + lane * 64 + (i ^ (lane >> 1 & 3)) * 16) = w;
                 }
-            }
-            __syncwarp();
-            const uint32_t rows = __ballot_sync(0xffffffffu, real);
-            if (ga.vec) {
-                const int c = lane % PPR;
+                __syncwarp();
+                if (ga.vec) {
+                    const int c = lane & 3;
 #pragma unroll
-                for (int i = 0; i < PPR; i++) {
-                    const int r = i * (32 / PPR) + lane / PPR;
-                    const long long to = __shfl_sync(0xffffffffu, at, r);
-                    if ((rows >> r & 1) && 8 * c < a.hd)
-                        *reinterpret_cast<uint4 *>((T *)a.out + to + 8 * c) =
-                            *reinterpret_cast<const uint4 *>(stage + r * RB + (c ^ (r & 7)) * 16);
-                }
-            } else {
-                for (int r = 0; r < 32; r++) {
-                    const long long to = __shfl_sync(0xffffffffu, at, r);
-                    for (int d = lane; (rows >> r & 1) && d < a.hd; d += 32)
-                        ((T *)a.out)[to + d] = *reinterpret_cast<const T *>(stage + r * RB + ((d >> 3) ^ (r & 7)) * 16 + (d & 7) * 2);
+                    for (int i = 0; i < 4; i++) {
+                        const int r = 8 * i + (lane >> 2);
+                        const long long to = __shfl_sync(0xffffffffu, at, r);
+                        if ((rows >> r & 1) && 32 * x + 8 * c < a.hd)
+                            *reinterpret_cast<uint4 *>((T *)a.out + to + 32 * x + 8 * c) =
+                                *reinterpret_cast<const uint4 *>(stage + r * 64 + (c ^ (r >> 1 & 3)) * 16);
+                    }
+                } else {
+                    for (int r = 0; r < 32; r++) {
+                        const long long to = __shfl_sync(0xffffffffu, at, r);
+                        if ((rows >> r & 1) && 32 * x + lane < a.hd)
+                            ((T *)a.out)[to + 32 * x + lane] =
+                                *reinterpret_cast<const T *>(stage + r * 64 + ((lane >> 3) ^ (r >> 1 & 3)) * 16 + (lane & 7) * 2);
+                    }
                 }
             }
             if (real && a.lse)
                 a.lse[(long long)h * a.total_q + q0 + tok] = none ? -INFINITY : (log2f(l) - off) * 0.6931471805599453f;
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(itemfree + k % GA_SLOTS);
         }
+        if (!ok && lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_SOFTMAX);
     }
+    __syncwarp();
     ptx::tc_fence_before();
     __syncthreads();
     if (warp == F::W_MMA) ptx::tmem_dealloc(tmem, F::TMEM);
@@ -644,7 +766,7 @@ __global__ void __launch_bounds__(256) gqa_rows_kernel(const uint16_t *src, long
 }
 
 template <class T, int HDP>
-static int ga_launch(const GaArgs &ga, cudaStream_t st, std::string *msg) {
+static int ga_launch(const GaArgs &ga, int sm_count, cudaStream_t st, std::string *msg) {
     using F = GaConf<HDP>;
     const GqaAttnArgs &a = ga.a;
     const CUtensorMapDataType dt =
@@ -672,21 +794,19 @@ static int ga_launch(const GaArgs &ga, cudaStream_t st, std::string *msg) {
         *msg = std::string("attention kernel attributes: ") + cudaGetErrorString(set);
         return WB_ECUDA;
     }
-    // at most this many tile pairs, whatever the sequences' lengths are
-    const long long items = std::min(a.total_q, a.total_q / (F::NT * ga.TT) + a.n_seq);
-    if (items * a.Hkv > 0x7fffffffLL) {
-        *msg = "too many query tiles";
-        return WB_EINVAL;
-    }
     ProfScope ps("gqa_attn", st);
-    gqa_attn_kernel<T, HDP><<<(unsigned)(items * a.Hkv), F::THREADS, F::BYTES, st>>>(tq, tk, tv, ga);
+    const unsigned grid = (unsigned)std::min<long long>(ga.items * a.Hkv, sm_count);
+    gqa_attn_kernel<T, HDP><<<grid, F::THREADS, F::BYTES, st>>>(tq, tk, tv, ga);
     return WB_OK;
 }
 
-int launch_gqa_attention(const GqaAttnArgs &args, int dtype, void *scratch, int, cudaStream_t st, std::string *msg) {
-    GaArgs ga{args, 0.0f, args.H / args.Hkv, 0, 0};
+int launch_gqa_attention(const GqaAttnArgs &args, int dtype, void *scratch, int sm_count, cudaStream_t st,
+                         std::string *msg) {
+    GaArgs ga{args, 0.0f, args.H / args.Hkv, 0, 0, 0};
     GqaAttnArgs &a = ga.a;
     ga.TT = GA_ROWS / ga.G;
+    // at most this many, whatever the sequences' lengths are
+    ga.items = std::min(a.total_q, a.total_q / (2 * ga.TT) + a.n_seq);
     ga.c = std::max(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // 0 would turn a hidden key's -inf into NaN
     ga.vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.o_ts % 8 == 0 && a.o_hs % 8 == 0 && a.hd % 8 == 0;
     const GaCopies cp = ga_copies(args);
@@ -704,8 +824,8 @@ int launch_gqa_attention(const GqaAttnArgs &args, int dtype, void *scratch, int,
     if (cp.k) copy(a.k, a.k_ts, a.k_hs, a.total_k, a.Hkv, 0, cp.ok);
     if (cp.v) copy(a.v, a.v_ts, a.v_hs, a.total_k, a.Hkv, 0, cp.ov);
     if (dtype == WB_BF16)
-        return a.hd <= 64 ? ga_launch<__nv_bfloat16, 64>(ga, st, msg) : ga_launch<__nv_bfloat16, 128>(ga, st, msg);
-    return a.hd <= 64 ? ga_launch<__half, 64>(ga, st, msg) : ga_launch<__half, 128>(ga, st, msg);
+        return a.hd <= 64 ? ga_launch<__nv_bfloat16, 64>(ga, sm_count, st, msg) : ga_launch<__nv_bfloat16, 128>(ga, sm_count, st, msg);
+    return a.hd <= 64 ? ga_launch<__half, 64>(ga, sm_count, st, msg) : ga_launch<__half, 128>(ga, sm_count, st, msg);
 }
 
 }  // namespace wb
