@@ -99,6 +99,39 @@ def test_quantised_edges(store):
         assert gk[4:7].isnan().all() and gv[4:7].isnan().all()
 
 
+@pytest.mark.parametrize("store", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_quantised_ties(store, dtype):
+    """Bit for bit the division's rounding, on many rows of every size, quotients midway between two stored values among them."""
+    import torch
+    import wave_engine_b200 as wb
+    dtype = getattr(torch, dtype)
+    n, Hkv, hd = 4096, 4, 128
+    k, v = _rows(21, dtype, n, Hkv, hd)
+    size = torch.exp2(torch.randint(-20, 12, (n, Hkv, 1), device="cuda").float())
+    k, v = (k.float() * size).to(dtype), (v.float() / size).to(dtype)
+    if dtype == torch.bfloat16:
+        k[:64] *= 2.0 ** -110   # scales below the range of the remainder
+        v[:64] *= 2.0 ** 100
+    for kind, top in ((torch.int8, 127), (torch.float8_e4m3fn, 448)):
+        q, s = ref.quantise(k, kind)
+        if kind == _kinds()[store]:
+            y = (k.float() / s[..., None]).abs()
+            ties = (y - y.floor() == 0.5) if store == "int8" else ((y.view(torch.int32) & 0xFFFFF) == 0x80000)
+            assert ties.sum() > 100
+    cache = wb.GqaCache(1, Hkv, hd, 1, n, n // 128, dtype=dtype, store=store)
+    cache.reserve(0, n)
+    cache.write(0, k, v, [0], [0, n])
+    gk, gv = cache.read(0, [0], [0, n])
+    assert _same(gk, _stored(k, store)) and _same(gv, _stored(v, store))
+    table = cache.table[0, :n // 128].long()
+    held = cache.k_pages[0].view(torch.uint8)[table].view(_kinds()[store]).float().permute(0, 2, 1, 3).reshape(n, Hkv, hd)
+    q, s = ref.quantise(k, _kinds()[store])
+    finite = torch.isfinite(s)
+    assert torch.equal(held[finite], q.float()[finite]) and finite.float().mean() > 0.9
+    assert torch.equal(cache.k_scale[0][table].permute(0, 2, 1).reshape(n, Hkv), s)
+
+
 def test_outside_the_pages():
     import torch
     import wave_engine_b200 as wb

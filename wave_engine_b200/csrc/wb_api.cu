@@ -2008,7 +2008,7 @@ int check_slots(const int32_t *slots, int n_seq, int n_slots) {
 // What the write and the read share: their index arrays.
 int gqa_move_indexes(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq, const int32_t *cu,
                      int64_t total, const int32_t *start, wb::GqaCacheArgs *ca, const int32_t **cu_d,
-                     const int32_t **start_d) {
+                     const int32_t **start_d, unsigned int **ticket) {
     if (total < 0 || total > 0x7fffffff) return fail(WB_EINVAL, "total out of range");
     if (!cu && total != n_seq) return fail(WB_EINVAL, "without cu there is one row per sequence");
     IndexArgs ix;
@@ -2021,12 +2021,10 @@ int gqa_move_indexes(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t 
             if (start[i] < 0 || start[i] + n > (int64_t)c->max_pages * WB_PAGE)
                 return fail(WB_EINVAL, "positions outside the slot's table");
         }
-    if (ix.bytes()) {
-        DevBuf *w;
-        WB_TRY(gqa_workspace(ctx, wb::GQA_WS_HEAD + ix.bytes(), &w));
-        WB_TRY(ix.upload((char *)w->p + wb::GQA_WS_HEAD, ctx->stream));
-    }
-    return WB_OK;
+    DevBuf *w;
+    WB_TRY(gqa_workspace(ctx, wb::GQA_WS_HEAD + ix.bytes(), &w));
+    *ticket = (unsigned int *)w->p + wb::GQA_WS_TICKET;
+    return ix.upload((char *)w->p + wb::GQA_WS_HEAD, ctx->stream);
 }
 
 }  // namespace
@@ -2092,10 +2090,11 @@ int wb_gqa_cache_write(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_
         if (total != 0 && !all_device({k, v})) return fail(WB_EINVAL, "k and v must be device memory");
         ProfBind pb(ctx);
         const int32_t *cu_d, *start_d;
-        WB_TRY(gqa_move_indexes(ctx, c, slots, n_seq, cu, total, start, &ca, &cu_d, &start_d));
+        unsigned int *ticket;
+        WB_TRY(gqa_move_indexes(ctx, c, slots, n_seq, cu, total, start, &ca, &cu_d, &start_d, &ticket));
         std::string msg;
         int rc = wb::launch_gqa_cache_write(ca, c->dtype, cu_d, total, start_d, k, v, k_ts, k_hs, v_ts, v_hs,
-                                            ctx->stream, &msg);
+                                            ticket, ctx->stream, &msg);
         if (rc != WB_OK) return fail(rc, msg);
         WB_CUDA(cudaGetLastError());
         return WB_OK;
@@ -2115,7 +2114,8 @@ int wb_gqa_cache_read(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t
         if (!all_device({k, v})) return fail(WB_EINVAL, "k and v must be device memory");
         ProfBind pb(ctx);
         const int32_t *cu_d, *start_d;
-        WB_TRY(gqa_move_indexes(ctx, c, slots, n_seq, cu, total, start, &ca, &cu_d, &start_d));
+        unsigned int *ticket;
+        WB_TRY(gqa_move_indexes(ctx, c, slots, n_seq, cu, total, start, &ca, &cu_d, &start_d, &ticket));
         std::string msg;
         int rc = wb::launch_gqa_cache_read(ca, c->dtype, cu_d, total, start_d, k, v, ctx->stream, &msg);
         if (rc != WB_OK) return fail(rc, msg);

@@ -46,6 +46,7 @@ struct GqaCacheArgs {
 // A stream's scratch begins with counters that every call finds and leaves
 // zero.
 static constexpr size_t GQA_WS_HEAD = 16384;
+static constexpr int GQA_WS_TICKET = 4095;  // the cache write's counter (the decode's are the first, one per CTA)
 
 // scratch bytes (after the counters and index arrays) of the calls below
 size_t gqa_attention_scratch(const GqaAttnArgs &a, int dtype);
@@ -56,7 +57,7 @@ int launch_gqa_attention(const GqaAttnArgs &a, int dtype, void *scratch, int sm_
 // cu: nullptr = one token per sequence; start: nullptr = the slots' lengths
 int launch_gqa_cache_write(const GqaCacheArgs &c, int dtype, const int32_t *cu, long long total, const int32_t *start,
                            const void *k, const void *v, long long k_ts, long long k_hs, long long v_ts, long long v_hs,
-                           cudaStream_t st, std::string *msg);
+                           unsigned int *ticket, cudaStream_t st, std::string *msg);
 int launch_gqa_cache_read(const GqaCacheArgs &c, int dtype, const int32_t *cu, long long total, const int32_t *start,
                           void *k, void *v, cudaStream_t st, std::string *msg);
 int launch_gqa_decode(const GqaCacheArgs &c, int dtype, int H, const void *q, long long q_ss, long long q_hs,
@@ -74,6 +75,11 @@ __device__ __forceinline__ int gqa_find_seq(const int32_t *cu, int n, long long 
         else hi = mid - 1;
     }
     return lo;
+}
+
+// a / b, by a 32-bit division where that does
+__device__ __forceinline__ long long gqa_quotient(long long a, long long b) {
+    return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
 }
 
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }

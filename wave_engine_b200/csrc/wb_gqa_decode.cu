@@ -144,10 +144,6 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// a / b, by a 32-bit division where that does
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-    return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
-}
 // over the 8 lanes of one cc
 __device__ __forceinline__ float oct_max(float v) {
 #pragma unroll
@@ -275,7 +271,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
     } else total = units + W * items;
     const long long grid = min((long long)gridDim.x, total);
     if ((long long)blockIdx.x >= grid) return;
-    const long long s0 = quotient(blockIdx.x * total, grid), s1 = quotient((blockIdx.x + 1) * total, grid);
+    const long long s0 = gqa_quotient(blockIdx.x * total, grid), s1 = gqa_quotient((blockIdx.x + 1) * total, grid);
 
     // The share's parts with keys, one after another, U = 0 past its end.  One
     // thread finds part x + 2 while part x is joined.
@@ -293,7 +289,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                 continue;
             }
             const long long rel = u - pref;
-            const int item = (int)quotient(rel, il), o0 = (int)(rel - (long long)item * il);
+            const int item = (int)gqa_quotient(rel, il), o0 = (int)(rel - (long long)item * il);
             const int o1 = (int)min((long long)il, o0 + (s1 - u));
             u += o1 - o0;
             if (o1 * P <= W) continue;
@@ -760,7 +756,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
         }
         if (!whole) {
             // ---- the item's last CTA joins the pieces
-            const int c0 = (int)quotient((g.first + 1) * grid - 1, total), c1 = (int)quotient((g.last + 1) * grid - 1, total);
+            const int c0 = (int)gqa_quotient((g.first + 1) * grid - 1, total), c1 = (int)gqa_quotient((g.last + 1) * grid - 1, total);
             __threadfence();
             __syncthreads();
             if (tid == 0) s_last = atomicAdd(a.counters + c0, 1) == (unsigned)(c1 - c0);
