@@ -35,3 +35,13 @@ def test_descriptors_match_the_header():
                     want.append((f.lstrip("*"), "p" if f.startswith("*") else m.group(1)))
         kind = {C.c_int32: "int32_t", C.c_int64: "int64_t", C.c_float: "float", C.c_void_p: "p"}
         assert [(n, kind[t]) for n, t in cls._fields_] == want
+
+
+def test_packed_descriptors_are_the_ctypes_ones():
+    """The struct formats that the entry points pack with lay every field where the descriptors have it."""
+    from wave_engine_b200 import _lib, gqa
+    for fmt, cls in ((gqa._ATTN, _lib.GqaAttnDesc), (gqa._CACHE, _lib.GqaCacheDesc)):
+        assert fmt.size == C.sizeof(cls)
+        values = [i + 1 for i in range(len(cls._fields_))]
+        d = cls.from_buffer_copy(fmt.pack(*values))
+        assert [getattr(d, n) for n, _ in cls._fields_] == values

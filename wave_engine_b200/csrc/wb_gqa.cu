@@ -747,22 +747,36 @@ static GaCopies ga_copies(const GqaAttnArgs &a) {
 
 size_t gqa_attention_scratch(const GqaAttnArgs &a, int) { return ga_copies(a).bytes; }
 
-// One thread per 8 output elements; flip: 0x8000 changes the sign.
-__global__ void __launch_bounds__(256) gqa_rows_kernel(const uint16_t *src, long long ts, long long hs, long long rows,
-                                                       int heads, int hd, uint32_t flip, uint4 *dst) {
-    const int per = (hd + 7) / 8;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * heads * per) return;
-    const int d0 = (int)(i % per) * 8;
-    const long long rh = i / per, row = rh / heads;
-    const uint16_t *p = src + row * ts + (rh - row * heads) * hs;
+struct GaCopyJob {
+    const uint16_t *src;
+    uint4 *dst;
+    long long ts, hs, n;  // n: pieces of 8 elements
+    int heads;
+    uint32_t flip;        // 0x8000 changes the sign
+};
+struct GaCopyJobs {
+    GaCopyJob job[3];
+    int hd;
+};
+// One thread per 8 output elements, all the rows to copy in one launch.
+__global__ void __launch_bounds__(256) gqa_rows_kernel(GaCopyJobs js) {
+    const int per = (js.hd + 7) / 8;
+    long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    int which = 0;
+    while (which < 3 && i >= js.job[which].n) i -= js.job[which++].n;
+    if (which == 3) return;
+    const GaCopyJob &j = js.job[which];
+    const long long rh = gqa_quotient(i, per), row = gqa_quotient(rh, j.heads);
+    const int d0 = (int)(i - rh * per) * 8;
+    const uint16_t *p = j.src + row * j.ts + (rh - row * j.heads) * j.hs;
     uint32_t w[4];
 #pragma unroll
     for (int x = 0; x < 4; x++) {
-        const uint32_t lo = d0 + 2 * x < hd ? p[d0 + 2 * x] ^ flip : 0, hi = d0 + 2 * x + 1 < hd ? p[d0 + 2 * x + 1] ^ flip : 0;
+        const uint32_t lo = d0 + 2 * x < js.hd ? p[d0 + 2 * x] ^ j.flip : 0;
+        const uint32_t hi = d0 + 2 * x + 1 < js.hd ? p[d0 + 2 * x + 1] ^ j.flip : 0;
         w[x] = lo | hi << 16;
     }
-    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    j.dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <class T, int HDP>
@@ -810,19 +824,29 @@ int launch_gqa_attention(const GqaAttnArgs &args, int dtype, void *scratch, int 
     ga.c = std::max(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // 0 would turn a hidden key's -inf into NaN
     ga.vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.o_ts % 8 == 0 && a.o_hs % 8 == 0 && a.hd % 8 == 0;
     const GaCopies cp = ga_copies(args);
-    auto copy = [&](const void *&p, long long &ts, long long &hs, long long rows, int heads, uint32_t flip, size_t off) {
-        const long long n = ga_copy_elems(rows, heads, a.hd) / 8;
-        void *d = (char *)scratch + off;
+    if (cp.q || cp.k || cp.v) {
+        GaCopyJobs js{};
+        js.hd = a.hd;
+        long long n = 0;
+        auto job = [&](GaCopyJob &j, const void *&p, long long &ts, long long &hs, long long rows, int heads, uint32_t flip,
+                       size_t off) {
+            j = GaCopyJob{(const uint16_t *)p, (uint4 *)((char *)scratch + off), ts, hs, ga_copy_elems(rows, heads, a.hd) / 8,
+                          heads, flip};
+            n += j.n;
+            p = j.dst;
+            hs = (a.hd + 7) & ~7;
+            ts = hs * heads;
+        };
+        if (cp.q) job(js.job[0], a.q, a.q_ts, a.q_hs, a.total_q, a.H, a.scale < 0.0f ? 0x8000 : 0, cp.oq);
+        if (cp.k) job(js.job[1], a.k, a.k_ts, a.k_hs, a.total_k, a.Hkv, 0, cp.ok);
+        if (cp.v) job(js.job[2], a.v, a.v_ts, a.v_hs, a.total_k, a.Hkv, 0, cp.ov);
+        if ((n + 255) / 256 > 0x7fffffffLL) {
+            *msg = "too many rows to copy";
+            return WB_EINVAL;
+        }
         ProfScope ps("gqa_rows", st);
-        gqa_rows_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>((const uint16_t *)p, ts, hs, rows, heads, a.hd, flip,
-                                                                     (uint4 *)d);
-        p = d;
-        hs = (a.hd + 7) & ~7;
-        ts = hs * heads;
-    };
-    if (cp.q) copy(a.q, a.q_ts, a.q_hs, a.total_q, a.H, a.scale < 0.0f ? 0x8000 : 0, cp.oq);
-    if (cp.k) copy(a.k, a.k_ts, a.k_hs, a.total_k, a.Hkv, 0, cp.ok);
-    if (cp.v) copy(a.v, a.v_ts, a.v_hs, a.total_k, a.Hkv, 0, cp.ov);
+        gqa_rows_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(js);
+    }
     if (dtype == WB_BF16)
         return a.hd <= 64 ? ga_launch<__nv_bfloat16, 64>(ga, sm_count, st, msg) : ga_launch<__nv_bfloat16, 128>(ga, sm_count, st, msg);
     return a.hd <= 64 ? ga_launch<__half, 64>(ga, sm_count, st, msg) : ga_launch<__half, 128>(ga, sm_count, st, msg);

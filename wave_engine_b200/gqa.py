@@ -16,7 +16,7 @@ sequences, which are checked.  The work runs in the CUDA library
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 
 import numpy as np
 
@@ -27,10 +27,16 @@ try:  # the package imports without torch; these entry points take torch tensors
     import torch
     _DTYPES = {torch.bfloat16: _lib.WB_BF16, torch.float16: _lib.WB_F16}
     _STORES = {**_DTYPES, torch.int8: _lib.WB_INT8, torch.float8_e4m3fn: _lib.WB_E4M3}
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 except Exception:  # pragma: no cover
-    torch, _DTYPES, _STORES = None, {}, {}
+    torch, _DTYPES, _STORES, _raw_stream = None, {}, {}, None
 
 PAGE = 128  # positions per page (WB_KV_PAGE)
+
+
+# wb_gqa_attn_desc and wb_gqa_cache_desc (include/wave_b200.h) in C's layout
+_ATTN = struct.Struct("@6if2q3P6q2PP2qP")
+_CACHE = struct.Struct("@7i6P")
 
 
 def _row(head_dim: int) -> int:
@@ -39,9 +45,9 @@ def _row(head_dim: int) -> int:
 
 
 def _index(a, n: int, name: str):
-    """(pointer, object to keep) of an int32 index array of n entries; None stays None."""
+    """(address, object to keep) of an int32 index array of n entries; None is (0, None)."""
     if a is None:
-        return None, None
+        return 0, None
     if isinstance(a, torch.Tensor) and a.is_cuda:
         if a.dtype != torch.int32 or a.dim() != 1 or not a.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 vector")
@@ -55,38 +61,42 @@ def _index(a, n: int, name: str):
 
 
 def _rows(x, name: str, dtype=None):
-    """Shape and strides check of [tokens][heads][head_dim] rows."""
+    """Strides of [tokens][heads][head_dim] rows, checked."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 3:
         raise ValueError(f"{name} must be a CUDA tensor [tokens][heads][head_dim]")
     if x.dtype not in _DTYPES or (dtype is not None and x.dtype != dtype):
         raise ValueError(f"{name} must be bfloat16 or float16, as the others")
-    if x.stride(2) != 1 and x.shape[2] > 1:
+    ts, hs, ds = x.stride()
+    if ds != 1 and x.shape[2] > 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")
-    return x.stride(0), x.stride(1)
+    return ts, hs
 
 
-def _context(ctx, x) -> Context:
-    """The context for x's device, on torch's current stream there."""
+def _context(ctx, device) -> Context:
+    """The context for a device, on torch's current stream there."""
+    index = device.index
     if ctx is None:
-        ctx = default_context(x.device.index)
-    elif ctx.device != x.device.index:
+        ctx = default_context(index)
+    elif ctx.device != index:
         raise ValueError("the context is on another device")
-    ctx.set_stream(torch.cuda.current_stream(x.device).cuda_stream)
+    stream = torch.cuda.current_stream(index).cuda_stream if _raw_stream is None else _raw_stream(index)
+    if ctx.stream != stream:
+        ctx.set_stream(stream)
     return ctx
 
 
-def _out(out, shape, dtype, like, name):
+def _out(out, shape, dtype, device, name):
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != like.device:
-        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on {like.device}")
+        return torch.empty(shape, dtype=dtype, device=device)  # contiguous, whatever the rows' strides are
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
+        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on {device}")
     return out
 
 
-def _same_device(x, **others) -> None:
-    for name, t in others.items():
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.device != x.device:
-            raise ValueError(f"{name} is on another device")
+def _same_device(device, *others) -> None:
+    for t in others:
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.device != device:
+            raise ValueError(f"tensors on {device} and on {t.device}")
 
 
 def gqa_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float | None = None,
@@ -104,45 +114,52 @@ def gqa_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float
     Tk, Hkv, _ = k.shape
     if k.shape != v.shape or k.shape[2] != hd:
         raise ValueError("k and v must be [tokens][n_kv_head][head_dim], head_dim as q's")
-    _same_device(q, k=k, v=v, cu_q=cu_q, cu_k=cu_k)
+    device = q.device
+    _same_device(device, k, v, cu_q, cu_k)
     n_seq = len(cu_q) - 1
     if n_seq < 0:
         raise ValueError("cu_q must have one entry more than there are sequences")
     pq, keep_q = _index(cu_q, n_seq + 1, "cu_q")
     pk, keep_k = _index(cu_k, n_seq + 1, "cu_k")
-    out = _out(out, (Tq, H, hd), q.dtype, q, "out")
+    out = _out(out, (Tq, H, hd), q.dtype, device, "out")
     o_ts, o_hs = _rows(out, "out", q.dtype)
-    lse = torch.empty((H, Tq), dtype=torch.float32, device=q.device) if return_lse else None
-    ctx = _context(ctx, q)
-    d = _lib.GqaAttnDesc(_DTYPES[q.dtype], H, Hkv, hd, n_seq, int(causal), hd ** -0.5 if scale is None else scale, Tq,
-                         Tk, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, pq, pk,
-                         out.data_ptr(), o_ts, o_hs, None if lse is None else lse.data_ptr())
-    _lib.call("wb_gqa_attention", ctx.handle, C.byref(d))
+    lse = torch.empty((H, Tq), dtype=torch.float32, device=device) if return_lse else None
+    ctx = _context(ctx, device)
+    d = _ATTN.pack(_DTYPES[q.dtype], H, Hkv, hd, n_seq, bool(causal), hd ** -0.5 if scale is None else scale, Tq, Tk,
+                   q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, pq, pk,
+                   out.data_ptr(), o_ts, o_hs, 0 if lse is None else lse.data_ptr())
+    _lib.call("wb_gqa_attention", ctx.handle, d)
     return (out, lse) if return_lse else out
 
 
 def _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, dtype, head_dim):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+    shape, device = k_pages.shape, k_pages.device
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != k_pages.dtype:
         raise ValueError("k_pages and v_pages must be [n_pages][n_kv_head][128][row]")
-    n_pages, Hkv, page, row = k_pages.shape
+    n_pages, Hkv, page, row = shape
     store = _STORES.get(k_pages.dtype)
     if store is None or page != PAGE or row != _row(head_dim):
         raise ValueError(f"pages must hold {PAGE} rows of {_row(head_dim)} bf16, fp16, int8 or float8_e4m3fn values")
-    if store in (_lib.WB_INT8, _lib.WB_E4M3):
+    arrays = [k_pages, v_pages, table]
+    ks = vs = 0
+    if store == _lib.WB_INT8 or store == _lib.WB_E4M3:
         for x in (k_scale, v_scale):
-            if x is None or tuple(x.shape) != (n_pages, Hkv, PAGE) or x.dtype != torch.float32:
+            if x is None or x.shape != shape[:3] or x.dtype != torch.float32:
                 raise ValueError("an 8-bit cache needs fp32 k_scale and v_scale [n_pages][n_kv_head][128]")
-    else:
-        k_scale = v_scale = None
-    if table.dim() != 2 or table.dtype != torch.int32 or (lens is not None and (lens.dtype != torch.int32 or
-                                                          tuple(lens.shape) != (table.shape[0],))):
-        raise ValueError("table must be int32 [n_slots][max_pages] and lens int32 [n_slots]")
-    for x in (k_pages, v_pages, k_scale, v_scale, table, lens):
-        if x is not None and (not x.is_contiguous() or x.device != k_pages.device or not x.is_cuda):
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+        arrays += (k_scale, v_scale)
+    if table.dim() != 2 or table.dtype != torch.int32:
+        raise ValueError("table must be int32 [n_slots][max_pages]")
+    if lens is not None:
+        if lens.dtype != torch.int32 or lens.dim() != 1 or lens.shape[0] != table.shape[0]:
+            raise ValueError("lens must be int32 [n_slots]")
+        arrays.append(lens)
+    for x in arrays:
+        if not x.is_contiguous() or not x.is_cuda or x.device != device:
             raise ValueError("cache arrays must be contiguous CUDA tensors of one device")
-    p = lambda x: None if x is None else x.data_ptr()  # noqa: E731
-    return _lib.GqaCacheDesc(_DTYPES[dtype], store, Hkv, head_dim, n_pages, table.shape[0], table.shape[1],
-                             k_pages.data_ptr(), v_pages.data_ptr(), p(k_scale), p(v_scale), table.data_ptr(), p(lens))
+    return _CACHE.pack(_DTYPES[dtype], store, Hkv, head_dim, n_pages, table.shape[0], table.shape[1],
+                       k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(),
+                       0 if lens is None else lens.data_ptr())
 
 
 def _n_seq(table, cu, slots, rows=None):
@@ -167,13 +184,13 @@ def gqa_cache_write(k, v, k_pages, v_pages, table, lens, *, cu=None, start=None,
         raise ValueError("k and v must be [tokens][n_kv_head][head_dim]")
     total, _, hd = k.shape
     d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, k.dtype, hd)
-    _same_device(k, v=v, k_pages=k_pages, cu=cu, start=start, slots=slots)
+    _same_device(k.device, v, k_pages, cu, start, slots)
     n_seq = _n_seq(table, cu, slots, total)
     pc, keep_c = _index(cu, n_seq + 1, "cu")
     ps, keep_s = _index(start, n_seq, "start")
     pl, keep_l = _index(slots, n_seq, "slots")
-    ctx = _context(ctx, k)
-    _lib.call("wb_gqa_cache_write", ctx.handle, C.byref(d), pl, n_seq, pc, total, ps, k.data_ptr(), k_ts, k_hs,
+    ctx = _context(ctx, k.device)
+    _lib.call("wb_gqa_cache_write", ctx.handle, d, pl, n_seq, pc, total, ps, k.data_ptr(), k_ts, k_hs,
               v.data_ptr(), v_ts, v_hs)
 
 
@@ -186,7 +203,7 @@ def gqa_cache_read(k_pages, v_pages, table, *, head_dim: int, dtype, cu=None, to
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16 or float16")
     d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, None, dtype, head_dim)
-    _same_device(k_pages, cu=cu, start=start, slots=slots)
+    _same_device(k_pages.device, cu, start, slots)
     n_seq = _n_seq(table, cu, slots)
     if total is None:
         if cu is not None and isinstance(cu, torch.Tensor) and cu.is_cuda:
@@ -198,8 +215,8 @@ def gqa_cache_read(k_pages, v_pages, table, *, head_dim: int, dtype, cu=None, to
     shape = (total, k_pages.shape[1], head_dim)
     k = torch.empty(shape, dtype=dtype, device=k_pages.device)
     v = torch.empty(shape, dtype=dtype, device=k_pages.device)
-    ctx = _context(ctx, k_pages)
-    _lib.call("wb_gqa_cache_read", ctx.handle, C.byref(d), pl, n_seq, pc, total, ps, k.data_ptr(), v.data_ptr())
+    ctx = _context(ctx, k_pages.device)
+    _lib.call("wb_gqa_cache_read", ctx.handle, d, pl, n_seq, pc, total, ps, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -211,15 +228,16 @@ def gqa_decode(q, k_pages, v_pages, table, lens, *, slots=None, k_scale=None, v_
     q_ss, q_hs = _rows(q, "q")
     n_seq, H, hd = q.shape
     d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, q.dtype, hd)
-    _same_device(q, k_pages=k_pages, slots=slots)
+    device = q.device
+    _same_device(device, k_pages, slots)
     pl, keep_l = _index(slots, n_seq, "slots")
-    out = _out(out, (n_seq, H, hd), q.dtype, q, "out")
+    out = _out(out, (n_seq, H, hd), q.dtype, device, "out")
     if not out.is_contiguous():
         raise ValueError("out must be contiguous")
-    lse = torch.empty((n_seq, H), dtype=torch.float32, device=q.device) if return_lse else None
-    ctx = _context(ctx, q)
-    _lib.call("wb_gqa_decode", ctx.handle, C.byref(d), pl, n_seq, H, q.data_ptr(), q_ss, q_hs,
-              hd ** -0.5 if scale is None else scale, out.data_ptr(), None if lse is None else lse.data_ptr())
+    lse = torch.empty((n_seq, H), dtype=torch.float32, device=device) if return_lse else None
+    ctx = _context(ctx, device)
+    _lib.call("wb_gqa_decode", ctx.handle, d, pl, n_seq, H, q.data_ptr(), q_ss, q_hs,
+              hd ** -0.5 if scale is None else scale, out.data_ptr(), 0 if lse is None else lse.data_ptr())
     return (out, lse) if return_lse else out
 
 

@@ -48,6 +48,7 @@ class Context:
         h = C.c_void_p()
         _lib.call("wb_context_create", device, C.byref(h))
         self.handle = h
+        self.stream = _lib.lib().wb_context_own_stream(h) or 0  # cudaStream_t that calls run on
         self._children = weakref.WeakSet()  # layers / caches to release first
 
     def adopt(self, obj) -> None:
@@ -71,10 +72,11 @@ class Context:
         """Run later calls on this cudaStream_t handle; 0/None is CUDA's legacy
         default stream (torch's default stream)."""
         _lib.call("wb_context_set_stream", self.handle, cuda_stream or None)
+        self.stream = cuda_stream or 0
 
     def use_own_stream(self) -> None:
         """Back to the context's private stream."""
-        _lib.call("wb_context_set_stream", self.handle, _lib.lib().wb_context_own_stream(self.handle))
+        self.set_stream(_lib.lib().wb_context_own_stream(self.handle))
 
     def synchronize(self) -> None:
         _lib.call("wb_context_synchronize", self.handle)
