@@ -571,10 +571,13 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                 const int lim = vis - j * GA_KEYS;
                 if (__any_sync(0xffffffffu, lim < GA_KEYS)) {
 #pragma unroll
-                    for (int x = 0; x < 4; x++)
+                    for (int x = 0; x < 4; x++) {
+                        const int n = min(32, max(0, lim - 32 * x));  // columns of this piece that the row sees
+                        const uint32_t seen = n == 32 ? 0xffffffffu : (1u << n) - 1;
 #pragma unroll
                         for (int i = 0; i < 32; i++)
-                            if (32 * x + i >= lim) s[x][i] = 0xff800000u;
+                            if (!(seen & 1u << i)) s[x][i] = 0xff800000u;
+                    }
                 }
                 float mx[4];
 #pragma unroll
