@@ -56,7 +56,7 @@ struct GaConf {
     static constexpr int W_TMA = 4 * NT, W_MMA = W_TMA + 1, W_FIX = W_MMA + 1;  // warps before: softmax
     static constexpr int THREADS = (W_FIX + 2) * 32;
     // registers: the softmax warps take what the other four give up
-    static constexpr int R_SOFTMAX = 200, R_OTHER = 104;
+    static constexpr int R_SOFTMAX = 208, R_OTHER = 88;
     static constexpr int TMEM = NT * 256, O_COL = NT * 128;  // columns: S of each tile, then O of each
     static constexpr int NC = HDP / 64;              // 64-column swizzle atoms of a row
     static constexpr int Q_BYTES = GA_ROWS * HDP * 2;
