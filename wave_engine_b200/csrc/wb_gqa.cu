@@ -23,7 +23,6 @@
 // polynomial on the FMA pipe were measured and not kept: a quarter of them
 // cost 4% at 8192 tokens, three eighths 7%.)
 #include "wb_gqa.h"
-#include "wb_ptx.cuh"
 #include "wb_tc.h"
 
 #include <algorithm>

@@ -15,7 +15,6 @@
 // block are loaded before their places in the cache are looked up (sequence,
 // slot, start, page: dependent loads that take as long as the data).
 #include "wb_gqa.h"
-#include "wb_ptx.cuh"
 
 #include <algorithm>
 
@@ -215,6 +214,7 @@ __global__ void __launch_bounds__(GM_THREADS, GM_CTAS) gqa_write_kernel(GqaMove 
     const uint32_t l0 = (uint32_t)(r0 - t0 * c.Hkv) + tid / LPR, left = (uint32_t)min(rest, 1LL << 30);
     const long long ts = v ? m.v_ts : m.k_ts, hs = v ? m.v_hs : m.k_hs;
     const uint16_t *in = (const uint16_t *)(v ? m.v : m.k) + t0 * ts + d0;
+    gqa_wait();
     // ---- loads
     uint4 x[GM_ROWS][2];
 #pragma unroll
@@ -309,6 +309,7 @@ __global__ void __launch_bounds__(GM_THREADS) gqa_read_kernel(GqaMove m) {
     const long long r0 = (long long)blockIdx.x * ROWS, t0 = gqa_quotient(r0, c.Hkv), rest = m.total * c.Hkv - t0 * c.Hkv;
     const uint32_t l0 = (uint32_t)(r0 - t0 * c.Hkv) + tid / LPR, left = (uint32_t)min(rest, 1LL << 30);
     const int nt = (int)min(m.total - t0, (long long)(((uint32_t)(r0 - t0 * c.Hkv) + ROWS + c.Hkv - 1) / (uint32_t)c.Hkv));
+    gqa_wait();
     for (int i = tid; i < nt; i += GM_THREADS) {
         const long long p = gqa_place(m, t0 + i);
         s_place[i] = p;
@@ -400,9 +401,9 @@ int launch_gqa_cache_write(const GqaCacheArgs &c, int dtype, const int32_t *cu, 
     by_types(dtype, c.store, [&](auto t, auto s) {
         using T = decltype(t);
         using S = decltype(s);
-        if (l == 2) gqa_write_kernel<T, S, 2><<<dim3((unsigned)blocks, 2), GM_THREADS, 0, st>>>(m);
-        else if (l == 4) gqa_write_kernel<T, S, 4><<<dim3((unsigned)blocks, 2), GM_THREADS, 0, st>>>(m);
-        else gqa_write_kernel<T, S, 8><<<dim3((unsigned)blocks, 2), GM_THREADS, 0, st>>>(m);
+        if (l == 2) gqa_launch(gqa_write_kernel<T, S, 2>, dim3((unsigned)blocks, 2), GM_THREADS, 0, st, m);
+        else if (l == 4) gqa_launch(gqa_write_kernel<T, S, 4>, dim3((unsigned)blocks, 2), GM_THREADS, 0, st, m);
+        else gqa_launch(gqa_write_kernel<T, S, 8>, dim3((unsigned)blocks, 2), GM_THREADS, 0, st, m);
     });
     return WB_OK;
 }
@@ -421,9 +422,9 @@ int launch_gqa_cache_read(const GqaCacheArgs &c, int dtype, const int32_t *cu, l
     by_types(dtype, c.store, [&](auto t, auto s) {
         using T = decltype(t);
         using S = decltype(s);
-        if (l == 4) gqa_read_kernel<T, S, 4><<<dim3((unsigned)blocks, 2), GM_THREADS, 0, st>>>(m);
-        else if (l == 8) gqa_read_kernel<T, S, 8><<<dim3((unsigned)blocks, 2), GM_THREADS, 0, st>>>(m);
-        else gqa_read_kernel<T, S, 16><<<dim3((unsigned)blocks, 2), GM_THREADS, 0, st>>>(m);
+        if (l == 4) gqa_launch(gqa_read_kernel<T, S, 4>, dim3((unsigned)blocks, 2), GM_THREADS, 0, st, m);
+        else if (l == 8) gqa_launch(gqa_read_kernel<T, S, 8>, dim3((unsigned)blocks, 2), GM_THREADS, 0, st, m);
+        else gqa_launch(gqa_read_kernel<T, S, 16>, dim3((unsigned)blocks, 2), GM_THREADS, 0, st, m);
     });
     return WB_OK;
 }

@@ -38,7 +38,6 @@
 // with its own product: the tensor pipe has the room, and 8 bits of p would
 // cost as much precision as the output's own rounding.
 #include "wb_gqa.h"
-#include "wb_ptx.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -62,6 +61,7 @@ static constexpr int GD_UNIT = 64;      // keys per unit: one 16-key block for e
 static constexpr int GD_ITEM = 2;       // what an item's start and end cost, in units of the line
 static constexpr int GD_FEW = 8;        // units per CTA below which items are cut into equal pieces ..
 static constexpr int GD_PIECE = 6;      // .. of this many units at least
+static constexpr int GD_JOIN = 12;      // pieces that a join loads at a time
 static constexpr int GD_SEQS = 256;     // sequences whose lengths a CTA holds in shared memory
 static constexpr float GD_SHIFT = 8.0f; // weights are kept as 2^8 exp2(s - m): see above
 
@@ -166,8 +166,8 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 // The sequence's slot and length; a slot or length that does not fit counts
 // as empty and is flagged.
 __device__ __forceinline__ int gd_len(const GqaCacheArgs &c, int b, int *slot) {
-    const int s = c.slots ? __ldg(c.slots + b) : b;
-    const int n = s >= 0 && s < c.n_slots ? __ldg(c.lens + s) : -1;
+    const int s = c.slots ? c.slots[b] : b;
+    const int n = s >= 0 && s < c.n_slots ? c.lens[s] : -1;
     *slot = s;
     if (n < 0 || n > c.max_pages * WB_PAGE) {
         atomicOr(c.dev_err, WB_DERR_BOUNDS);
@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, cc = lane & 3;
     const int G = a.H / c.Hkv, nch = (G + ROWS - 1) / ROWS, ips = c.Hkv * nch;  // items of a sequence
 
+    gqa_wait();
     // ---- the line of units and this CTA's share s0 .. s1-1
     const int per = (c.n_seq + GD_THREADS - 1) / GD_THREADS;
     long long sum = 0;  // units of a head in this thread's sequences, and how many have any (low 24 bits)
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
     // ---- loads of a part's blocks: this warp's are keys k0 + 16 (warp + 4 i)
     int pbase = 0, pid = -1;  // page ids of pages pbase + lane of the part
     auto pages_of = [&](const GdSeg &g, int p) {
-        return p + lane <= (g.k1 - 1) >> WB_PAGE_SHIFT ? __ldg(c.table + (long long)g.slot * c.max_pages + p + lane) : -1;
+        return p + lane <= (g.k1 - 1) >> WB_PAGE_SHIFT ? c.table[(long long)g.slot * c.max_pages + p + lane] : -1;
     };
     auto key_of = [&](int k0, int i) { return k0 + 16 * (warp + GD_WARPS * i); };
     auto blocks_of = [&](const GdSeg &g) { return (((g.k1 - g.k0 + 15) >> 4) - warp + GD_WARPS - 1) / GD_WARPS; };
@@ -404,11 +405,11 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                 uint2 w = make_uint2(0, 0);
                 if (row < g.nrow) {
                     if (q8) {
-                        if (d0 < c.hd) w = __ldg(reinterpret_cast<const uint2 *>(qp + d0));
+                        if (d0 < c.hd) w = *reinterpret_cast<const uint2 *>(qp + d0);
                     } else {
                         uint32_t e[4];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) e[i] = d0 + i < c.hd ? __ldg(qp + d0 + i) : 0;
+                        for (int i = 0; i < 4; i++) e[i] = d0 + i < c.hd ? qp[d0 + i] : 0;
                         w = make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
                     }
                 }
@@ -741,14 +742,26 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
         const bool whole = g.ua == 0 && g.ub == g.U;
         float *piece = a.part + ((long long)blockIdx.x * 2 + (g.ua == 0 ? 1 : 0)) * gqa_piece(HDP);
         const long long row_out = (long long)g.b * a.H + g.h0;
-        for (int i = tid; i < g.nrow * HDP; i += GD_THREADS) {
-            const int row = i / HDP, d = i % HDP;
-            float o = 0.0f;
+        auto put = [&](int row, int d, const float (&o)[4]) {
+            T *to = (T *)a.out + (row_out + row) * c.hd + d;
 #pragma unroll
-            for (int w = 0; w < GD_WARPS; w++) o += row_at(w, s_stage[w], row)[d] * s_f[w][row];
-            if (whole) {
-                if (d < c.hd) ((T *)a.out)[(row_out + row) * c.hd + d] = from_f<T>(o);
-            } else __stcg(piece + 16 + i, o);
+            for (int y = 0; y < 4; y++)
+                if (d + y < c.hd) to[y] = from_f<T>(o[y]);
+        };
+        for (int i = tid; i < g.nrow * (HDP / 4); i += GD_THREADS) {
+            const int row = i / (HDP / 4), d = i % (HDP / 4) * 4;
+            float o[4] = {};
+#pragma unroll
+            for (int w = 0; w < GD_WARPS; w++) {
+                const float4 v = *reinterpret_cast<const float4 *>(row_at(w, s_stage[w], row) + d);
+                const float f = s_f[w][row];
+                o[0] += v.x * f;
+                o[1] += v.y * f;
+                o[2] += v.z * f;
+                o[3] += v.w * f;
+            }
+            if (whole) put(row, d, o);
+            else __stcg(reinterpret_cast<float4 *>(piece + 16 + 4 * i), make_float4(o[0], o[1], o[2], o[3]));
         }
         if (tid < g.nrow) {
             if (!whole) __stcg(piece + tid, s_row[tid]);
@@ -767,52 +780,44 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                 const int n = c1 - c0 + 1;
                 // piece x of the item: the first CTA's second slot, the others' first
                 auto at = [&](int x) { return a.part + ((long long)(c0 + x) * 2 + (x == 0 ? 1 : 0)) * gqa_piece(HDP); };
-                if (n <= 8) {  // all of a value's pieces in one round of loads
-                    for (int i = tid; i < g.nrow * HDP; i += GD_THREADS) {
-                        const int row = i / HDP, d = i % HDP;
-                        float z[8], v[8], M = -INFINITY, L = 0.0f, o = 0.0f;
+                // four values a thread, GD_JOIN pieces in one round of loads
+                for (int i = tid; i < g.nrow * (HDP / 4); i += GD_THREADS) {
+                    const int row = i / (HDP / 4), d = i % (HDP / 4) * 4;
+                    float M = -INFINITY, L = 0.0f, o[4] = {};
+                    for (int x0 = 0; x0 < n; x0 += GD_JOIN) {
+                        float z[GD_JOIN];
+                        float4 v[GD_JOIN];
 #pragma unroll
-                        for (int x = 0; x < 8; x++) {
-                            z[x] = x < n ? __ldcg(at(x) + row) : -INFINITY;
-                            v[x] = x < n ? __ldcg(at(x) + 16 + i) : 0.0f;
+                        for (int x = 0; x < GD_JOIN; x++) {
+                            z[x] = -INFINITY;
+                            v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (x0 + x < n) {
+                                z[x] = __ldcg(at(x0 + x) + row);
+                                v[x] = __ldcg(reinterpret_cast<const float4 *>(at(x0 + x) + 16 + 4 * i));
+                            }
                         }
+                        float top = M;
 #pragma unroll
-                        for (int x = 0; x < 8; x++) M = fmaxf(M, z[x]);
-                        if (M == -INFINITY) M = 0.0f;
+                        for (int x = 0; x < GD_JOIN; x++) top = fmaxf(top, z[x]);
+                        const float ref = top == -INFINITY ? 0.0f : top, f = ex2(M - ref);
+                        M = top;
+                        L *= f;
 #pragma unroll
-                        for (int x = 0; x < 8; x++) {
-                            const float w = ex2(z[x] - M);
+                        for (int y = 0; y < 4; y++) o[y] *= f;
+#pragma unroll
+                        for (int x = 0; x < GD_JOIN; x++) {
+                            const float w = ex2(z[x] - ref);
                             L += w;
-                            o += v[x] * w;
+                            o[0] += v[x].x * w;
+                            o[1] += v[x].y * w;
+                            o[2] += v[x].z * w;
+                            o[3] += v[x].w * w;
                         }
-                        if (d < c.hd) ((T *)a.out)[(row_out + row) * c.hd + d] = from_f<T>(L == 0.0f ? 0.0f : o / L);
-                        if (d == 0 && a.lse)
-                            a.lse[row_out + row] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
                     }
-                } else {
-                for (int row = warp; row < g.nrow; row += GD_WARPS) {
-                    float M = -INFINITY, L = 0.0f;
-                    for (int x = lane; x < n; x += 32) M = fmaxf(M, __ldcg(at(x) + row));
-                    M = warp_max(M);
-                    const float M0 = M == -INFINITY ? 0.0f : M;
-                    for (int x = lane; x < n; x += 32) L += ex2(__ldcg(at(x) + row) - M0);
-                    L = warp_sum(L);
-                    if (lane == 0) {
-                        s_m[0][row] = M0;
-                        s_f[0][row] = L == 0.0f ? 0.0f : 1.0f / L;
-                        s_row[row] = L == 0.0f ? -INFINITY : M0 + log2f(L);
-                    }
-                }
-                __syncthreads();
-                for (int i = tid; i < g.nrow * HDP; i += GD_THREADS) {
-                    const int row = i / HDP, d = i % HDP;
-                    const float M0 = s_m[0][row];
-                    float o = 0.0f;
-#pragma unroll 8
-                    for (int x = 0; x < n; x++) o += __ldcg(at(x) + 16 + i) * ex2(__ldcg(at(x) + row) - M0);
-                    if (d < c.hd) ((T *)a.out)[(row_out + row) * c.hd + d] = from_f<T>(o * s_f[0][row]);
-                }
-                if (tid < g.nrow && a.lse) a.lse[row_out + tid] = s_row[tid] * 0.6931471805599453f;
+#pragma unroll
+                    for (int y = 0; y < 4; y++) o[y] = L == 0.0f ? 0.0f : o[y] / L;
+                    put(row, d, o);
+                    if (d == 0 && a.lse) a.lse[row_out + row] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
                 }
             }
         }
@@ -842,7 +847,7 @@ static int gd_launch_as(const GqaDecodeArgs &a, int sm_count, cudaStream_t st, s
         return WB_ECUDA;
     }
     ProfScope ps("gqa_decode", st);
-    gqa_decode_kernel<T, KIND, HDP, NB, FULL><<<gd_grid(a.c, a.H, sm_count, F::CTAS), GD_THREADS, F::BYTES, st>>>(a);
+    gqa_launch(gqa_decode_kernel<T, KIND, HDP, NB, FULL>, gd_grid(a.c, a.H, sm_count, F::CTAS), GD_THREADS, F::BYTES, st, a);
     return WB_OK;
 }
 
