@@ -441,10 +441,10 @@ WB_API int wb_lm_head(wb_context *ctx, const float *hidden, int n_rows, int n_em
  * whole fp32 layer calls and no cache for this attention.  The projections
  * around it stay with the caller.  Data pointers here are DEVICE memory;
  * index arrays (cu_*, slots, start) may be host memory, which is checked in
- * full before anything is queued, or device memory, which the host does not
- * read (no synchronisation; can be captured in a CUDA graph): the kernels
- * then skip what lies outside the buffers and set bit 0x8 (bounds) of the
- * device error word. */
+ * full before anything is queued and refused while the stream is captured, or
+ * device memory, which the host does not read (no synchronisation; can be
+ * captured in a CUDA graph): the kernels then skip what lies outside the
+ * buffers and set bit 0x8 (bounds) of the device error word. */
 /* element types */
 #define WB_BF16 0
 #define WB_F16 1

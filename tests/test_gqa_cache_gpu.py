@@ -367,3 +367,35 @@ def test_decode_graph_and_step():
         a, b = out.double(), at(full, t).double()
         assert ((a - b).abs() <= 2 ** -7 * (1 + b.abs())).all()
     assert cache.lens[0].tolist() == [T, T]
+
+
+def test_host_index_arrays_are_refused_during_a_capture():
+    """A graph would read them after they are gone; the capture itself goes on."""
+    import torch
+    import wave_engine_b200 as wb
+    T, Hkv, hd = 5, 2, 64
+    k, v = _rows(3, torch.bfloat16, T, Hkv, hd)
+    q = torch.randn(T, 4, hd, device="cuda").to(torch.bfloat16)
+    cu = torch.tensor([0, 2, T], dtype=torch.int32, device="cuda")
+    cache = wb.GqaCache(1, Hkv, hd, 2, 128, 2)
+    cache.reserve(0, 8)
+    cache.reserve(1, 8)
+    calls = [lambda c: wb.gqa_attention(q, k, v, c), lambda c: cache.write(0, k, v, cu=c),
+             lambda c: cache.read(0, cu=c, total=T)]
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for call in calls:
+            call(cu)
+        want = wb.gqa_attention(q, k, v, cu)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = wb.gqa_attention(q, k, v, cu)
+            for call in calls:
+                with pytest.raises(wb.WaveB200Error, match="captured"):
+                    call([0, 2, T])
+            with pytest.raises(wb.WaveB200Error, match="captured"):
+                cache.decode(0, q[:2], slots=[1, 0])
+        graph.replay()
+        stream.synchronize()
+    assert torch.equal(out, want)

@@ -175,4 +175,6 @@ def check(rc: int, func: str) -> None:
 
 
 def call(func: str, *args) -> None:
-    check(getattr(lib(), func)(*args), func)
+    rc = getattr(_lib or lib(), func)(*args)
+    if rc != WB_OK:
+        check(rc, func)

@@ -1937,6 +1937,11 @@ struct IndexArgs {
     size_t bytes() const { return ints * sizeof(int32_t); }
     int upload(void *at, cudaStream_t st) {
         if (host.empty()) return WB_OK;
+        // a graph would copy from host memory that is gone when it runs
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        WB_CUDA(cudaStreamIsCapturing(st, &capture));
+        if (capture != cudaStreamCaptureStatusNone)
+            return fail(WB_EINVAL, "index arrays must be device memory while the stream is captured");
         std::vector<int32_t> all(ints, 0);
         size_t off = 0;
         for (const One &o : host) {

@@ -11,7 +11,7 @@ Tensors are torch CUDA tensors, bf16 or fp16, used in place on torch's
 current stream; q, k and v may be slices of a fused projection's rows (only
 the last dimension has to be contiguous).  Index arrays (``cu``, ``start``,
 ``slots``) are int32 CUDA tensors, which the host does not read, or host
-sequences, which are checked.  The work runs in the CUDA library
+sequences, which are checked (not while a CUDA graph is captured).  The work runs in the CUDA library
 (``wb_gqa_*``, include/wave_b200.h); there is no CPU path.
 """
 from __future__ import annotations
@@ -72,9 +72,8 @@ def _rows(x, name: str, dtype=None):
     return ts, hs
 
 
-def _context(ctx, device) -> Context:
+def _context(ctx, index: int) -> Context:
     """The context for a device, on torch's current stream there."""
-    index = device.index
     if ctx is None:
         ctx = default_context(index)
     elif ctx.device != index:
@@ -85,18 +84,19 @@ def _context(ctx, device) -> Context:
     return ctx
 
 
-def _out(out, shape, dtype, device, name):
+def _out(out, q):
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)  # contiguous, whatever the rows' strides are
-    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
-        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on {device}")
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {q.device}")
     return out
 
 
-def _same_device(device, *others) -> None:
+def _same_device(x, *others) -> None:
+    index = x.get_device()
     for t in others:
-        if isinstance(t, torch.Tensor) and t.is_cuda and t.device != device:
-            raise ValueError(f"tensors on {device} and on {t.device}")
+        if t is not None and isinstance(t, torch.Tensor) and t.get_device() != index and t.is_cuda:
+            raise ValueError(f"tensors on {x.device} and on {t.device}")
 
 
 def gqa_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float | None = None,
@@ -114,17 +114,16 @@ def gqa_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float
     Tk, Hkv, _ = k.shape
     if k.shape != v.shape or k.shape[2] != hd:
         raise ValueError("k and v must be [tokens][n_kv_head][head_dim], head_dim as q's")
-    device = q.device
-    _same_device(device, k, v, cu_q, cu_k)
+    _same_device(q, k, v, cu_q, cu_k)
     n_seq = len(cu_q) - 1
     if n_seq < 0:
         raise ValueError("cu_q must have one entry more than there are sequences")
     pq, keep_q = _index(cu_q, n_seq + 1, "cu_q")
     pk, keep_k = _index(cu_k, n_seq + 1, "cu_k")
-    out = _out(out, (Tq, H, hd), q.dtype, device, "out")
+    out = _out(out, q)
     o_ts, o_hs = _rows(out, "out", q.dtype)
-    lse = torch.empty((H, Tq), dtype=torch.float32, device=device) if return_lse else None
-    ctx = _context(ctx, device)
+    lse = q.new_empty((H, Tq), dtype=torch.float32) if return_lse else None
+    ctx = _context(ctx, q.get_device())
     d = _ATTN.pack(_DTYPES[q.dtype], H, Hkv, hd, n_seq, bool(causal), hd ** -0.5 if scale is None else scale, Tq, Tk,
                    q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, pq, pk,
                    out.data_ptr(), o_ts, o_hs, 0 if lse is None else lse.data_ptr())
@@ -133,7 +132,7 @@ def gqa_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float
 
 
 def _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, dtype, head_dim):
-    shape, device = k_pages.shape, k_pages.device
+    shape, index = k_pages.shape, k_pages.get_device()
     if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != k_pages.dtype:
         raise ValueError("k_pages and v_pages must be [n_pages][n_kv_head][128][row]")
     n_pages, Hkv, page, row = shape
@@ -155,9 +154,10 @@ def _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, dtype, head_dim
             raise ValueError("lens must be int32 [n_slots]")
         arrays.append(lens)
     for x in arrays:
-        if not x.is_contiguous() or not x.is_cuda or x.device != device:
+        if index < 0 or x.get_device() != index or not x.is_contiguous():
             raise ValueError("cache arrays must be contiguous CUDA tensors of one device")
-    return _CACHE.pack(_DTYPES[dtype], store, Hkv, head_dim, n_pages, table.shape[0], table.shape[1],
+    n_slots, max_pages = table.shape
+    return _CACHE.pack(_DTYPES[dtype], store, Hkv, head_dim, n_pages, n_slots, max_pages,
                        k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(),
                        0 if lens is None else lens.data_ptr())
 
@@ -184,12 +184,12 @@ def gqa_cache_write(k, v, k_pages, v_pages, table, lens, *, cu=None, start=None,
         raise ValueError("k and v must be [tokens][n_kv_head][head_dim]")
     total, _, hd = k.shape
     d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, k.dtype, hd)
-    _same_device(k.device, v, k_pages, cu, start, slots)
+    _same_device(k, v, k_pages, cu, start, slots)
     n_seq = _n_seq(table, cu, slots, total)
     pc, keep_c = _index(cu, n_seq + 1, "cu")
     ps, keep_s = _index(start, n_seq, "start")
     pl, keep_l = _index(slots, n_seq, "slots")
-    ctx = _context(ctx, k.device)
+    ctx = _context(ctx, k.get_device())
     _lib.call("wb_gqa_cache_write", ctx.handle, d, pl, n_seq, pc, total, ps, k.data_ptr(), k_ts, k_hs,
               v.data_ptr(), v_ts, v_hs)
 
@@ -203,7 +203,7 @@ def gqa_cache_read(k_pages, v_pages, table, *, head_dim: int, dtype, cu=None, to
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16 or float16")
     d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, None, dtype, head_dim)
-    _same_device(k_pages.device, cu, start, slots)
+    _same_device(k_pages, cu, start, slots)
     n_seq = _n_seq(table, cu, slots)
     if total is None:
         if cu is not None and isinstance(cu, torch.Tensor) and cu.is_cuda:
@@ -212,10 +212,9 @@ def gqa_cache_read(k_pages, v_pages, table, *, head_dim: int, dtype, cu=None, to
     pc, keep_c = _index(cu, n_seq + 1, "cu")
     ps, keep_s = _index(start, n_seq, "start")
     pl, keep_l = _index(slots, n_seq, "slots")
-    shape = (total, k_pages.shape[1], head_dim)
-    k = torch.empty(shape, dtype=dtype, device=k_pages.device)
-    v = torch.empty(shape, dtype=dtype, device=k_pages.device)
-    ctx = _context(ctx, k_pages.device)
+    k = k_pages.new_empty((total, k_pages.shape[1], head_dim), dtype=dtype)
+    v = torch.empty_like(k)
+    ctx = _context(ctx, k_pages.get_device())
     _lib.call("wb_gqa_cache_read", ctx.handle, d, pl, n_seq, pc, total, ps, k.data_ptr(), v.data_ptr())
     return k, v
 
@@ -228,14 +227,13 @@ def gqa_decode(q, k_pages, v_pages, table, lens, *, slots=None, k_scale=None, v_
     q_ss, q_hs = _rows(q, "q")
     n_seq, H, hd = q.shape
     d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, q.dtype, hd)
-    device = q.device
-    _same_device(device, k_pages, slots)
+    _same_device(q, k_pages, slots)
     pl, keep_l = _index(slots, n_seq, "slots")
-    out = _out(out, (n_seq, H, hd), q.dtype, device, "out")
+    out = _out(out, q)
     if not out.is_contiguous():
         raise ValueError("out must be contiguous")
-    lse = torch.empty((n_seq, H), dtype=torch.float32, device=device) if return_lse else None
-    ctx = _context(ctx, device)
+    lse = q.new_empty((n_seq, H), dtype=torch.float32) if return_lse else None
+    ctx = _context(ctx, q.get_device())
     _lib.call("wb_gqa_decode", ctx.handle, d, pl, n_seq, H, q.data_ptr(), q_ss, q_hs,
               hd ** -0.5 if scale is None else scale, out.data_ptr(), 0 if lse is None else lse.data_ptr())
     return (out, lse) if return_lse else out
