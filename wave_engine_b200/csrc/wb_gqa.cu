@@ -664,58 +664,63 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
             const int edges = max(0, mine - edge);
             // 32 columns at a time through shared memory, so that a store
             // instruction writes 64 bytes of eight rows (a thread per row
-            // took 4 us): 16-byte piece c of a row at place c ^ (row / 2 & 3)
+            // took 4 us): 16-byte piece c of a row at place c ^ (row / 2 & 3).
+            // The loops are short: this code runs once an item and is fetched
+            // anew each time (unrolled it took 1 us of an item's 3).
             uint8_t *stage = sm + F::OFF_OUT + warp * F::OUT_WARP;
 #pragma unroll 1
-            for (int x = 0; x < HDP / 32 && 32 * x < a.hd; x++) {
-                uint32_t o[32];
-                __syncwarp();
+            for (int x = 0; x < HDP / 16 && 16 * x < a.hd; x++) {
+                uint32_t o[16];
                 if (mine > 0) {
-                    ptx::tmem_ld32(O + 32 * x, o);
+                    ptx::tmem_ld16(O + 16 * x, o);
                     ptx::tmem_ld_wait();
                 }
-                if (noted && real) {
-                    for (int e = 0; e < edges; e++)
-                        for (int i = 0; i < GA_KEYS; i++) {
-                            const int key = (edge + e) * GA_KEYS + i;
-                            if (key >= vis || !(it->bad[e][i >> 5] >> (i & 31) & 1)) continue;
-                            const T *v = (const T *)a.v + (long long)(k0 + key) * a.v_ts + (long long)hk * a.v_hs;
+                uint32_t w[8];
 #pragma unroll
-                            for (int d = 0; d < 32; d++)
-                                if (32 * x + d < a.hd) {
-                                    const float y = to_f(v[32 * x + d]);
-                                    if (!isfinite(y)) o[d] = __float_as_uint(__uint_as_float(o[d]) + y);
-                                }
-                        }
+                for (int i = 0; i < 8; i++) {
+                    w[i] = ga_pack<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+                    if (none) w[i] = 0;
                 }
 #pragma unroll
-                for (int i = 0; i < 32; i++) o[i] = none ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint4 w;
-                    w.x = ga_pack<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]));
-                    w.y = ga_pack<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
-                    w.z = ga_pack<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
-                    w.w = ga_pack<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
-                    *reinterpret_cast<uint4 *>(stage + lane * 64 + (i ^ (lane >> 1 & 3)) * 16) = w;
-                }
+                for (int i = 0; i < 2; i++)
+                    *reinterpret_cast<uint4 *>(stage + lane * 64 + ((2 * (x & 1) + i) ^ (lane >> 1 & 3)) * 16) =
+                        make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                if (!(x & 1) && 16 * x + 16 < a.hd) continue;
                 __syncwarp();
+                const int x0 = 32 * (x >> 1);
                 if (ga.vec) {
-                    const int c = lane & 3;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int r = 8 * i + (lane >> 2);
+                    const int d = x0 + 8 * (lane & 3);
+#pragma unroll 1
+                    for (int r = lane >> 2; r < 32; r += 8) {
                         const long long to = __shfl_sync(0xffffffffu, at, r);
-                        if ((rows >> r & 1) && 32 * x + 8 * c < a.hd)
-                            *reinterpret_cast<uint4 *>((T *)a.out + to + 32 * x + 8 * c) =
-                                *reinterpret_cast<const uint4 *>(stage + r * 64 + (c ^ (r >> 1 & 3)) * 16);
+                        if ((rows >> r & 1) && d < a.hd)
+                            *reinterpret_cast<uint4 *>((T *)a.out + to + d) =
+                                *reinterpret_cast<const uint4 *>(stage + r * 64 + ((lane & 3) ^ (r >> 1 & 3)) * 16);
                     }
                 } else {
+#pragma unroll 8
                     for (int r = 0; r < 32; r++) {
                         const long long to = __shfl_sync(0xffffffffu, at, r);
-                        if ((rows >> r & 1) && 32 * x + lane < a.hd)
-                            ((T *)a.out)[to + 32 * x + lane] =
+                        if ((rows >> r & 1) && x0 + lane < a.hd)
+                            ((T *)a.out)[to + x0 + lane] =
                                 *reinterpret_cast<const T *>(stage + r * 64 + ((lane >> 3) ^ (r >> 1 & 3)) * 16 + (lane & 7) * 2);
+                    }
+                }
+                __syncwarp();
+            }
+            // Values at the edges that are not finite: the sum is whatever
+            // they make of it.
+            if (noted && real) {
+#pragma unroll 1
+                for (int i = 0; i < edges * GA_KEYS; i++) {
+                    const int key = edge * GA_KEYS + i;
+                    if (key >= vis || !(it->bad[i / GA_KEYS][(i >> 5) & 3] >> (i & 31) & 1)) continue;
+                    const T *v = (const T *)a.v + (long long)(k0 + key) * a.v_ts + (long long)hk * a.v_hs;
+                    T *o = (T *)a.out + at;
+#pragma unroll 1
+                    for (int d = 0; d < a.hd; d++) {
+                        const float y = to_f(v[d]);
+                        if (!isfinite(y)) o[d] = from_f<T>(to_f(o[d]) + y);
                     }
                 }
             }
