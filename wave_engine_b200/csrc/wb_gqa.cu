@@ -16,12 +16,27 @@
 // tile: row = token * G + g, 128 / G tokens of G heads, which TMA gathers as
 // one box.  A CTA has two such tiles, one softmax warpgroup each: while the
 // tensor cores work for one, the other's warps take exponentials, and both
-// read the same K and V tiles (128 keys).  At head_dim 128 a pair of tiles
-// costs 2048 tensor cycles and, at 16 ex2 per cycle and SM, 2048 cycles of
-// the exponential unit; what a tile waits for is the chain S -> softmax ->
-// P V -> next S, so P is handed over in two halves.  (Exponentials by a
-// polynomial on the FMA pipe were measured and not kept: a quarter of them
-// cost 4% at 8192 tokens, three eighths 7%.)
+// read the same K and V tiles (128 keys).  P is handed over in two halves,
+// so that its product begins while the second is computed.
+//
+// What bounds it.  A pair of tiles costs 2048 cycles of the tensor cores at
+// head_dim 128 (1024 at 64) and, at 16 ex2 per cycle and SM, 2048 of the
+// exponential unit.  It takes about 3400 (3050): a tile's chain is 400 to 600
+// cycles for the maximum, 1350 to 1700 for the exponentials (the other tile's
+// among them), then 700 (400) to issue and run P V and the next Q K^T and 350
+// until the scores are seen.  One sequence of 8192 tokens, 32 heads on 8,
+// head_dim 128, causal: 431 us, 1277 TFLOP/s, 76% of the measured cuBLAS
+// rate; there the chip is at its power limit (with the two tiles half a
+// period apart a pair takes 3310 cycles at a clock 4% lower: the same time).
+// Short sequences pay the start and end of an item, about 4000 cycles: 32
+// sequences of 1 to 1024 tokens, 12 heads on 4, head_dim 64: 60 us.
+//
+// Measured and not kept: exponentials by a polynomial on the FMA pipe (a
+// quarter of them cost 4% at 8192 tokens, three eighths 7%); eight softmax
+// warps a tile (+10%); a warp for each tile's products (+25%); a third S
+// buffer at head_dim 64, so that Q K^T runs ahead (+12%: more barriers and
+// registers than it hides); the next item's first Q K^T issued before this
+// one's epilogue (+4% at head_dim 64: it waits for Q).
 #include "wb_gqa.h"
 #include "wb_tc.h"
 
@@ -116,17 +131,6 @@ __device__ __forceinline__ uint32_t ga_pack(float lo, float hi) {
     return r;
 }
 
-__device__ __forceinline__ void ga_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-
 // tcgen05.mma with A from shared memory or TMEM; descriptors as low and high
 // words
 template <bool ACC>
@@ -157,12 +161,15 @@ __device__ __forceinline__ int ga_items(const GqaAttnArgs &a, int b, int per_ite
 }
 
 // Finds the sequence and tiles of ascending item indexes; one warp.  Up to
-// 256 sequences: tiles late in their sequences (with the most keys) first --
+// 64 sequences: tiles late in their sequences (with the most keys) first --
 // the largest t with more than `index` items at or behind place t, then by
-// sequence -- so that long items are dealt out first.  More: in the order of
-// the sequences, one pass over them for all items of the CTA.
+// sequence -- so that long items are dealt out first (8 sequences up to 4096:
+// 135 us, 159 in the sequences' order; 32 up to 1024: 62, 67).  More: in
+// the order of the sequences, one pass over them for all items of the CTA
+// (64 up to 600: 65 us both ways; 255 up to 400: 126 us, 140 with the longest
+// first).
 struct GaFinder {
-    static constexpr int N = 8;
+    static constexpr int N = 2;
     int n[N];                // items of sequences lane + 32 x (or of sequences b0 + lane, in n[0])
     int top = 0, b0 = 0;
     long long before = 0;    // items of sequences before b0
@@ -865,6 +872,8 @@ int launch_gqa_attention(const GqaAttnArgs &args, int dtype, void *scratch, int 
         ProfScope ps("gqa_rows", st);
         gqa_rows_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(js);
     }
+    // rows of up to 64 in 64 columns (in 128: 71 us instead of 62, packed
+    // 768-wide batch)
     if (dtype == WB_BF16)
         return a.hd <= 64 ? ga_launch<__nv_bfloat16, 64>(ga, sm_count, st, msg) : ga_launch<__nv_bfloat16, 128>(ga, sm_count, st, msg);
     return a.hd <= 64 ? ga_launch<__half, 64>(ga, sm_count, st, msg) : ga_launch<__half, 128>(ga, sm_count, st, msg);

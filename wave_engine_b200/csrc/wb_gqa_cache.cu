@@ -14,6 +14,10 @@
 // reading, four rows a thread under way at once.  The rows of a
 // block are loaded before their places in the cache are looked up (sequence,
 // slot, start, page: dependent loads that take as long as the data).
+// 8 x 4096 positions of 8 heads x 128, fp16 to e4m3 and back: 45.9 + 35.7 us
+// apart, 76 us in a row (203 MB each way, 5.3 TB/s of 6.5; below it stays what
+// a warp has to do a row: the maximum over its lanes, the quotients).  One
+// position of 32 sequences: 7.0 us for both, launches and the dependent loads.
 #include "wb_gqa.h"
 
 #include <algorithm>
