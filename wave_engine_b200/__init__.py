@@ -5,7 +5,9 @@ The hot path of wave-engine's causal multi-head wave attention forward
 (include/wave_b200.h) implemented by the in-tree CUDA library
 ``libwave_b200.so``.  This package is the host-side mirror of the
 reference's interface for that path, plus the legacy dot-product attention
-of ComputeBackend::attention (src/common/compute.rs:43, :357-414).
+of ComputeBackend::attention (src/common/compute.rs:43, :357-414), and a
+16-bit serving form of that attention with shared key-value heads: packed
+prompts, a paged cache, one new token over it (gqa.py).
 """
 from .weights import CONTENT_DIM, Rng, WaveAttnHeadWeights, WaveAttnWeights, gaussian_block_attn, init_block_attn
 from .runtime import AttnLayer, Context, default_context
