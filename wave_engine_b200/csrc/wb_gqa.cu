@@ -36,7 +36,8 @@
 // warps a tile (+10%); a warp for each tile's products (+25%); a third S
 // buffer at head_dim 64, so that Q K^T runs ahead (+12%: more barriers and
 // registers than it hides); the next item's first Q K^T issued before this
-// one's epilogue (+4% at head_dim 64: it waits for Q).
+// one's epilogue (+4% at head_dim 64, with Q in two buffers +5%: it goes in
+// front of the other tile's last products).
 #include "wb_gqa.h"
 #include "wb_tc.h"
 
