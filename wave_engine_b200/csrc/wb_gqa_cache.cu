@@ -14,8 +14,8 @@
 // reading, four rows a thread under way at once.  The rows of a
 // block are loaded before their places in the cache are looked up (sequence,
 // slot, start, page: dependent loads that take as long as the data).
-// 8 x 4096 positions of 8 heads x 128, fp16 to e4m3 and back: 45.9 + 35.7 us
-// apart, 76 us in a row (203 MB each way, 5.3 TB/s of 6.5; below it stays what
+// 8 x 4096 positions of 8 heads x 128, fp16 to e4m3 and back: 43.6 + 35.2 us
+// apart, 74 us in a row (203 MB each way, 5.5 TB/s of 6.5; below it stays what
 // a warp has to do a row: the maximum over its lanes, the quotients).  One
 // position of 32 sequences: 7.0 us for both, launches and the dependent loads.
 #include "wb_gqa.h"
@@ -35,8 +35,8 @@ struct GqaMove {
     uint32_t inv;          // 2^32 / Hkv rounded up
 };
 
-static constexpr int GM_THREADS = 256, GM_ROWS = 4;  // rows of a thread
-static constexpr int GM_CTAS = 4;  // write blocks per SM
+static constexpr int GM_THREADS = 128, GM_ROWS = 4;  // rows of a thread
+static constexpr int GM_CTAS = 8;  // write blocks per SM (256 threads and 4 blocks: 76 us instead of 74, 64 and 16: 82)
 
 // Row `local` of a block (counted from its first token's first head): token
 // and head.  inv = 2^32 / Hkv rounded up, so the quotient is right or one
