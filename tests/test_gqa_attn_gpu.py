@@ -164,6 +164,33 @@ def test_unseen_values_do_not_leak(bad, H, Hkv, hd):
     assert torch.equal(got[~own], clean[~own]) and not torch.isfinite(got[own]).any()
 
 
+@pytest.mark.parametrize("n", [63, 64, 65, 200])
+def test_many_sequences(n):
+    """Both orders in which items are dealt out: sequences of no tokens up to several items."""
+    _run("bfloat16", 6, 2, 64, [(i * 37) % 211 if i % 5 else 0 for i in range(n)], seed=n)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("H,Hkv,hd", [(6, 2, 64), (8, 1, 128), (6, 2, 42)])
+def test_queries_do_not_reach_each_other(bad, H, Hkv, hd):
+    """A query that is not finite makes its own head NaN; rows of the same
+    tile (the next sequence's among them) stay as they are."""
+    import torch
+    import wave_engine_b200 as wb
+    cu = ref.starts([70, 1, 300])
+    q, k, v = _inputs(12, torch.bfloat16, H, Hkv, hd, cu[-1], cu[-1])
+    clean, clean_lse = wb.gqa_attention(q, k, v, cu, return_lse=True)
+    q2 = q.clone()
+    hit = torch.zeros(cu[-1], H, dtype=torch.bool, device="cuda")
+    for t, h in ((70, 1), (71, 0), (71 + 41, H - 1), (370, 2)):
+        q2[t, h, 0] = bad
+        hit[t, h] = True
+    got, lse = wb.gqa_attention(q2, k, v, cu, return_lse=True)
+    assert torch.equal(got[~hit], clean[~hit]) and torch.equal(lse.T[~hit], clean_lse.T[~hit])
+    if bad != bad:
+        assert got[hit].isnan().all() and lse.T[hit].isnan().all()
+
+
 def test_same_bits_and_streams():
     import torch
     import wave_engine_b200 as wb
