@@ -1,5 +1,5 @@
-"""Grouped-head dot-product attention in 16 bits, for serving: attention over
-packed prompts, a paged key-value cache (16-bit, or quantised to int8 / e4m3
+"""Grouped-head dot-product attention in 16 bits, for serving (forward only):
+attention over packed prompts, a paged key-value cache (16-bit, or quantised to int8 / e4m3
 as it is written) and the attention of one new token over it.
 
     out = gqa_attention(q, k, v, cu_q)                       # whole prompts
@@ -44,14 +44,25 @@ def _row(head_dim: int) -> int:
     return -(-head_dim // 16) * 16
 
 
-def _index(a, n: int, name: str):
+def _elsewhere(a: int, b: int):
+    return ValueError(f"tensors on devices {a} and {b} (-1 is the host)")
+
+
+def _entries(a) -> int:
+    return a.shape[0] if isinstance(a, torch.Tensor) and a.dim() == 1 else len(a)
+
+
+def _index(a, n: int, name: str, device: int):
     """(address, object to keep) of an int32 index array of n entries; None is (0, None)."""
     if a is None:
         return 0, None
-    if isinstance(a, torch.Tensor) and a.is_cuda:
-        if a.dtype != torch.int32 or a.dim() != 1 or not a.is_contiguous():
+    if isinstance(a, torch.Tensor) and (at := a.get_device()) >= 0:
+        shape = a.shape
+        if a.dtype is not torch.int32 or len(shape) != 1 or not a.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 vector")
-        keep, size, ptr = a, a.shape[0], a.data_ptr()
+        if at != device:
+            raise _elsewhere(device, at)
+        keep, size, ptr = a, shape[0], a.data_ptr()
     else:
         keep = np.ascontiguousarray(a.numpy() if isinstance(a, torch.Tensor) else a, dtype=np.int32)
         size, ptr = keep.size, keep.ctypes.data
@@ -64,7 +75,8 @@ def _rows(x, name: str, dtype=None):
     """Strides of [tokens][heads][head_dim] rows, checked."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 3:
         raise ValueError(f"{name} must be a CUDA tensor [tokens][heads][head_dim]")
-    if x.dtype not in _DTYPES or (dtype is not None and x.dtype != dtype):
+    t = x.dtype
+    if t not in _DTYPES or (dtype is not None and t is not dtype):
         raise ValueError(f"{name} must be bfloat16 or float16, as the others")
     ts, hs, ds = x.stride()
     if ds != 1 and x.shape[2] > 1:
@@ -92,13 +104,6 @@ def _out(out, q):
     return out
 
 
-def _same_device(x, *others) -> None:
-    index = x.get_device()
-    for t in others:
-        if t is not None and isinstance(t, torch.Tensor) and t.get_device() != index and t.is_cuda:
-            raise ValueError(f"tensors on {x.device} and on {t.device}")
-
-
 def gqa_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float | None = None,
                   return_lse: bool = False, out=None, ctx: Context | None = None):
     """Attention over packed prompts (wb_gqa_attention).
@@ -108,23 +113,29 @@ def gqa_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float
     None: head_dim ** -0.5.  Returns out like q, and with ``return_lse`` also
     the log sum exp of every query's scores, [n_head][tokens] fp32."""
     q_ts, q_hs = _rows(q, "q")
-    k_ts, k_hs = _rows(k, "k", q.dtype)
-    v_ts, v_hs = _rows(v, "v", q.dtype)
+    dtype, device = q.dtype, q.get_device()
+    k_ts, k_hs = _rows(k, "k", dtype)
+    v_ts, v_hs = _rows(v, "v", dtype)
     Tq, H, hd = q.shape
-    Tk, Hkv, _ = k.shape
-    if k.shape != v.shape or k.shape[2] != hd:
+    Tk, Hkv, k_hd = shape = k.shape
+    if v.shape != shape or k_hd != hd:
         raise ValueError("k and v must be [tokens][n_kv_head][head_dim], head_dim as q's")
-    _same_device(q, k, v, cu_q, cu_k)
-    n_seq = len(cu_q) - 1
+    if k.get_device() != device or v.get_device() != device:
+        raise _elsewhere(device, k.get_device() if k.get_device() != device else v.get_device())
+    n_seq = _entries(cu_q) - 1
     if n_seq < 0:
         raise ValueError("cu_q must have one entry more than there are sequences")
-    pq, keep_q = _index(cu_q, n_seq + 1, "cu_q")
-    pk, keep_k = _index(cu_k, n_seq + 1, "cu_k")
-    out = _out(out, q)
-    o_ts, o_hs = _rows(out, "out", q.dtype)
+    pq, keep_q = _index(cu_q, n_seq + 1, "cu_q", device)
+    pk, keep_k = _index(cu_k, n_seq + 1, "cu_k", device)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        o_ts, o_hs = H * hd, hd
+    else:
+        out = _out(out, q)
+        o_ts, o_hs = _rows(out, "out", dtype)
     lse = q.new_empty((H, Tq), dtype=torch.float32) if return_lse else None
-    ctx = _context(ctx, q.get_device())
-    d = _ATTN.pack(_DTYPES[q.dtype], H, Hkv, hd, n_seq, bool(causal), hd ** -0.5 if scale is None else scale, Tq, Tk,
+    ctx = _context(ctx, device)
+    d = _ATTN.pack(_DTYPES[dtype], H, Hkv, hd, n_seq, bool(causal), hd ** -0.5 if scale is None else scale, Tq, Tk,
                    q.data_ptr(), k.data_ptr(), v.data_ptr(), q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, pq, pk,
                    out.data_ptr(), o_ts, o_hs, 0 if lse is None else lse.data_ptr())
     _lib.call("wb_gqa_attention", ctx.handle, d)
@@ -132,41 +143,46 @@ def gqa_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float
 
 
 def _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, dtype, head_dim):
-    shape, index = k_pages.shape, k_pages.get_device()
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != k_pages.dtype:
+    shape, kind, index = k_pages.shape, k_pages.dtype, k_pages.get_device()
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not kind:
         raise ValueError("k_pages and v_pages must be [n_pages][n_kv_head][128][row]")
     n_pages, Hkv, page, row = shape
-    store = _STORES.get(k_pages.dtype)
+    store = _STORES.get(kind)
     if store is None or page != PAGE or row != _row(head_dim):
         raise ValueError(f"pages must hold {PAGE} rows of {_row(head_dim)} bf16, fp16, int8 or float8_e4m3fn values")
-    arrays = [k_pages, v_pages, table]
+    good = _held(k_pages, index) and _held(v_pages, index) and _held(table, index)
     ks = vs = 0
     if store == _lib.WB_INT8 or store == _lib.WB_E4M3:
+        scales = (n_pages, Hkv, page)
         for x in (k_scale, v_scale):
-            if x is None or x.shape != shape[:3] or x.dtype != torch.float32:
+            if x is None or x.shape != scales or x.dtype is not torch.float32:
                 raise ValueError("an 8-bit cache needs fp32 k_scale and v_scale [n_pages][n_kv_head][128]")
+        good = good and _held(k_scale, index) and _held(v_scale, index)
         ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
-        arrays += (k_scale, v_scale)
-    if table.dim() != 2 or table.dtype != torch.int32:
+    if table.dim() != 2 or table.dtype is not torch.int32:
         raise ValueError("table must be int32 [n_slots][max_pages]")
-    if lens is not None:
-        if lens.dtype != torch.int32 or lens.dim() != 1 or lens.shape[0] != table.shape[0]:
-            raise ValueError("lens must be int32 [n_slots]")
-        arrays.append(lens)
-    for x in arrays:
-        if index < 0 or x.get_device() != index or not x.is_contiguous():
-            raise ValueError("cache arrays must be contiguous CUDA tensors of one device")
     n_slots, max_pages = table.shape
+    pl = 0
+    if lens is not None:
+        if lens.dtype is not torch.int32 or lens.shape != (n_slots,):
+            raise ValueError("lens must be int32 [n_slots]")
+        good = good and _held(lens, index)
+        pl = lens.data_ptr()
+    if not good or index < 0:
+        raise ValueError("cache arrays must be contiguous CUDA tensors of one device")
     return _CACHE.pack(_DTYPES[dtype], store, Hkv, head_dim, n_pages, n_slots, max_pages,
-                       k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(),
-                       0 if lens is None else lens.data_ptr())
+                       k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(), pl)
+
+
+def _held(x, index: int) -> bool:
+    return x.get_device() == index and x.is_contiguous()
 
 
 def _n_seq(table, cu, slots, rows=None):
     if cu is not None:
-        return len(cu) - 1
+        return _entries(cu) - 1
     if slots is not None:
-        return len(slots)
+        return _entries(slots)
     return int(table.shape[0] if rows is None else rows)
 
 
@@ -179,17 +195,20 @@ def gqa_cache_write(k, v, k_pages, v_pages, table, lens, *, cu=None, start=None,
     length.  ``cu`` None: one row per sequence; ``start`` None: append;
     ``slots`` None: 0, 1, .."""
     k_ts, k_hs = _rows(k, "k")
-    v_ts, v_hs = _rows(v, "v", k.dtype)
-    if k.shape != v.shape or k.shape[1] != k_pages.shape[1]:
+    dtype, device = k.dtype, k.get_device()
+    v_ts, v_hs = _rows(v, "v", dtype)
+    total, Hkv, hd = shape = k.shape
+    if v.shape != shape or Hkv != k_pages.shape[1]:
         raise ValueError("k and v must be [tokens][n_kv_head][head_dim]")
-    total, _, hd = k.shape
-    d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, k.dtype, hd)
-    _same_device(k, v, k_pages, cu, start, slots)
+    d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, dtype, hd)
+    for x in (v, k_pages):
+        if x.get_device() != device:
+            raise _elsewhere(device, x.get_device())
     n_seq = _n_seq(table, cu, slots, total)
-    pc, keep_c = _index(cu, n_seq + 1, "cu")
-    ps, keep_s = _index(start, n_seq, "start")
-    pl, keep_l = _index(slots, n_seq, "slots")
-    ctx = _context(ctx, k.get_device())
+    pc, keep_c = _index(cu, n_seq + 1, "cu", device)
+    ps, keep_s = _index(start, n_seq, "start", device)
+    pl, keep_l = _index(slots, n_seq, "slots", device)
+    ctx = _context(ctx, device)
     _lib.call("wb_gqa_cache_write", ctx.handle, d, pl, n_seq, pc, total, ps, k.data_ptr(), k_ts, k_hs,
               v.data_ptr(), v_ts, v_hs)
 
@@ -203,18 +222,18 @@ def gqa_cache_read(k_pages, v_pages, table, *, head_dim: int, dtype, cu=None, to
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16 or float16")
     d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, None, dtype, head_dim)
-    _same_device(k_pages, cu, start, slots)
+    device = k_pages.get_device()
     n_seq = _n_seq(table, cu, slots)
     if total is None:
         if cu is not None and isinstance(cu, torch.Tensor) and cu.is_cuda:
             raise ValueError("total must be given when cu is on the device")
         total = n_seq if cu is None else int(cu[-1])
-    pc, keep_c = _index(cu, n_seq + 1, "cu")
-    ps, keep_s = _index(start, n_seq, "start")
-    pl, keep_l = _index(slots, n_seq, "slots")
+    pc, keep_c = _index(cu, n_seq + 1, "cu", device)
+    ps, keep_s = _index(start, n_seq, "start", device)
+    pl, keep_l = _index(slots, n_seq, "slots", device)
     k = k_pages.new_empty((total, k_pages.shape[1], head_dim), dtype=dtype)
     v = torch.empty_like(k)
-    ctx = _context(ctx, k_pages.get_device())
+    ctx = _context(ctx, device)
     _lib.call("wb_gqa_cache_read", ctx.handle, d, pl, n_seq, pc, total, ps, k.data_ptr(), v.data_ptr())
     return k, v
 
@@ -225,15 +244,17 @@ def gqa_decode(q, k_pages, v_pages, table, lens, *, slots=None, k_scale=None, v_
     (wb_gqa_decode): q [n_seq][n_head][head_dim] -> out like q (and lse
     [n_seq][n_head] fp32).  Write the token's own key and value first."""
     q_ss, q_hs = _rows(q, "q")
+    device = q.get_device()
     n_seq, H, hd = q.shape
     d = _cache_desc(k_pages, v_pages, k_scale, v_scale, table, lens, q.dtype, hd)
-    _same_device(q, k_pages, slots)
-    pl, keep_l = _index(slots, n_seq, "slots")
+    if k_pages.get_device() != device:
+        raise _elsewhere(device, k_pages.get_device())
+    pl, keep_l = _index(slots, n_seq, "slots", device)
     out = _out(out, q)
     if not out.is_contiguous():
         raise ValueError("out must be contiguous")
     lse = q.new_empty((n_seq, H), dtype=torch.float32) if return_lse else None
-    ctx = _context(ctx, q.get_device())
+    ctx = _context(ctx, device)
     _lib.call("wb_gqa_decode", ctx.handle, d, pl, n_seq, H, q.data_ptr(), q_ss, q_hs,
               hd ** -0.5 if scale is None else scale, out.data_ptr(), 0 if lse is None else lse.data_ptr())
     return (out, lse) if return_lse else out
