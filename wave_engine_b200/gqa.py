@@ -285,6 +285,9 @@ class GqaCache:
         self.k_scale, self.v_scale = scale(), scale()
         self.table = torch.full((max_seqs, self.max_pages), -1, dtype=torch.int32, device=dev)
         self.lens = torch.zeros((n_layers, max_seqs), dtype=torch.int32, device=dev)
+        # one layer's arrays: indexing them anew costs more than the rest of a call
+        self._layer = [(k, v, self.table, n, {"k_scale": ks, "v_scale": vs, "ctx": ctx}) for k, v, n, ks, vs in
+                       zip(self.k_pages, self.v_pages, self.lens, self.k_scale, self.v_scale)]
         self._free = list(range(n_pages - 1, -1, -1))
         self._held = [[] for _ in range(max_seqs)]
 
@@ -314,20 +317,19 @@ class GqaCache:
     def free_pages(self) -> int:
         return len(self._free)
 
-    def _layer(self, layer: int) -> dict:
-        return {"k_scale": self.k_scale[layer], "v_scale": self.v_scale[layer], "ctx": self.ctx}
-
     def write(self, layer: int, k, v, slots=None, cu=None, start=None) -> None:
         """gqa_cache_write into one layer."""
-        gqa_cache_write(k, v, self.k_pages[layer], self.v_pages[layer], self.table, self.lens[layer], cu=cu,
-                        start=start, slots=slots, **self._layer(layer))
+        k_pages, v_pages, table, lens, more = self._layer[layer]
+        gqa_cache_write(k, v, k_pages, v_pages, table, lens, cu=cu, start=start, slots=slots, **more)
 
     def read(self, layer: int, slots=None, cu=None, total: int | None = None, start=None):
         """gqa_cache_read from one layer, in the cache's dtype."""
-        return gqa_cache_read(self.k_pages[layer], self.v_pages[layer], self.table, head_dim=self.head_dim,
-                              dtype=self.dtype, cu=cu, total=total, start=start, slots=slots, **self._layer(layer))
+        k_pages, v_pages, table, _, more = self._layer[layer]
+        return gqa_cache_read(k_pages, v_pages, table, head_dim=self.head_dim, dtype=self.dtype, cu=cu, total=total,
+                              start=start, slots=slots, **more)
 
     def decode(self, layer: int, q, slots=None, *, scale: float | None = None, return_lse: bool = False, out=None):
         """gqa_decode over one layer."""
-        return gqa_decode(q, self.k_pages[layer], self.v_pages[layer], self.table, self.lens[layer], slots=slots,
-                          scale=scale, return_lse=return_lse, out=out, **self._layer(layer))
+        k_pages, v_pages, table, lens, more = self._layer[layer]
+        return gqa_decode(q, k_pages, v_pages, table, lens, slots=slots, scale=scale, return_lse=return_lse, out=out,
+                          **more)
