@@ -114,20 +114,12 @@ __device__ __forceinline__ long long gqa_quotient(long long a, long long b) {
 
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(int8_t x) { return (float)x; }
-__device__ __forceinline__ float to_f(__nv_fp8_e4m3 x) { return (float)x; }
 template <class T>
 __device__ __forceinline__ T from_f(float x);
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <>
 __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
-// A non-finite quotient (of a non-finite value) stores 0: its scale is not
-// finite either, so the position reads back as NaN.
-template <>
-__device__ __forceinline__ int8_t from_f<int8_t>(float x) { return isfinite(x) ? (int8_t)__float2int_rn(x) : (int8_t)0; }
-template <>
-__device__ __forceinline__ __nv_fp8_e4m3 from_f<__nv_fp8_e4m3>(float x) { return __nv_fp8_e4m3(x); }
 #endif
 
 }  // namespace wb

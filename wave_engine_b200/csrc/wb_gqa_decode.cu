@@ -225,12 +225,6 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
             s_slot[b] = slot;
         }
         sum += (long long)((n + GD_UNIT - 1) / GD_UNIT) << 24 | (n > 0);
-        if (n == 0 && b % (int)gridDim.x == (int)blockIdx.x) {
-            T *op = (T *)a.out + (long long)b * a.H * c.hd;
-            for (int i = 0; i < a.H * c.hd; i++) op[i] = from_f<T>(0.0f);
-            if (a.lse)
-                for (int h = 0; h < a.H; h++) a.lse[(long long)b * a.H + h] = -INFINITY;
-        }
     }
     // exclusive sum over the threads, and the total
     auto scan = [&](long long x, long long *all) {
@@ -253,6 +247,18 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
     };
     long long total;
     const long long sums = scan(sum, &total);
+    auto length = [&](int b, int *slot) {
+        if (b >= GD_SEQS) return gd_len(c, b, slot);
+        *slot = s_slot[b];
+        return s_len[b];
+    };
+    for (int b = blockIdx.x; b < c.n_seq; b += gridDim.x) {  // sequences without positions
+        int slot;
+        if (length(b, &slot)) continue;
+        T *op = (T *)a.out + (long long)b * a.H * c.hd;
+        for (int i = tid; i < a.H * c.hd; i += GD_THREADS) op[i] = from_f<T>(0.0f);
+        for (int h = tid; a.lse && h < a.H; h += GD_THREADS) a.lse[(long long)b * a.H + h] = -INFINITY;
+    }
     const long long units = (total >> 24) * ips, items = (total & 0xffffff) * ips;
     // Few units for the CTAs there are: every item in equal pieces of P
     // units, one for each CTA (a piece that ends with its item has one join
@@ -266,11 +272,6 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
         P = max(GD_PIECE, (int)((units + (gridDim.x - items) - 1) / (gridDim.x - items)));
     }
     auto item_len = [&](int n) { return n == 0 ? 0 : ((n + GD_UNIT - 1) / GD_UNIT + W + P - 1) / P; };
-    auto length = [&](int b, int *slot) {
-        if (b >= GD_SEQS) return gd_len(c, b, slot);
-        *slot = s_slot[b];
-        return s_len[b];
-    };
 
     long long mine = ((sum >> 24) + W * (sum & 0xffffff)) * ips, before = ((sums >> 24) + W * (sums & 0xffffff)) * ips;
     if (W == 0) {
