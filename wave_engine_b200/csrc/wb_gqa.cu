@@ -828,8 +828,8 @@ static int ga_launch(const GaArgs &ga, int sm_count, cudaStream_t st, std::strin
     } else {  // never loaded from
         tk = tv = tq;
     }
-    static const cudaError_t set =
-        cudaFuncSetAttribute(gqa_attn_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t set = gqa_smem_limit(gqa_attn_kernel<T, HDP>, F::BYTES, done);
     if (set != cudaSuccess) {
         *msg = std::string("attention kernel attributes: ") + cudaGetErrorString(set);
         return WB_ECUDA;

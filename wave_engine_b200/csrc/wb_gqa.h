@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
 #include <string>
 
 namespace wb {
@@ -89,6 +90,17 @@ static void gqa_launch(void (*kernel)(KArgs...), dim3 grid, unsigned block, size
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     cudaLaunchKernelEx(&cfg, kernel, args...);  // an error stays for the caller's check
+}
+// A kernel's shared memory limit, once per device (`done`: a bit each).
+template <typename K>
+static cudaError_t gqa_smem_limit(K *kernel, int bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (e != cudaSuccess || (done.load(std::memory_order_relaxed) & bit)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 __device__ __forceinline__ void gqa_wait() {
     ptx::griddep_wait();

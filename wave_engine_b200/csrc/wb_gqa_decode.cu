@@ -853,8 +853,8 @@ size_t gqa_decode_scratch(const GqaCacheArgs &c, int H, int sm_count) {
 template <class T, int KIND, int HDP, int NB, bool FULL>
 static int gd_launch_as(const GqaDecodeArgs &a, int sm_count, cudaStream_t st, std::string *msg) {
     using F = GdConf<KIND, HDP, NB>;
-    static const cudaError_t set =
-        cudaFuncSetAttribute(gqa_decode_kernel<T, KIND, HDP, NB, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::BYTES);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t set = gqa_smem_limit(gqa_decode_kernel<T, KIND, HDP, NB, FULL>, F::BYTES, done);
     if (set != cudaSuccess) {
         *msg = std::string("decode kernel attributes: ") + cudaGetErrorString(set);
         return WB_ECUDA;
