@@ -444,7 +444,9 @@ WB_API int wb_lm_head(wb_context *ctx, const float *hidden, int n_rows, int n_em
  * full before anything is queued and refused while the stream is captured, or
  * device memory, which the host does not read (no synchronisation; can be
  * captured in a CUDA graph): the kernels then skip what lies outside the
- * buffers and set bit 0x8 (bounds) of the device error word. */
+ * buffers and set bit 0x8 (bounds) of the device error word.  Scratch is the
+ * context's, one per stream: graphs captured on the same stream share it and
+ * must not run at the same time, nor beside calls on that stream. */
 /* element types */
 #define WB_BF16 0
 #define WB_F16 1
