@@ -369,6 +369,13 @@ def test_decode_graph_and_step():
     assert cache.lens[0].tolist() == [T, T]
 
 
+@pytest.mark.parametrize("n", [256, 257, 700])
+@pytest.mark.parametrize("store", STORES)
+def test_many_sequences(n, store):
+    """More sequences than a block holds the lengths of, a third of them empty."""
+    _decode(store, "bfloat16", 4, 2, 64, [(i * 37) % 150 if i % 3 else 0 for i in range(n)])
+
+
 def test_host_index_arrays_are_refused_during_a_capture():
     """A graph would read them after they are gone; the capture itself goes on."""
     import torch
