@@ -1,0 +1,82 @@
+"""Edges of the grouped-head attention and its cache: infinities in visible
+values, values and scores at the ends of the range, index arrays that do not
+fit their rows, scratch under memory pressure and under graph captures."""
+from __future__ import annotations
+
+import pytest
+
+from tests import gqa_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _ints(*values):
+    import torch
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _rows(seed, dtype, T, Hkv, hd):
+    import torch
+    g = torch.Generator("cuda").manual_seed(seed)
+    return tuple(torch.randn(T, Hkv, hd, generator=g, device="cuda").to(dtype) for _ in range(2))
+
+
+def _cache(k, v, lens, store="native"):
+    """Slots 0.. of one layer that hold the packed rows."""
+    import wave_engine_b200 as wb
+    c = wb.GqaCache(1, k.shape[1], k.shape[2], len(lens), max(lens), sum(-(-n // 128) for n in lens), dtype=k.dtype, store=store)
+    for i, n in enumerate(lens):
+        c.reserve(i, n)
+    c.write(0, k, v, list(range(len(lens))), ref.starts(lens))
+    return c
+
+
+def _held(x, store):
+    """What the cache's rows stand for, in 64 bits."""
+    import torch
+    if store == "native":
+        return x.double()
+    q, s = ref.quantise(x, {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}[store])
+    return q.double() * s.double()[..., None]
+
+
+def _check_decode(c, q, k, v, lens, store, scale):
+    """The cache's decode against 64 bits."""
+    import torch
+    import wave_engine_b200 as wb
+    out, lse = c.decode(0, q, return_lse=True, scale=scale)
+    vv = _held(v, store)
+    o, m, z = ref.attention(q, _held(k, store), vv, list(range(len(lens) + 1)), ref.starts(lens), True, scale)
+    pair = store == "native" and q.dtype == torch.bfloat16
+    ref.check(out, lse.T, o, m, z, 2.0 ** -16 if pair else 2.0 ** -11, 0.0 if pair else ref.floor(max(lens), vv))
+    assert wb.default_context(0).take_device_error() == 0
+    return out, lse
+
+
+@pytest.mark.parametrize("op", ["prompt", "decode"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("H,Hkv,hd", [(4, 2, 64), (24, 2, 128), (3, 1, 42)])
+def test_visible_infinities_in_values(op, dtype, H, Hkv, hd):
+    """An infinity or NaN among the values of visible keys reaches its column as in 64 bits (opposite infinities are
+    NaN), whatever the weights round to, and no other column."""
+    import torch
+    import wave_engine_b200 as wb
+    dtype = getattr(torch, dtype)
+    lens = [300, 2000, 1, 40]
+    cu = ref.starts(lens)
+    k, v = _rows(1, dtype, cu[-1], Hkv, hd)
+    q = _rows(2, dtype, len(lens), H, hd)[0] * 0.25
+    bad = v.clone()
+    for key, col, x in ((5, 0, "inf"), (17, 3, "-inf"), (130, 4, "nan"), (255, 9, "inf"), (299, 9, "-inf"), (299, 10, "inf"),
+                        (300 + 64, 1, "inf"), (300 + 65, 2, "-inf"), (300 + 1999, 20, "inf"), (2300, 7, "-inf"),
+                        (2301 + 39, 8, "inf"), (2301, 8, "inf")):
+        bad[key, 0, col] = float(x)
+    if op == "decode":
+        clean, got = (_cache(k, x, lens).decode(0, q) for x in (v, bad))
+    else:
+        starts = _ints(*range(len(lens) + 1)), _ints(*cu)
+        clean, got = (wb.gqa_attention(q, k, x, *starts) for x in (v, bad))
+    want = ref.attention(q, k, bad, list(range(len(lens) + 1)), cu, True, hd ** -0.5)[0]
+    hit = ~torch.isfinite(want)
+    assert hit.sum() == 10 * (H // Hkv) and torch.equal(got[~hit], clean[~hit])
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[hit].double().nan_to_num(7.0), want[hit].nan_to_num(7.0))

@@ -46,7 +46,8 @@
 // values survive the rounding of w to fp16 (kept as 2^8 w: weights down to
 // 2^-32 of the largest count).  With bf16 values p is the sum of two bf16 numbers, each
 // with its own product: the tensor pipe has the room, and 8 bits of p would
-// cost as much precision as the output's own rounding.
+// cost as much precision as the output's own rounding.  The second one, what
+// the first leaves, may be 0 or negative: it meets finite values alone.
 #include "wb_gqa.h"
 
 #include <algorithm>
@@ -141,6 +142,13 @@ __device__ __forceinline__ uint32_t to_f16x2(uint32_t x) {
         const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&m), __half2half2(__ushort_as_half(0x6480)));
         r = *reinterpret_cast<const uint32_t *>(&v);
     }
+    return r;
+}
+
+// two bf16 magnitudes each: the larger ones, NaN if one is (signs as they come)
+__device__ __forceinline__ uint32_t bf16_top(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 
@@ -616,13 +624,10 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                     pf[nb][g] = transposed(pf[nb][g]);
                 }
             }
-            auto product = [&](int j, uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
+            auto product = [&](int j, const uint32_t (&p)[NB][2], uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
                 const uint32_t vf[4] = {v0, v1, v2, v3};
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++) {
-                    mma16816<BF>(acc[nb][j], vf, pf[nb][0], pf[nb][1]);
-                    if (BF) mma16816<BF>(acc[nb][j], vf, pl[nb][0], pl[nb][1]);
-                }
+                for (int nb = 0; nb < NB; nb++) mma16816<BF>(acc[nb][j], vf, p[nb][0], p[nb][1]);
             };
 
             // values: piece r of rows 2cc, 2cc+1, 2cc+8, 2cc+9
@@ -636,10 +641,44 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                         const uint4 v = *reinterpret_cast<const uint4 *>(sv + ((e & 1) + 8 * (e >> 1)) * F::RB + x * 128);
                         w[e][0] = v.x; w[e][1] = v.y; w[e][2] = v.z; w[e][3] = v.w;
                     }
-#pragma unroll
-                    for (int d = 0; d < 4; d++)
-                        product(4 * x + d, __byte_perm(w[0][d], w[1][d], 0x5410), __byte_perm(w[0][d], w[1][d], 0x7632),
+                    auto dims = [&](int d, const uint32_t (&p)[NB][2]) {
+                        product(4 * x + d, p, __byte_perm(w[0][d], w[1][d], 0x5410), __byte_perm(w[0][d], w[1][d], 0x7632),
                                 __byte_perm(w[2][d], w[3][d], 0x5410), __byte_perm(w[2][d], w[3][d], 0x7632));
+                    };
+                    if constexpr (!BF) {
+#pragma unroll
+                        for (int d = 0; d < 4; d++) dims(d, pf);
+                    } else {
+                        // The second part of p may be 0 or negative, which would
+                        // turn an infinite value into a NaN: it gets the values
+                        // without what is not finite.
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+#pragma unroll
+                            for (int d = 0; d < 4; d++) top = bf16_top(top, w[e][d]);
+                        const bool bad = (top & 0x7f80u) == 0x7f80u || (top & 0x7f800000u) == 0x7f800000u;
+                        if (!__any_sync(0xffffffffu, bad)) {
+#pragma unroll
+                            for (int d = 0; d < 4; d++) {
+                                dims(d, pf);
+                                dims(d, pl);
+                            }
+                        } else {
+#pragma unroll
+                            for (int d = 0; d < 4; d++) dims(d, pf);
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+#pragma unroll
+                                for (int d = 0; d < 4; d++) {
+                                    uint32_t &y = w[e][d];
+                                    if ((y & 0x7f80u) == 0x7f80u) y &= 0xffff0000u;
+                                    if ((y & 0x7f800000u) == 0x7f800000u) y &= 0xffffu;
+                                }
+#pragma unroll
+                            for (int d = 0; d < 4; d++) dims(d, pl);
+                        }
+                    }
                 }
             } else {
                 uint32_t w[4][HDP / 32];
@@ -658,8 +697,8 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                     // (key a byte, key b byte) pairs of dims 4d, 4d+1 and 4d+2, 4d+3
                     const uint32_t a01 = __byte_perm(w[0][d], w[1][d], 0x5140), a23 = __byte_perm(w[0][d], w[1][d], 0x7362);
                     const uint32_t b01 = __byte_perm(w[2][d], w[3][d], 0x5140), b23 = __byte_perm(w[2][d], w[3][d], 0x7362);
-                    product(2 * d, to_f16x2<KIND, 0>(a01), to_f16x2<KIND, 1>(a01), to_f16x2<KIND, 0>(b01), to_f16x2<KIND, 1>(b01));
-                    product(2 * d + 1, to_f16x2<KIND, 0>(a23), to_f16x2<KIND, 1>(a23), to_f16x2<KIND, 0>(b23), to_f16x2<KIND, 1>(b23));
+                    product(2 * d, pf, to_f16x2<KIND, 0>(a01), to_f16x2<KIND, 1>(a01), to_f16x2<KIND, 0>(b01), to_f16x2<KIND, 1>(b01));
+                    product(2 * d + 1, pf, to_f16x2<KIND, 0>(a23), to_f16x2<KIND, 1>(a23), to_f16x2<KIND, 0>(b23), to_f16x2<KIND, 1>(b23));
                 }
             }
         };
