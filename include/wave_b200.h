@@ -503,7 +503,10 @@ typedef struct {
  * (strides as above) become positions start[i], start[i] + 1, ... of slot
  * slots[i], and lens[slots[i]] the position after the last.  cu NULL: one
  * row per sequence; start NULL: append (start = lens); slots NULL: 0, 1, ...
- * total: rows of k and v (cu's last entry).  A slot may appear once. */
+ * total: rows of k and v (cu's last entry).  A slot may appear once.  Device
+ * arrays: a sequence whose rows do not all lie inside the total is skipped
+ * and flagged, rows of no sequence are skipped and flagged, and a length
+ * changes only when all its positions have a page. */
 WB_API int wb_gqa_cache_write(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq,
                               const int32_t *cu, int64_t total, const int32_t *start, const void *k, int64_t k_ts,
                               int64_t k_hs, const void *v, int64_t v_ts, int64_t v_hs);

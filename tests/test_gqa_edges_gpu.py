@@ -80,3 +80,27 @@ def test_visible_infinities_in_values(op, dtype, H, Hkv, hd):
     hit = ~torch.isfinite(want)
     assert hit.sum() == 10 * (H // Hkv) and torch.equal(got[~hit], clean[~hit])
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[hit].double().nan_to_num(7.0), want[hit].nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("store", ["native", "int8"])
+def test_starts_past_the_rows_are_flagged(store):
+    """Starts on the device that end behind the rows at hand: flagged, no length changes for what was not written."""
+    import torch
+    import wave_engine_b200 as wb
+    ctx = wb.Context(0)
+    c = wb.GqaCache(1, 2, 64, 3, 256, 6, store=store, ctx=ctx)
+    for i in range(3):
+        c.reserve(i, 256)
+    k, v = _rows(11, torch.bfloat16, 5, 2, 64)
+    for slots, cu, start, lens in (((0,), (0, 8), None, [0, 0, 0]), ((0, 1, 2), (0, 3, 5, 9), None, [3, 2, 0]),
+                                   ((0, 1, 2), (0, 5, 200, 300), (7, 0, 0), [12, 2, 0]), ((1,), (0, 9), (4,), [12, 2, 0]),
+                                   ((2,), (0, -3), None, [12, 2, 0]), ((1, 2), (0, 5, 4), (0, 9), [12, 5, 0])):
+        c.write(0, k, v, _ints(*slots), _ints(*cu), None if start is None else _ints(*start))
+        assert ctx.take_device_error() & 0x8, cu
+        assert c.lens[0].tolist() == lens, cu
+    for cu, total in (((0, 8), 5), ((0, 5, 9), 5), ((0, 5, 4), 5)):
+        c.read(0, _ints(*range(len(cu) - 1)), _ints(*cu), total)
+        assert ctx.take_device_error() & 0x8, cu
+    c.read(0, _ints(0, 1), _ints(0, 3, 5), 5)
+    assert ctx.take_device_error() == 0
+    ctx.close()

@@ -52,19 +52,25 @@ __device__ __forceinline__ long long gqa_start(const GqaMove &m, int b, int slot
     return m.start ? m.start[b] : m.append ? m.c.lens[slot] : 0;
 }
 
+// Sequence b's rows lie inside the tensors.
+__device__ __forceinline__ bool gqa_rows_fit(const GqaMove &m, int b) {
+    const int r0 = m.cu[b], r1 = m.cu[b + 1];
+    return r0 >= 0 && r1 >= r0 && r1 <= m.total;
+}
+
 // The row index of packed token t's position (page, head 0), or -1 outside
-// the cache.
+// the cache or when the sequence's rows do not all lie inside the tensors.
 __device__ __forceinline__ long long gqa_place(const GqaMove &m, long long t) {
     const GqaCacheArgs &c = m.c;
     int b = (int)t;
-    long long i = 0, n = 1;
+    long long i = 0, end = t + 1;
     if (m.cu) {
         b = gqa_find_seq(m.cu, c.n_seq, t);
         i = t - m.cu[b];
-        n = (long long)m.cu[b + 1] - m.cu[b];
+        end = m.cu[b + 1];
     }
     const int slot = c.slots ? c.slots[b] : b;
-    if (slot < 0 || slot >= c.n_slots || i < 0 || i >= n) return -1;
+    if (slot < 0 || slot >= c.n_slots || i < 0 || t >= end || end > m.total) return -1;
     const long long s0 = gqa_start(m, b, slot);
     const long long pos = s0 + i;
     if (s0 < 0 || pos >= (long long)c.max_pages * WB_PAGE) return -1;
@@ -73,13 +79,17 @@ __device__ __forceinline__ long long gqa_place(const GqaMove &m, long long t) {
     return (long long)pg * c.Hkv * WB_PAGE + (pos & (WB_PAGE - 1));
 }
 
-// lens[slot] = the position after sequence b's last token, when all its
-// positions have a page.
+// lens[slot] = the position after sequence b's last token, when its rows are
+// there and all its positions have a page.
 __device__ __forceinline__ void gqa_set_len(const GqaMove &m, int b) {
     const GqaCacheArgs &c = m.c;
+    if (m.cu && !gqa_rows_fit(m, b)) {
+        atomicOr(c.dev_err, WB_DERR_BOUNDS);  // no row of it may have been looked at
+        return;
+    }
     const long long n = m.cu ? (long long)m.cu[b + 1] - m.cu[b] : 1;
     const int slot = c.slots ? c.slots[b] : b;
-    if (slot < 0 || slot >= c.n_slots || n < 0) return;
+    if (slot < 0 || slot >= c.n_slots) return;
     const long long s0 = gqa_start(m, b, slot), end = s0 + n;
     if (s0 < 0 || end > (long long)c.max_pages * WB_PAGE) return;
     for (long long p = s0 >> WB_PAGE_SHIFT; p << WB_PAGE_SHIFT < end; p++) {
@@ -319,6 +329,9 @@ __global__ void __launch_bounds__(GM_THREADS) gqa_read_kernel(GqaMove m) {
         s_place[i] = p;
         if (p < 0) atomicOr(c.dev_err, WB_DERR_BOUNDS);
     }
+    // starts that leave out rows, or sequences that no row belongs to
+    if (m.cu && blockIdx.x + blockIdx.y == 0 && tid == GM_THREADS - 1 && (m.cu[0] != 0 || m.cu[c.n_seq] != m.total))
+        atomicOr(c.dev_err, WB_DERR_BOUNDS);
     __syncthreads();
     const S *pages = (const S *)(v ? c.v_pages : c.k_pages) + d0;
     const float *scales = v ? c.v_scale : c.k_scale;
