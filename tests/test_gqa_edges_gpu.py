@@ -104,3 +104,19 @@ def test_starts_past_the_rows_are_flagged(store):
     c.read(0, _ints(0, 1), _ints(0, 3, 5), 5)
     assert ctx.take_device_error() == 0
     ctx.close()
+
+
+@pytest.mark.parametrize("store", ["int8", "e4m3"])
+@pytest.mark.parametrize("upto", [64, 70, 300])
+def test_decode_value_scales_of_zero(store, upto):
+    """Pages that the caller filled: rows whose value scale is 0 are values of 0, at the start of every warp's keys too."""
+    import torch
+    lens = [300]
+    k, v = _rows(5, torch.bfloat16, 300, 1, 64)
+    q = _rows(6, torch.bfloat16, 1, 4, 64)[0]
+    c = _cache(k, v, lens, store)
+    for key in range(upto):
+        c.v_scale[0, c.table[0, key // 128], 0, key % 128] = 0.0
+    v = v.clone()
+    v[:upto] = 0
+    _check_decode(c, q, k, v, lens, store, 0.125)

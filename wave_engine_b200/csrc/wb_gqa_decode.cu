@@ -589,7 +589,9 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                             if (!TAIL || r + 8 * g < n) {
                                 const float x = s[nb][2 * g + e] * fac[nb][e];
                                 mx = fmaxf(mx, x);
-                                if (QUANT) mx2 = fmaxf(mx2, x + lg2(vs[g]));
+                                // a scale of 0 (a caller's own pages) counts as 2^-118: m2
+                                // follows m, and 2^(m - m2) stays finite
+                                if (QUANT) mx2 = fmaxf(mx2, x + fmaxf(lg2(vs[g]), -118.0f));
                             }
                         const float mn = fmaxf(m[nb][e], oct_max(mx)), mn2 = QUANT ? fmaxf(m2[nb][e], oct_max(mx2)) : mn;
                         l[nb][e] *= ex2(m[nb][e] - mn);
