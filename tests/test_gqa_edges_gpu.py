@@ -120,3 +120,18 @@ def test_decode_value_scales_of_zero(store, upto):
     v = v.clone()
     v[:upto] = 0
     _check_decode(c, q, k, v, lens, store, 0.125)
+
+
+@pytest.mark.parametrize("store", ["native", "int8", "e4m3"])
+@pytest.mark.parametrize("H,hd", [(2, 64), (12, 128)])
+def test_decode_values_at_the_end_of_the_range(store, H, hd):
+    """bf16 values near the type's largest: the output is between them, also where the scores rise along the keys."""
+    import torch
+    lens = [600, 40, 1]
+    cu = ref.starts(lens)
+    k, v = _rows(3, torch.bfloat16, cu[-1], 1, hd)
+    v = (v.sign() * 1.25 * 2.0 ** 127).to(torch.bfloat16)
+    q = _rows(4, torch.bfloat16, 3, H, hd)[0]
+    q[:, :, 0] = 3.0
+    k[:, 0, 0] = torch.linspace(-12, 12, cu[-1], device="cuda").to(torch.bfloat16)
+    _check_decode(_cache(k, v, lens, store), q, k, v, lens, store, 1.0)

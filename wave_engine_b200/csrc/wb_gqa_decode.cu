@@ -40,10 +40,10 @@
 // Only the 16 x 8 probabilities change sides (movmatrix).
 // 8-bit values become fp16 exactly (e4m3 by cvt, int8 by exponent insertion
 // and a subtraction); the K scale multiplies the finished score.  The V
-// scale joins the weight, w_j = p_j vscale_j 2^(m - m2), where m2 is a running
+// scale joins the weight, w_j = p_j vscale_j 2^(8 - d2), where d2 is a running
 // maximum of its own, of log2 (p_j vscale_j): w_j is then relative to the
 // largest weight times scale, so keys with a large probability and small
-// values survive the rounding of w to fp16 (kept as 2^8 w: weights down to
+// values survive the rounding of w to fp16 (as 2^8 w: weights down to
 // 2^-32 of the largest count).  With bf16 values p is the sum of two bf16 numbers, each
 // with its own product: the tensor pipe has the room, and 8 bits of p would
 // cost as much precision as the output's own rounding.  The second one, what
@@ -74,9 +74,19 @@ static constexpr int GD_FEW = 8;        // units per CTA below which items are c
 static constexpr int GD_PIECE = 6;      // .. of this many units at least
 static constexpr int GD_JOIN = 12;      // pieces that a join loads at a time
 static constexpr int GD_SEQS = 256;     // sequences whose lengths a CTA holds in shared memory
-static constexpr float GD_SHIFT = 8.0f; // weights are kept as 2^8 exp2(s - m): see above
 
 enum { GD_NATIVE = 0, GD_INT8 = 1, GD_E4M3 = 2 };
+
+// A key at the running maximum has p = 2^gd_shift, and the maximum is
+// followed when p is 2^6 beyond that.  fp16 weights: 2^8, so that 2^-32 of the
+// largest still counts.  bf16, which has fp32's range: 2^-26, so that up to
+// 2^20 products with the type's largest value add up in fp32 (the definition's
+// result is between the values, whatever their size).  8-bit values: 1, as p
+// meets their scale before the factor 2^(8 - d2).
+__host__ __device__ constexpr float gd_shift(bool quant, bool bf) { return quant ? 0.0f : bf ? -26.0f : 8.0f; }
+static constexpr float GD_WEIGHT = 8.0f;    // 8-bit values: the largest weight is 2^8
+static constexpr float GD_SMALL = -118.0f;  // least d2: 2^(8 - d2) stays finite
+static constexpr float GD_NONE = 3.402823466e38f;  // off before the first key: any finite score replaces it
 
 // CTAs per SM and ring depth: what registers (HDP / 4 NB output and HDP / 8
 // NB query registers a thread) and shared memory leave.
@@ -205,6 +215,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
     using F = GdConf<KIND, HDP, NB>;
     constexpr bool BF = KIND == GD_NATIVE && __is_same(T, __nv_bfloat16);  // product type
     constexpr bool QUANT = KIND != GD_NATIVE;
+    constexpr float SHIFT = gd_shift(QUANT, BF);
     constexpr int NK = HDP / 16;  // products of 16 keys and 8 heads over the dims ..
     constexpr int NV = HDP / 16;  // .. and over the keys
     constexpr int ROWS = F::ROWS;
@@ -215,7 +226,8 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
     __shared__ GdSeg s_seg[3];
     __shared__ int s_seq;
     __shared__ int s_len[GD_SEQS], s_slot[GD_SEQS];
-    __shared__ float s_m[GD_WARPS][16], s_l[GD_WARPS][16], s_m2[GD_WARPS][16], s_f[GD_WARPS][16], s_row[16];
+    __shared__ float s_off[GD_WARPS][16], s_l[GD_WARPS][16], s_f[GD_WARPS][16], s_row[16];
+    [[maybe_unused]] __shared__ float s_g[GD_WARPS][16];  // 8-bit values: 2^(d2 - 8)
     __shared__ int s_last, s_stage[GD_WARPS];
     const GqaCacheArgs &c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, cc = lane & 3;
@@ -499,16 +511,16 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
 
         // acc[nb][j]: dims of piece r (two per product), heads 2cc, 2cc+1
         float acc[NB][NV][4] = {};
-        // finite stand-ins for -inf: the first visible score replaces them
-        float m[NB][2], m2[NB][2], l[NB][2], off[NB][2], e2[NB][2];  // off = 8 - m, e2 = 2^(m - m2)
+        // p = 2^(score + off), off = SHIFT - maximum; d2, e2 = 2^(8 - d2): 8-bit values
+        float l[NB][2], off[NB][2], d2[NB][2], e2[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                m[nb][e] = m2[nb][e] = -1e30f;
                 l[nb][e] = 0.0f;
-                off[nb][e] = 1e30f;
-                e2[nb][e] = 1.0f;
+                off[nb][e] = GD_NONE;
+                d2[nb][e] = GD_SMALL;
+                e2[nb][e] = ex2(GD_WEIGHT - GD_SMALL);
             }
         bool unmapped = false;
 
@@ -571,35 +583,36 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                         most += pr[nb][2 * g] + pr[nb][2 * g + 1];
                     }
                 }
-                // a weight above 2^14 (fp16), or sums that could leave fp32's range
-                bool far = most > 1.8e19f;
+                // p 2^6 beyond its place, or an fp16 weight above 2^14
+                bool far = BF ? most > 9.5367431640625e-7f : QUANT && most > 64.0f;
                 if (!BF) far |= __hgt2_mask(top, __half2half2(__ushort_as_half(0x7400))) != 0;
                 return far;
             };
-            // The references m, m2 stay until then; then they follow the maxima.
+            // The references off, d2 stay until then; then they follow the maxima.
             if (__any_sync(0xffffffffu, weigh())) {
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++) {
                     float f2[2];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float mx = -INFINITY, mx2 = -INFINITY;
+                        float mx = -INFINITY, mx2 = GD_SMALL;
 #pragma unroll
                         for (int g = 0; g < 2; g++)
-                            if (!TAIL || r + 8 * g < n) {
-                                const float x = s[nb][2 * g + e] * fac[nb][e];
-                                mx = fmaxf(mx, x);
-                                // a scale of 0 (a caller's own pages) counts as 2^-118: m2
-                                // follows m, and 2^(m - m2) stays finite
-                                if (QUANT) mx2 = fmaxf(mx2, x + fmaxf(lg2(vs[g]), -118.0f));
-                            }
-                        const float mn = fmaxf(m[nb][e], oct_max(mx)), mn2 = QUANT ? fmaxf(m2[nb][e], oct_max(mx2)) : mn;
-                        l[nb][e] *= ex2(m[nb][e] - mn);
-                        f2[e] = ex2(m2[nb][e] - mn2);
-                        m[nb][e] = mn;
-                        m2[nb][e] = mn2;
-                        off[nb][e] = GD_SHIFT - mn;
-                        if (QUANT) e2[nb][e] = ex2(mn - mn2);
+                            if (!TAIL || r + 8 * g < n) mx = fmaxf(mx, s[nb][2 * g + e] * fac[nb][e]);
+                        const float to = fminf(off[nb][e], SHIFT - oct_max(mx)), d = to - off[nb][e];
+                        l[nb][e] *= ex2(d);
+                        off[nb][e] = to;
+                        f2[e] = ex2(d);
+                        if (QUANT) {
+                            // a scale of 0 (a caller's own pages) counts as 2^-118
+#pragma unroll
+                            for (int g = 0; g < 2; g++)
+                                if (!TAIL || r + 8 * g < n) mx2 = fmaxf(mx2, fmaf(s[nb][2 * g + e], fac[nb][e], to) + lg2(vs[g]));
+                            const float to2 = fmaxf(d2[nb][e] + d, oct_max(mx2));
+                            f2[e] = ex2(d + d2[nb][e] - to2);
+                            d2[nb][e] = to2;
+                            e2[nb][e] = ex2(GD_WEIGHT - to2);
+                        }
                     }
 #pragma unroll
                     for (int j = 0; j < NV; j++) {
@@ -753,9 +766,9 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
             for (int e = 0; e < 2; e++) {
                 l[nb][e] = oct_sum(l[nb][e]);
                 if (r == 0) {
-                    s_m[warp][8 * nb + 2 * cc + e] = m[nb][e];
+                    s_off[warp][8 * nb + 2 * cc + e] = off[nb][e];
                     s_l[warp][8 * nb + 2 * cc + e] = l[nb][e];
-                    s_m2[warp][8 * nb + 2 * cc + e] = QUANT ? m2[nb][e] : m[nb][e];
+                    if (QUANT) s_g[warp][8 * nb + 2 * cc + e] = ex2(d2[nb][e] - GD_WEIGHT);
                 }
             }
         if (lane == 0) s_stage[warp] = stage;
@@ -782,15 +795,12 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
         __syncthreads();
         if (tid == GD_THREADS - 1) next_seg(s_seg[(part + 2) % 3]);
         if (tid < ROWS) {
-            float M = -1e30f, M2 = -1e30f, L = 0.0f;
-            for (int w = 0; w < GD_WARPS; w++) {
-                M = fmaxf(M, s_m[w][tid]);
-                M2 = fmaxf(M2, s_m2[w][tid]);
-            }
-            for (int w = 0; w < GD_WARPS; w++) L += s_l[w][tid] * ex2(s_m[w][tid] - M);
-            const float inv = L == 0.0f ? 0.0f : ex2(M2 - M) / L;
-            for (int w = 0; w < GD_WARPS; w++) s_f[w][tid] = ex2(s_m2[w][tid] - M2) * inv;
-            s_row[tid] = L == 0.0f ? -INFINITY : M - GD_SHIFT + log2f(L);  // log2 sum exp
+            float to = GD_NONE, L = 0.0f;
+            for (int w = 0; w < GD_WARPS; w++) to = fminf(to, s_off[w][tid]);
+            for (int w = 0; w < GD_WARPS; w++) L += s_l[w][tid] * ex2(to - s_off[w][tid]);
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            for (int w = 0; w < GD_WARPS; w++) s_f[w][tid] = ex2(to - s_off[w][tid]) * inv;
+            s_row[tid] = L == 0.0f ? -INFINITY : log2f(L) - to;  // log2 sum exp
         }
         __syncthreads();
         const bool whole = g.ua == 0 && g.ub == g.U;
@@ -808,11 +818,11 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
 #pragma unroll
             for (int w = 0; w < GD_WARPS; w++) {
                 const float4 v = *reinterpret_cast<const float4 *>(row_at(w, s_stage[w], row) + d);
-                const float f = s_f[w][row];
-                o[0] += v.x * f;
-                o[1] += v.y * f;
-                o[2] += v.z * f;
-                o[3] += v.w * f;
+                const float f = s_f[w][row], g8 = QUANT ? s_g[w][row] : 1.0f;
+                o[0] += v.x * f * g8;
+                o[1] += v.y * f * g8;
+                o[2] += v.z * f * g8;
+                o[3] += v.w * f * g8;
             }
             if (whole) put(row, d, o);
             else __stcg(reinterpret_cast<float4 *>(piece + 16 + 4 * i), make_float4(o[0], o[1], o[2], o[3]));
