@@ -135,3 +135,17 @@ def test_decode_values_at_the_end_of_the_range(store, H, hd):
     q[:, :, 0] = 3.0
     k[:, 0, 0] = torch.linspace(-12, 12, cu[-1], device="cuda").to(torch.bfloat16)
     _check_decode(_cache(k, v, lens, store), q, k, v, lens, store, 1.0)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_values_at_the_end_of_the_range(hd):
+    import torch
+    import wave_engine_b200 as wb
+    T = 700
+    k, v = _rows(3, torch.bfloat16, T, 1, hd)
+    v = (v.sign() * 1.25 * 2.0 ** 127).to(torch.bfloat16)
+    q = _rows(4, torch.bfloat16, T, 2, hd)[0]
+    q[:, :, 0] = 3.0
+    k[:, 0, 0] = torch.linspace(-6, 6, T, device="cuda").to(torch.bfloat16)
+    out, lse = wb.gqa_attention(q, k, v, [0, T], return_lse=True)
+    ref.check(out, lse, *ref.attention(q, k, v, [0, T], [0, T], True, hd ** -0.5))

@@ -555,7 +555,10 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::R_SOFTMAX));
         // ---- softmax of tile t: thread = row
-        constexpr float SHIFT = BF ? 0.0f : 5.0f;  // fp16 probabilities: 2^5 times, up to 2^13, down to 2^-29
+        // fp16 probabilities: 2^5 times, up to 2^13, down to 2^-29.  bf16, which
+        // has fp32's range: 2^-28 times, so that up to 2^20 products with the
+        // type's largest value add up in fp32.
+        constexpr float SHIFT = BF ? -28.0f : 5.0f;
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(row & 96) << 16;
         const uint32_t S = tmem + t * 128 + lanes, O = tmem + F::O_COL + t * HDP + lanes;
