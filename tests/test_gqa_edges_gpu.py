@@ -149,3 +149,46 @@ def test_prompt_values_at_the_end_of_the_range(hd):
     k[:, 0, 0] = torch.linspace(-6, 6, T, device="cuda").to(torch.bfloat16)
     out, lse = wb.gqa_attention(q, k, v, [0, T], return_lse=True)
     ref.check(out, lse, *ref.attention(q, k, v, [0, T], [0, T], True, hd ** -0.5))
+
+
+@pytest.mark.parametrize("store", ["native", "int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("H,Hkv,hd", [(8, 1, 64), (24, 2, 128), (2, 1, 64), (2, 2, 64), (3, 1, 42)])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+def test_decode_queries_do_not_reach_each_other(store, dtype, H, Hkv, hd, bad):
+    """A query that is not finite leaves every other head right, whose scores rise along the keys, and so do keys with
+    infinities: products in no head's place are NaN there."""
+    import torch
+    dtype = getattr(torch, dtype)
+    lens = [300, 5000, 1, 40]
+    k, v = _rows(20, dtype, sum(lens), Hkv, hd)
+    q = _rows(21, dtype, len(lens), H, hd)[0]
+    k[:, :, 1] = torch.linspace(-4, 4, len(k), device="cuda")[:, None]  # scores that rise by 2^200 and more
+    q[:, :, 1] = 200.0
+    c = _cache(k, v, lens, store)
+    clean, clean_lse = _check_decode(c, q, k, v, lens, store, hd ** -0.5)
+    hit = torch.zeros(len(lens), H, dtype=torch.bool, device="cuda")
+    q2 = q.clone()
+    for i, h in ((0, 1), (1, H - 1), (2, 0), (3, 1)):
+        q2[i, h, 0] = float(bad)
+        hit[i, h] = True
+    got, lse = c.decode(0, q2, return_lse=True)
+    assert got[hit].isnan().all() or bad == "inf"
+    got[hit], lse[hit] = clean[hit], clean_lse[hit]
+    vv = _held(v, store)
+    o, m, z = ref.attention(q, _held(k, store), vv, list(range(len(lens) + 1)), ref.starts(lens), True, hd ** -0.5)
+    u_p, floor = (2.0 ** -16, 0.0) if store == "native" and dtype == torch.bfloat16 else (2.0 ** -11, ref.floor(max(lens), vv))
+    ref.check(got, lse.T, o, m, z, u_p, floor)
+    if store == "native":  # -infinity for the scores of the first half of the keys
+        first = 0
+        half = [n // 32 * 16 + 8 if n > 32 else 0 for n in lens]
+        for n, x in zip(lens, half):
+            k[first:first + x, :, 0] = -float("inf")
+            first += n
+        q[:, :, 0] = 1.0
+        c = _cache(k, v, lens)
+        out, lse = c.decode(0, q, return_lse=True)
+        rest = [n - x for n, x in zip(lens, half)]
+        keep = torch.isfinite(k[:, 0, 0])
+        o, m, z = ref.attention(q, k[keep], v[keep], list(range(len(lens) + 1)), ref.starts(rest), True, hd ** -0.5)
+        ref.check(out, lse.T, o, m, z, u_p, floor)

@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                         }
                         pf[nb][g] = pack2(w[0], w[1], BF);
                         if (!BF) top = __hmax2(top, *reinterpret_cast<const __half2 *>(&pf[nb][g]));
-                        most += pr[nb][2 * g] + pr[nb][2 * g + 1];
+                        most = fmaxf(most, fmaxf(pr[nb][2 * g], pr[nb][2 * g + 1]));  // a NaN hides no other head's
                     }
                 }
                 // p 2^6 beyond its place, or an fp16 weight above 2^14
