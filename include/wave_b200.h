@@ -460,7 +460,8 @@ WB_API int wb_lm_head(wb_context *ctx, const float *hidden, int n_rows, int n_em
  *   of n_q sees keys j <= i + (n_k - n_q), so queries that continue a cached
  *   prefix are given with all keys of the sequence.
  *   lse = log sum exp of the visible scaled scores.
- * A query that sees no key gives out 0 and lse -inf.  Values of keys that a
+ * A query that sees no key, or only scores of -infinity, gives out 0 and lse
+ * -inf; one that sees a score of +infinity or NaN gives NaN for both.  Values of keys that a
  * query does not see never reach it, not even as infinities or NaN.
  * Scores, softmax statistics and the output sums are fp32; the
  * unnormalised probabilities are rounded to dtype for the product with v. */
@@ -519,8 +520,8 @@ WB_API int wb_gqa_cache_read(wb_context *ctx, const wb_gqa_cache_desc *c, const 
 /* Attention of one new token per sequence over positions 0 .. lens-1 of its
  * slot (the token's own key and value among them: write it first).  q
  * element (sequence, head, d) at sequence*q_ss + head*q_hs + d; out [n_seq]
- * [n_head][head_dim] contiguous, lse NULL or [n_seq][n_head].  An empty slot
- * gives 0 and -inf; positions before the length whose page is unmapped are
+ * [n_head][head_dim] contiguous, lse NULL or [n_seq][n_head].  An empty slot,
+ * or scores of -infinity alone, gives 0 and -inf; positions before the length whose page is unmapped are
  * left out and flagged. */
 WB_API int wb_gqa_decode(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq, int n_head,
                          const void *q, int64_t q_ss, int64_t q_hs, float scale, void *out, float *lse);

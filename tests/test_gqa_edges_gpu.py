@@ -192,3 +192,32 @@ def test_decode_queries_do_not_reach_each_other(store, dtype, H, Hkv, hd, bad):
         keep = torch.isfinite(k[:, 0, 0])
         o, m, z = ref.attention(q, k[keep], v[keep], list(range(len(lens) + 1)), ref.starts(rest), True, hd ** -0.5)
         ref.check(out, lse.T, o, m, z, u_p, floor)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("H,Hkv,hd", [(2, 2, 64), (8, 1, 128), (3, 1, 42)])
+def test_scores_of_minus_infinity(dtype, H, Hkv, hd):
+    """A query whose visible scores are all -infinity has no weight anywhere: 0 and -inf from the prompt attention and
+    from the decode; keys with such scores count for nothing beside others."""
+    import torch
+    import wave_engine_b200 as wb
+    dtype = getattr(torch, dtype)
+    n, T = 200, 420
+    k, v = _rows(7, dtype, T, Hkv, hd)
+    q = _rows(8, dtype, T, H, hd)[0]
+    q[:, :, 0] = 1.0
+    k[:, :, 0] = 0.0
+    hidden = k.clone()
+    hidden[:n, :, 0] = -float("inf")
+    out, lse = wb.gqa_attention(q, hidden, v, [0, T], return_lse=True)
+    assert not out[:n].any() and (lse[:, :n] == -float("inf")).all()
+    o, m, z = ref.attention(q[n:], k[n:], v[n:], [0, T - n], [0, T - n], True, hd ** -0.5)
+    ref.check(out[n:], lse[:, n:], o, m, z, floor=ref.floor(T, v, 5) if dtype == torch.float16 else 0.0)
+    c = _cache(hidden, v, [T])
+    for held in (1, n, T):
+        c.lens[0, 0] = held
+        out, lse = c.decode(0, q[-1:], return_lse=True)
+        if held <= n:
+            assert not out.any() and (lse == -float("inf")).all()
+        else:
+            ref.check(out, lse.T, o[-1:], m[-1:], (z[0][:, -1:], z[1][:, -1:]), 2.0 ** -11, ref.floor(T, v))

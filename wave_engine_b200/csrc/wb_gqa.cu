@@ -3,7 +3,8 @@
 //   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij) / sum_j exp(s_ij),
 //   s_ij = scale q_i . k_j  over the keys j <= i + (n_k - n_q) of the
 //   query's own sequence (all of them when not causal);
-//   lse_i = log sum_j exp(s_ij); a query without keys gives 0 and -inf.
+//   lse_i = log sum_j exp(s_ij); a query without keys, or whose scores are all
+//   -infinity, gives 0 and -inf.
 //
 // One pass over the keys per query tile with the running maximum m and sum
 // l of the softmax: S = Q K^T on tcgen05 into TMEM, P = 2^(c S - m) in
@@ -661,7 +662,8 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
             // ---- epilogue: O / l
             float l0, l1;
             ptx::f2_unpack(ptx::f2_add(l2[0], l2[1]), l0, l1);
-            const float l = l0 + l1, inv = 1.0f / l;
+            // l is 0 where no key is visible or every visible score is -infinity
+            const float l = l0 + l1, inv = l == 0.0f ? 0.0f : 1.0f / l;
             const bool none = vis == 0;
             const int h = hk * G + row_g;
             const long long at = (long long)(q0 + tok) * a.o_ts + (long long)h * a.o_hs;  // the row's place in out
@@ -731,7 +733,7 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
 #pragma unroll 1
                     for (int d = 0; d < a.hd; d++) {
                         const float y = to_f(v[d]);
-                        if (!isfinite(y)) o[d] = from_f<T>(to_f(o[d]) + y);
+                        if (!isfinite(y)) o[d] = from_f<T>(to_f(o[d]) + (l == 0.0f ? l * y : y));
                     }
                 }
             }
