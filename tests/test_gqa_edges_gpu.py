@@ -221,3 +221,46 @@ def test_scores_of_minus_infinity(dtype, H, Hkv, hd):
             assert not out.any() and (lse == -float("inf")).all()
         else:
             ref.check(out, lse.T, o[-1:], m[-1:], (z[0][:, -1:], z[1][:, -1:]), 2.0 ** -11, ref.floor(T, v))
+
+
+def _lowest(dtype, Hkv, hd, H, n, T, big):
+    """Rows whose first n keys have, through dimension 0, the lowest scores that the type can make."""
+    import torch
+    k, v = _rows(9, dtype, T, Hkv, hd)
+    q = _rows(10, dtype, T, H, hd)[0]
+    q[:, :, 0] = big
+    k[:, :, 0] = 0.0
+    low = k.clone()
+    low[:n, :, 0] = torch.finfo(dtype).min
+    return q, k, low, v
+
+
+# scores of 2^128 and 2^38 (bf16), 2^32 (fp16), 2^25 times the scale
+LOWEST = [("bfloat16", 1.0), ("bfloat16", 2.0 ** -90), ("float16", 60000.0), ("bfloat16", 2.0 ** -103)]
+
+
+@pytest.mark.parametrize("dtype,big", LOWEST)
+@pytest.mark.parametrize("H,Hkv,hd", [(2, 2, 64), (8, 1, 128)])
+def test_prompt_lowest_scores(dtype, big, H, Hkv, hd):
+    """Keys whose scores are the lowest numbers there are (masked by a dimension of the type's lowest value) count for
+    nothing beside others; queries that see nothing else still get a mean of values."""
+    import torch
+    import wave_engine_b200 as wb
+    dtype = getattr(torch, dtype)
+    n, T = 300, 700
+    q, k, low, v = _lowest(dtype, Hkv, hd, H, n, T, big)
+    out, lse = wb.gqa_attention(q, low, v, [0, T], return_lse=True)
+    o, m, z = ref.attention(q[n:], k[n:], v[n:], [0, T - n], [0, T - n], True, hd ** -0.5)
+    ref.check(out[n:], lse[:, n:], o, m, z, floor=ref.floor(T, v, 5) if dtype == torch.float16 else 0.0)
+    assert torch.isfinite(out[:n]).all() and out[:n].abs().max() <= v.abs().max()
+    want = ref.attention(q[:n], low[:n], v[:n], [0, n], [0, n], True, hd ** -0.5)[2][0]
+    assert ((lse[:, :n].double() - want) / want).abs().max() < 1e-5
+    # the highest scores: one key takes all, those before it nothing
+    high = k.clone()
+    high[n, :, 0] = torch.finfo(dtype).max
+    out, lse = wb.gqa_attention(q, high, v, [0, T], return_lse=True)
+    o = v[n].double().repeat_interleave(H // Hkv, 0).expand(T - n, H, hd)
+    z = ref.attention(q[n:], high[n:n + 1], v[n:n + 1], [0, T - n], [0, 1], False, hd ** -0.5)[2]
+    assert ((out[n:].double() - o).abs() <= 2.02 * ref.ROUNDOFF[dtype] * o.abs()).all()
+    assert ((lse[:, n:].double() - z[0]) / z[0]).abs().max() < 1e-5
+    assert torch.equal(out[:n], wb.gqa_attention(q, k, v, [0, T])[:n])

@@ -52,6 +52,7 @@ static constexpr int GA_EDGES = 4;  // most key tiles that some row of a CTA see
 struct GaArgs {
     GqaAttnArgs a;
     float c;      // |scale| log2 e, at least 1e-30
+    float c_two;  // the largest power of two that is not above c
     int G, TT;    // heads per key-value head, tokens of a query tile
     int vec;      // out rows take 16-byte stores
     long long items;  // no more than this many (sequence, tiles) items
@@ -564,7 +565,6 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
         const uint32_t lanes = (uint32_t)(row & 96) << 16;
         const uint32_t S = tmem + t * 128 + lanes, O = tmem + F::O_COL + t * HDP + lanes;
         const int row_tok = t * TT + row / G, row_g = row % G;
-        const uint64_t c2 = ptx::f2_pack(ga.c, ga.c);
         uint32_t n_s = 0, n_o = 0;
         bool ok = true;
         for (int k = 0; ok; k++) {
@@ -581,6 +581,17 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
             // cost no masking (2 of 128 rows with 3 heads: 430 cycles a tile)
             const int vis = real ? visible(nq, it->nk, tok) : 0x7fffffff;
             float m = -INFINITY, off = 0.0f;  // reference of the exponents, and what is added to c s
+            // c s + off in one operation differs from the difference of the
+            // rounded c s and m by up to half an ulp of m: a factor without
+            // bounds for large scores (the type's lowest value as a mask).
+            // From |m| = BIG on the row's scores, whose differences are then
+            // 0, an ulp's noise, or too large for the smaller key to count,
+            // are multiplied by a power of two up to c instead, which is
+            // exact (scores times c first, in the rows that need it: 21.5
+            // us instead of 20.8, 16 x 512 tokens, 8 heads of 48).
+            constexpr float BIG = BF ? 268435456.0f : 16777216.0f;  // half an ulp: 2^3, 2^-1
+            float shift = SHIFT;
+            uint64_t c2 = ptx::f2_pack(ga.c, ga.c);
             uint64_t l2[2] = {0, 0};
             for (int j = 0; j < mine; j++, n_s++) {
                 ok = ga_wait(sfull + t, n_s & 1, gave_up);
@@ -610,14 +621,21 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                         mx[x] = i == 0 ? ga_max(u, u, v) : ga_max(mx[x], u, v);
                     }
                 // a row that sees a NaN or +infinity is NaN from here on
-                float top = ga_max(ga_max(mx[0], mx[1], mx[2]), mx[3], mx[3]) * ga.c;
+                const float most = ga_max(ga_max(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+                float top = most * ga.c;
                 const bool far = real && !(top <= m + 8.0f);
                 if (__any_sync(0xffffffffu, far)) {
                     if (!(top < INFINITY)) top = NAN;
-                    const float mn = far ? top : m;
-                    const float f = far ? (m == -INFINITY ? 0.0f : ga_ex2(m - mn)) : 1.0f;
-                    m = mn;
-                    off = m == -INFINITY ? 0.0f : SHIFT - m;
+                    float f = 1.0f;
+                    if (far) {
+                        const bool big = fabsf(top) >= BIG && top > -INFINITY;
+                        const float to = big ? 0.0f : SHIFT, c = big ? ga.c_two : ga.c;
+                        f = m == -INFINITY ? 0.0f : ga_ex2(m - top + (to - shift));
+                        m = top;
+                        shift = to;
+                        off = m == -INFINITY ? 0.0f : to - (big ? most * c : m);
+                        c2 = ptx::f2_pack(c, c);
+                    }
                     const uint64_t f2 = ptx::f2_pack(f, f);
                     l2[0] = ptx::f2_fma(l2[0], f2, 0);
                     l2[1] = ptx::f2_fma(l2[1], f2, 0);
@@ -738,7 +756,7 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                 }
             }
             if (real && a.lse)
-                a.lse[(long long)h * a.total_q + q0 + tok] = none ? -INFINITY : (log2f(l) - off) * 0.6931471805599453f;
+                a.lse[(long long)h * a.total_q + q0 + tok] = none ? -INFINITY : (log2f(l) - shift + m) * 0.6931471805599453f;
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(itemfree + k % GA_SLOTS);
         }
@@ -847,12 +865,15 @@ static int ga_launch(const GaArgs &ga, int sm_count, cudaStream_t st, std::strin
 
 int launch_gqa_attention(const GqaAttnArgs &args, int dtype, void *scratch, int sm_count, cudaStream_t st,
                          std::string *msg) {
-    GaArgs ga{args, 0.0f, args.H / args.Hkv, 0, 0, 0};
+    GaArgs ga{args, 0.0f, 0.0f, args.H / args.Hkv, 0, 0, 0};
     GqaAttnArgs &a = ga.a;
     ga.TT = GA_ROWS / ga.G;
     // at most this many, whatever the sequences' lengths are
     ga.items = std::min(a.total_q, a.total_q / (2 * ga.TT) + a.n_seq);
     ga.c = std::max(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // 0 would turn a hidden key's -inf into NaN
+    int up;
+    frexpf(ga.c, &up);  // c / 2^up is in [0.5, 1)
+    ga.c_two = ldexpf(0.5f, up);
     ga.vec = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.o_ts % 8 == 0 && a.o_hs % 8 == 0 && a.hd % 8 == 0;
     const GaCopies cp = ga_copies(args);
     if (cp.q || cp.k || cp.v) {
