@@ -264,3 +264,35 @@ def test_prompt_lowest_scores(dtype, big, H, Hkv, hd):
     assert ((out[n:].double() - o).abs() <= 2.02 * ref.ROUNDOFF[dtype] * o.abs()).all()
     assert ((lse[:, n:].double() - z[0]) / z[0]).abs().max() < 1e-5
     assert torch.equal(out[:n], wb.gqa_attention(q, k, v, [0, T])[:n])
+
+
+@pytest.mark.parametrize("store", ["native", "int8", "e4m3"])
+@pytest.mark.parametrize("dtype,big", LOWEST)
+@pytest.mark.parametrize("H,Hkv,hd", [(2, 2, 64), (24, 2, 128)])
+def test_decode_lowest_scores(store, dtype, big, H, Hkv, hd):
+    import torch
+    if store != "native" and big < 1.0:
+        return  # 8-bit keys: dimensions of a bf16 query far below its largest are 0
+    dtype = getattr(torch, dtype)
+    n, T = 300, 700
+    q, k, low, v = _lowest(dtype, Hkv, hd, H, n, T, big)
+    q = q[-1:]
+    c = _cache(low, v, [T], store)
+    out, lse = c.decode(0, q, return_lse=True)
+    kk, vv = _held(k[n:], store), _held(v[n:], store)
+    o, m, z = ref.attention(q, kk, vv, [0, 1], [0, T - n], True, hd ** -0.5)
+    pair = store == "native" and dtype == torch.bfloat16
+    ref.check(out, lse.T, o, m, z, 2.0 ** -16 if pair else 2.0 ** -11, 0.0 if pair else ref.floor(T, vv))
+    for held in (1, 30, n):
+        c.lens[0, 0] = held
+        out, lse = c.decode(0, q, return_lse=True)
+        assert torch.isfinite(out).all() and out.abs().max() <= 1.01 * v.abs().max()
+        want = ref.attention(q, _held(low[:held], store), _held(v[:held], store), [0, 1], [0, held], True, hd ** -0.5)[2][0]
+        assert ((lse.T.double() - want) / want).abs().max() < 1e-5
+    if store == "native":
+        c.lens[0, 0] = T
+        high = k[n:n + 1].clone()
+        high[:, :, 0] = torch.finfo(dtype).max
+        c.write(0, high, v[n:n + 1], [0], [0, 1], [T - 1])
+        o = v[n].double().repeat_interleave(H // Hkv, 0)[None]
+        assert ((c.decode(0, q).double() - o).abs() <= 2.02 * ref.ROUNDOFF[dtype] * o.abs()).all()

@@ -560,6 +560,14 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
 #pragma unroll
                     for (int i = 0; i < 4; i++) s[nb][i] *= sc[8 * (i >> 1)];
             }
+            // Scores as rounded products: their difference from the largest is
+            // then exact, however large they are (the type's lowest value as
+            // a mask); as one operation, fac s + off, it would be off by up to
+            // half an ulp of the largest.
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[nb][i] = __fmul_rn(s[nb][i], fac[nb][i & 1]);
             // weights of the first n keys (all 16 unless TAIL)
             float pr[NB][4];
             uint32_t pf[NB][2];  // fp16 or bf16: key r, key r + 8
@@ -574,7 +582,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             float &p = pr[nb][2 * g + e];
-                            p = ex2(fmaf(s[nb][2 * g + e], fac[nb][e], off[nb][e]));
+                            p = ex2(__fadd_rn(s[nb][2 * g + e], off[nb][e]));
                             w[e] = QUANT ? p * vs[g] * e2[nb][e] : p;  // in this order 0 stays 0
                             if (TAIL && r + 8 * g >= n) p = w[e] = 0.0f;
                         }
@@ -598,8 +606,10 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                         float mx = -INFINITY, mx2 = GD_SMALL;
 #pragma unroll
                         for (int g = 0; g < 2; g++)
-                            if (!TAIL || r + 8 * g < n) mx = fmaxf(mx, s[nb][2 * g + e] * fac[nb][e]);
-                        const float to = fminf(off[nb][e], SHIFT - oct_max(mx)), d = to - off[nb][e];
+                            if (!TAIL || r + 8 * g < n) mx = fmaxf(mx, s[nb][2 * g + e]);
+                        mx = oct_max(mx);
+                        // SHIFT - mx would be rounded from 2^24 on
+                        const float to = fminf(off[nb][e], (fabsf(mx) < 16777216.0f ? SHIFT : 0.0f) - mx), d = to - off[nb][e];
                         l[nb][e] *= ex2(d);
                         off[nb][e] = to;
                         f2[e] = ex2(d);
@@ -607,7 +617,7 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
                             // a scale of 0 (a caller's own pages) counts as 2^-118
 #pragma unroll
                             for (int g = 0; g < 2; g++)
-                                if (!TAIL || r + 8 * g < n) mx2 = fmaxf(mx2, fmaf(s[nb][2 * g + e], fac[nb][e], to) + lg2(vs[g]));
+                                if (!TAIL || r + 8 * g < n) mx2 = fmaxf(mx2, s[nb][2 * g + e] + to + lg2(vs[g]));
                             const float to2 = fmaxf(d2[nb][e] + d, oct_max(mx2));
                             f2[e] = ex2(d + d2[nb][e] - to2);
                             d2[nb][e] = to2;
