@@ -296,3 +296,17 @@ def test_decode_lowest_scores(store, dtype, big, H, Hkv, hd):
         c.write(0, high, v[n:n + 1], [0], [0, 1], [T - 1])
         o = v[n].double().repeat_interleave(H // Hkv, 0)[None]
         assert ((c.decode(0, q).double() - o).abs() <= 2.02 * ref.ROUNDOFF[dtype] * o.abs()).all()
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-36, -1e-36])
+def test_scales_near_zero(scale):
+    """Scores of 1e32 and a scale that makes them nothing, or little: the mean of the values."""
+    import torch
+    import wave_engine_b200 as wb
+    T, hd = 300, 64
+    k, v = _rows(18, torch.bfloat16, T, 1, hd)
+    q, _ = _rows(19, torch.bfloat16, T, 2, hd)
+    out, lse = wb.gqa_attention(q * 1e16, k * 1e16, v, [0, T], scale=scale, return_lse=True)
+    o, m, z = ref.attention(q, k, v, [0, T], [0, T], True, 0.0)
+    ref.check(out, None, o, m, z)
+    assert (lse.double() - z[0]).abs().max() < 1e-2

@@ -51,7 +51,7 @@ static constexpr int GA_EDGES = 4;  // most key tiles that some row of a CTA see
 
 struct GaArgs {
     GqaAttnArgs a;
-    float c;      // |scale| log2 e, at least 1e-30
+    float c;      // |scale| log2 e, at least the smallest subnormal
     float c_two;  // the largest power of two that is not above c
     int G, TT;    // heads per key-value head, tokens of a query tile
     int vec;      // out rows take 16-byte stores
@@ -870,7 +870,9 @@ int launch_gqa_attention(const GqaAttnArgs &args, int dtype, void *scratch, int 
     ga.TT = GA_ROWS / ga.G;
     // at most this many, whatever the sequences' lengths are
     ga.items = std::min(a.total_q, a.total_q / (2 * ga.TT) + a.n_seq);
-    ga.c = std::max(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);  // 0 would turn a hidden key's -inf into NaN
+    // 0 would turn a hidden key's -inf into NaN; times the smallest subnormal
+    // every finite score is 0, to 2^-21
+    ga.c = std::max(fabsf(a.scale) * 1.4426950408889634f, 1.40129846e-45f);
     int up;
     frexpf(ga.c, &up);  // c / 2^up is in [0.5, 1)
     ga.c_two = ldexpf(0.5f, up);
