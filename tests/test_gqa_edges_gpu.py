@@ -310,3 +310,29 @@ def test_scales_near_zero(scale):
     o, m, z = ref.attention(q, k, v, [0, T], [0, T], True, 0.0)
     ref.check(out, None, o, m, z)
     assert (lse.double() - z[0]).abs().max() < 1e-2
+
+
+def test_first_call_inside_a_capture_on_the_own_stream():
+    """Scratch that is made while the context's own stream is captured stays out of the graph."""
+    import torch
+    import wave_engine_b200 as wb
+    from wave_engine_b200 import _lib
+    ctx = wb.Context(0)
+    q, _ = _rows(12, torch.bfloat16, 40, 4, 42)  # rows that are copied into scratch
+    k, v = _rows(13, torch.bfloat16, 40, 2, 42)
+    cu = _ints(0, 25, 40)
+    want = wb.gqa_attention(q, k, v, cu)
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    stream = torch.cuda.ExternalStream(_lib.lib().wb_context_own_stream(ctx.handle))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        wb.gqa_attention(q, k, v, cu, out=out, ctx=ctx)
+    for _ in range(2):
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    graph.reset()
+    ctx.close()

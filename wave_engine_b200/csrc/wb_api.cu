@@ -1891,7 +1891,8 @@ int guarded(F &&f) {
 // keeps the replaced buffer until the context ends (kernels in flight and
 // captured graphs may name it) and doubles, so the kept ones sum to less than
 // the live one.  A new buffer is zeroed before first use, also during a
-// stream capture (where nothing may run on the captured stream itself).
+// stream capture: on a copy stream, which callers cannot capture (their own
+// streams and the context's they can).
 int gqa_workspace(wb_context *ctx, size_t bytes, DevBuf **out) {
     DevBuf &w = ctx->gqa_ws[ctx->stream];
     *out = &w;
@@ -1901,11 +1902,13 @@ int gqa_workspace(wb_context *ctx, size_t bytes, DevBuf **out) {
     w = DevBuf{};
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     cudaThreadExchangeStreamCaptureMode(&mode);
+    const int rc = copy_streams(ctx, 0);
     void *p = nullptr;
-    cudaError_t e = cudaMalloc(&p, want);
-    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, want, ctx->own);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->own);
+    cudaError_t e = rc == WB_OK ? cudaMalloc(&p, want) : cudaErrorUnknown;
+    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, want, ctx->cp_in);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->cp_in);
     cudaThreadExchangeStreamCaptureMode(&mode);
+    if (rc != WB_OK) return rc;
     if (e != cudaSuccess) {
         cudaGetLastError();
         if (p) ctx->gqa_old.push_back(p);
