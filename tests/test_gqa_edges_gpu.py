@@ -336,3 +336,34 @@ def test_first_call_inside_a_capture_on_the_own_stream():
         assert torch.equal(out, want)
     graph.reset()
     ctx.close()
+
+
+def test_scratch_that_cannot_grow():
+    """A call whose scratch does not fit is refused and costs nothing: the scratch there was serves the next call.  Growth
+    that fits but not twice over is granted."""
+    import torch
+    import wave_engine_b200 as wb
+    ctx = wb.Context(0)
+    hd = 127  # rows that are copied into scratch: 256 bytes a key here, whatever the keys' own stride
+    q, _ = _rows(14, torch.bfloat16, 3, 1, hd)
+    one, _ = _rows(15, torch.bfloat16, 1, 1, hd)
+    cu, ck = _ints(0, 3), _ints(0, 3)
+
+    def call(rows):
+        k = one.expand(rows, 1, hd)
+        return wb.gqa_attention(q, k, one[0, 0].expand(rows, 1, hd), cu, ck, ctx=ctx)
+
+    want = call(1000)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(3):
+        with pytest.raises(wb.WaveB200Error):
+            call(2 ** 31 - 1)  # two terabytes
+        assert torch.equal(call(1000), want)
+        torch.cuda.synchronize()
+        assert torch.cuda.mem_get_info()[0] >= free - 2 ** 20
+    part = free // 512  # keys whose copies (K and V) fill the memory
+    assert torch.equal(call(int(0.35 * part)), want)
+    assert torch.equal(call(int(0.42 * part)), want)
+    ctx.close()

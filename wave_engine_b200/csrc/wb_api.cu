@@ -1888,34 +1888,41 @@ int guarded(F &&f) {
 }
 
 // At least `bytes` of the context's scratch for its current stream.  Growing
-// keeps the replaced buffer until the context ends (kernels in flight and
-// captured graphs may name it) and doubles, so the kept ones sum to less than
-// the live one.  A new buffer is zeroed before first use, also during a
-// stream capture: on a copy stream, which callers cannot capture (their own
-// streams and the context's they can).
+// doubles where that fits, and keeps the replaced buffer until the context
+// ends (kernels in flight and captured graphs may name it); a growth that
+// fails leaves the scratch as it was.  The counters of a new buffer are
+// zeroed before first use, also during a stream capture: on a copy stream,
+// which callers cannot capture (their own streams and the context's they can).
 int gqa_workspace(wb_context *ctx, size_t bytes, DevBuf **out) {
     DevBuf &w = ctx->gqa_ws[ctx->stream];
     *out = &w;
     if (bytes <= w.n) return WB_OK;
-    const size_t want = std::max(bytes, 2 * w.n);
-    if (w.p) ctx->gqa_old.push_back(w.p);
-    w = DevBuf{};
+    ctx->gqa_old.reserve(ctx->gqa_old.size() + 1);
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     cudaThreadExchangeStreamCaptureMode(&mode);
-    const int rc = copy_streams(ctx, 0);
-    void *p = nullptr;
-    cudaError_t e = rc == WB_OK ? cudaMalloc(&p, want) : cudaErrorUnknown;
-    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, want, ctx->cp_in);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->cp_in);
+    DevBuf n;
+    n.n = std::max(bytes, 2 * w.n);
+    int rc = copy_streams(ctx, 0);
+    if (rc == WB_OK) {
+        cudaError_t e = cudaMalloc(&n.p, n.n);
+        if (e != cudaSuccess && n.n > bytes) {
+            cudaGetLastError();
+            n.n = bytes;
+            e = cudaMalloc(&n.p, n.n);
+        }
+        if (e != cudaSuccess) n.p = nullptr;
+        else e = cudaMemsetAsync(n.p, 0, wb::GQA_WS_HEAD, ctx->cp_in);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->cp_in);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            rc = fail(n.p ? WB_ECUDA : WB_ENOMEM, "scratch of " + std::to_string(n.n) + " bytes: " + cudaGetErrorString(e));
+            if (n.p) cudaFree(n.p);
+        }
+    }
     cudaThreadExchangeStreamCaptureMode(&mode);
     if (rc != WB_OK) return rc;
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        if (p) ctx->gqa_old.push_back(p);
-        return fail(p ? WB_ECUDA : WB_ENOMEM, "scratch of " + std::to_string(want) + " bytes: " + cudaGetErrorString(e));
-    }
-    w.p = p;
-    w.n = want;
+    if (w.p) ctx->gqa_old.push_back(w.p);
+    w = n;
     return WB_OK;
 }
 
