@@ -445,8 +445,10 @@ WB_API int wb_lm_head(wb_context *ctx, const float *hidden, int n_rows, int n_em
  * device memory, which the host does not read (no synchronisation; can be
  * captured in a CUDA graph): the kernels then skip what lies outside the
  * buffers and set bit 0x8 (bounds) of the device error word.  Scratch is the
- * context's, one per stream: graphs captured on the same stream share it and
- * must not run at the same time, nor beside calls on that stream. */
+ * context's, one per stream.  Calls during a capture take scratch of their
+ * own, which the graph keeps: graphs may run beside each other and beside
+ * calls, and after the context is gone.  Executables instantiated from one and
+ * the same graph share it and must not run at the same time. */
 /* element types */
 #define WB_BF16 0
 #define WB_F16 1

@@ -367,3 +367,127 @@ def test_scratch_that_cannot_grow():
     assert torch.equal(call(int(0.35 * part)), want)
     assert torch.equal(call(int(0.42 * part)), want)
     ctx.close()
+
+
+def _step(seed, lens, H=8, Hkv=2, hd=128, store="native"):
+    """A decode and an append with queries and rows at fixed places, and what the decode gives."""
+    import torch
+    k, v = _rows(seed, torch.bfloat16, sum(lens), Hkv, hd)
+    c = _cache(k, v, lens, store)
+    q = _rows(seed + 1, torch.bfloat16, len(lens), H, hd)[0]
+    odd = _rows(seed + 2, torch.bfloat16, 50, 2, 42)[0]  # rows that are copied into scratch
+    out, prompt = torch.zeros_like(q), torch.zeros_like(odd)
+    start, cu = _ints(*(n - 1 for n in lens)), _ints(0, 20, 50)
+    last = torch.stack([k[n - 1] for n in ref.starts(lens)[1:]]), torch.stack([v[n - 1] for n in ref.starts(lens)[1:]])
+
+    def step():
+        import wave_engine_b200 as wb
+        c.write(0, *last, None, None, start)
+        c.decode(0, q, out=out)
+        wb.gqa_attention(odd, odd, odd, cu, out=prompt)
+
+    return step, out, prompt
+
+
+def test_a_graph_outlives_its_thread():
+    """The context of a thread that captured a graph ends with it; the graph keeps what its kernels use."""
+    import gc
+    import threading
+    import torch
+    import wave_engine_b200 as wb
+    made = {}
+
+    def capture():
+        step, out, prompt = _step(30, [3000, 70, 1500])
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            step()
+            stream.synchronize()
+            made["want"] = out.clone(), prompt.clone()
+            made["graph"] = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(made["graph"], stream=stream):
+                step()
+            stream.synchronize()
+        made["out"], made["keep"] = (out, prompt), step
+
+    thread = threading.Thread(target=capture)
+    thread.start()
+    thread.join()
+    gc.collect()
+    ctx = wb.Context(0)  # takes what memory the thread's context gave back
+    junk = torch.full((64 << 20,), -1, dtype=torch.int32, device="cuda")
+    q, _ = _rows(33, torch.bfloat16, 2000, 4, 42)
+    wb.gqa_attention(q, q, q, [0, 2000], ctx=ctx)
+    for _ in range(3):
+        for x in made["out"]:
+            x.zero_()
+        made["graph"].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(made["out"], made["want"]))
+    assert (junk == -1).all()
+    ctx.close()
+
+
+def test_graphs_of_one_stream_run_side_by_side():
+    """Two graphs captured on one stream, replayed on two at the same time, beside calls."""
+    import torch
+    steps = [_step(40 + 10 * i, [5000 + 100 * i, 64, 900]) for i in range(3)]
+    capture = torch.cuda.Stream()
+    capture.wait_stream(torch.cuda.current_stream())
+    graphs, want = [], []
+    with torch.cuda.stream(capture):
+        for step, out, prompt in steps:
+            step()
+            capture.synchronize()
+            want.append((out.clone(), prompt.clone()))
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=capture):
+                step()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(50):
+        for _, out, prompt in steps:
+            out.zero_(), prompt.zero_()
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for graph, stream in zip(graphs[:2], streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            with torch.cuda.stream(capture):
+                steps[2][0]()
+        torch.cuda.synchronize()
+        for (_, out, prompt), (o, p) in zip(steps, want):
+            assert torch.equal(out, o) and torch.equal(prompt, p)
+
+
+def test_scratch_of_graphs_is_given_back():
+    import time
+    import torch
+    import wave_engine_b200 as wb
+    q, _ = _rows(50, torch.bfloat16, 1, 1, 127)
+    rows = 4000000  # 2 GB of copies
+    k, cu = q.expand(rows, 1, 127), _ints(0, 1)
+    ctx = wb.Context(0)
+    out = torch.empty_like(q)
+    ck = _ints(0, 10)
+    wb.gqa_attention(q, k[:10], k[:10], cu, ck, out=out, ctx=ctx)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        wb.gqa_attention(q, k, k, cu, ck, out=out, ctx=ctx)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, q) and torch.cuda.mem_get_info()[0] < free - 2 ** 30
+    ctx.close()
+    graph.replay()
+    torch.cuda.synchronize()
+    graph.reset()
+    torch.cuda.empty_cache()
+    for _ in range(100):
+        wb.Context(0).close()  # frees what no graph holds any more
+        if torch.cuda.mem_get_info()[0] >= free - 2 ** 28:
+            break
+        time.sleep(0.05)
+    assert torch.cuda.mem_get_info()[0] >= free - 2 ** 28

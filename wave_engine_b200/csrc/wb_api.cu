@@ -10,12 +10,15 @@
 #include "wb_serve.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
+#include <utility>
 #include <vector>
 
 namespace {
@@ -107,6 +110,73 @@ int upload(T **dst, const std::vector<T> &src) {
     return WB_OK;
 }
 
+// Device memory that a context and captured graphs hold together: a graph may
+// be launched after the context is gone.  The destructor of a graph's
+// reference may not call CUDA, so the last one to let go only says so, and
+// buf_reap frees what nobody holds.
+struct HeldBuf {
+    void *p;
+    size_t n;
+    int device;
+    std::atomic<int> refs{1};
+};
+std::mutex g_held_mutex;
+std::vector<HeldBuf *> g_held;
+
+// Takes over p (freed when it fails).
+HeldBuf *buf_hold(void *p, size_t n, int device) {
+    HeldBuf *b = new (std::nothrow) HeldBuf{p, n, device};
+    if (b) {
+        try {
+            std::lock_guard<std::mutex> lock(g_held_mutex);
+            g_held.push_back(b);
+            return b;
+        } catch (...) {
+            delete b;
+        }
+    }
+    cudaFree(p);
+    return nullptr;
+}
+
+void CUDART_CB buf_drop(void *b) { static_cast<HeldBuf *>(b)->refs.fetch_sub(1, std::memory_order_acq_rel); }
+
+// Frees the current device's buffers that nobody holds (cudaFree waits for
+// kernels in flight).  Not while this thread's stream is captured.
+void buf_reap(int device) {
+    std::lock_guard<std::mutex> lock(g_held_mutex);
+    size_t kept = 0;
+    for (HeldBuf *b : g_held) {
+        if (b->device == device && b->refs.load(std::memory_order_acquire) == 0) {
+            cudaFree(b->p);
+            delete b;
+        } else g_held[kept++] = b;
+    }
+    g_held.resize(kept);
+}
+
+// One more holder: the graph under capture.
+cudaError_t buf_retain(HeldBuf *b, cudaGraph_t graph) {
+    cudaUserObject_t obj;
+    b->refs.fetch_add(1, std::memory_order_acq_rel);
+    cudaError_t e = cudaUserObjectCreate(&obj, b, buf_drop, 1, cudaUserObjectNoDestructorSync);
+    if (e != cudaSuccess) {
+        buf_drop(b);
+        return e;
+    }
+    e = cudaGraphRetainUserObject(graph, obj, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) cudaUserObjectRelease(obj, 1);  // drops b
+    return e;
+}
+
+// Calls that are not allowed while another stream is captured, such as
+// allocations, are while one of these lives (none touches a captured stream).
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 }  // namespace
 
 struct wb_context {
@@ -121,11 +191,14 @@ struct wb_context {
     // host-buffer pipelines: copies up, copies down, and their events
     cudaStream_t cp_in = nullptr, cp_out = nullptr;
     std::vector<cudaEvent_t> ev;
+    HeldBuf *err = nullptr;  // holds dev_err
     // wb_gqa_* scratch, one per stream (calls on different streams never
-    // share one), and the buffers that growth replaced (a captured graph may
-    // still name them)
-    std::map<cudaStream_t, DevBuf> gqa_ws;
-    std::vector<void *> gqa_old;
+    // share one), and one per stream and capture, which the graph keeps
+    struct GqaScratch {
+        HeldBuf *buf = nullptr, *captured = nullptr;
+        unsigned long long capture = 0;  // id of the capture that `captured` belongs to
+    };
+    std::map<cudaStream_t, GqaScratch> gqa_ws;
 };
 
 // Creates ctx's copy streams and at least n events on first need.
@@ -359,13 +432,15 @@ int wb_context_create(int device, wb_context **out) {
     c->sm_count = prop.multiProcessorCount;
     if (cudaStreamCreateWithFlags(&c->own, cudaStreamNonBlocking) != cudaSuccess ||
         cudaMalloc(&c->dev_err, sizeof(uint32_t)) != cudaSuccess ||
-        cudaMemset(c->dev_err, 0, sizeof(uint32_t)) != cudaSuccess) {
+        cudaMemset(c->dev_err, 0, sizeof(uint32_t)) != cudaSuccess ||
+        !(c->err = buf_hold(std::exchange(c->dev_err, nullptr), sizeof(uint32_t), device))) {
         cudaGetLastError();
         if (c->own) cudaStreamDestroy(c->own);
         if (c->dev_err) cudaFree(c->dev_err);
         delete c;
         return fail(WB_ECUDA, "context allocation failed");
     }
+    c->dev_err = (uint32_t *)c->err->p;
     c->stream = c->own;
     *out = c;
     return WB_OK;
@@ -377,7 +452,6 @@ int wb_context_destroy(wb_context *ctx) {
     cudaStreamSynchronize(ctx->stream);
     if (ctx->ws.p) cudaFree(ctx->ws.p);
     if (ctx->io.p) cudaFree(ctx->io.p);
-    if (ctx->dev_err) cudaFree(ctx->dev_err);
     if (ctx->cp_in) {
         cudaStreamSynchronize(ctx->cp_in);
         cudaStreamDestroy(ctx->cp_in);
@@ -388,8 +462,13 @@ int wb_context_destroy(wb_context *ctx) {
     }
     for (cudaEvent_t e : ctx->ev) cudaEventDestroy(e);
     for (auto &w : ctx->gqa_ws)
-        if (w.second.p) cudaFree(w.second.p);
-    for (void *p : ctx->gqa_old) cudaFree(p);
+        for (HeldBuf *b : {w.second.buf, w.second.captured})
+            if (b) buf_drop(b);
+    buf_drop(ctx->err);
+    {
+        RelaxedCapture relaxed;
+        buf_reap(ctx->device);
+    }
     if (ctx->own) cudaStreamDestroy(ctx->own);
     wb::prof_destroy(ctx->prof);
     delete ctx;
@@ -1887,42 +1966,56 @@ int guarded(F &&f) {
     }
 }
 
-// At least `bytes` of the context's scratch for its current stream.  Growing
-// doubles where that fits, and keeps the replaced buffer until the context
-// ends (kernels in flight and captured graphs may name it); a growth that
-// fails leaves the scratch as it was.  The counters of a new buffer are
-// zeroed before first use, also during a stream capture: on a copy stream,
+// At least `bytes` of scratch for a call on the context's current stream: the
+// stream's or, while it is captured, one that belongs to the capture and that
+// the graph keeps (with the error word), so that graphs share scratch neither
+// with each other nor with calls, and outlive the context.  Growing
+// doubles where that fits; a growth that fails leaves the scratch as it was.
+// The counters of a new buffer are zeroed before first use, on a copy stream,
 // which callers cannot capture (their own streams and the context's they can).
-int gqa_workspace(wb_context *ctx, size_t bytes, DevBuf **out) {
-    DevBuf &w = ctx->gqa_ws[ctx->stream];
-    *out = &w;
-    if (bytes <= w.n) return WB_OK;
-    ctx->gqa_old.reserve(ctx->gqa_old.size() + 1);
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    DevBuf n;
-    n.n = std::max(bytes, 2 * w.n);
-    int rc = copy_streams(ctx, 0);
-    if (rc == WB_OK) {
-        cudaError_t e = cudaMalloc(&n.p, n.n);
-        if (e != cudaSuccess && n.n > bytes) {
-            cudaGetLastError();
-            n.n = bytes;
-            e = cudaMalloc(&n.p, n.n);
-        }
-        if (e != cudaSuccess) n.p = nullptr;
-        else e = cudaMemsetAsync(n.p, 0, wb::GQA_WS_HEAD, ctx->cp_in);
-        if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->cp_in);
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            rc = fail(n.p ? WB_ECUDA : WB_ENOMEM, "scratch of " + std::to_string(n.n) + " bytes: " + cudaGetErrorString(e));
-            if (n.p) cudaFree(n.p);
-        }
+int gqa_workspace(wb_context *ctx, size_t bytes, HeldBuf **out) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    WB_CUDA(cudaStreamGetCaptureInfo_v2(ctx->stream, &status, &id, &graph, nullptr, nullptr));
+    const bool capturing = status == cudaStreamCaptureStatusActive;
+    wb_context::GqaScratch &w = ctx->gqa_ws[ctx->stream];
+    if (capturing && w.capture != id) {
+        if (w.captured) buf_drop(w.captured);
+        w.captured = nullptr;
+        w.capture = id;
     }
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    if (rc != WB_OK) return rc;
-    if (w.p) ctx->gqa_old.push_back(w.p);
-    w = n;
+    HeldBuf *&slot = capturing ? w.captured : w.buf;
+    *out = slot;
+    if (slot && bytes <= slot->n) return WB_OK;
+    RelaxedCapture relaxed;
+    WB_TRY(copy_streams(ctx, 0));
+    if (!capturing) buf_reap(ctx->device);
+    size_t n = slot ? std::max(bytes, 2 * slot->n) : bytes;
+    void *p = nullptr;
+    cudaError_t e = cudaMalloc(&p, n);
+    if (e != cudaSuccess && n > bytes) {
+        cudaGetLastError();
+        n = bytes;
+        e = cudaMalloc(&p, n);
+    }
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(WB_ENOMEM, "scratch of " + std::to_string(n) + " bytes: " + cudaGetErrorString(e));
+    }
+    HeldBuf *b = buf_hold(p, n, ctx->device);
+    if (!b) return fail(WB_ENOMEM, "out of host memory");
+    e = cudaMemsetAsync(p, 0, wb::GQA_WS_HEAD, ctx->cp_in);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->cp_in);
+    if (e == cudaSuccess && capturing) e = buf_retain(b, graph);
+    if (e == cudaSuccess && capturing && !slot) e = buf_retain(ctx->err, graph);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        buf_drop(b);
+        return fail(WB_ECUDA, std::string("scratch: ") + cudaGetErrorString(e));
+    }
+    if (slot) buf_drop(slot);
+    *out = slot = b;
     return WB_OK;
 }
 
@@ -2036,7 +2129,7 @@ int gqa_move_indexes(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t 
             if (start[i] < 0 || start[i] + n > (int64_t)c->max_pages * WB_PAGE)
                 return fail(WB_EINVAL, "positions outside the slot's table");
         }
-    DevBuf *w;
+    HeldBuf *w;
     WB_TRY(gqa_workspace(ctx, wb::GQA_WS_HEAD + ix.bytes(), &w));
     *ticket = (unsigned int *)w->p + wb::GQA_WS_TICKET;
     return ix.upload((char *)w->p + wb::GQA_WS_HEAD, ctx->stream);
@@ -2077,7 +2170,7 @@ int wb_gqa_attention(wb_context *ctx, const wb_gqa_attn_desc *d) {
         IndexArgs ix;
         if (ix.add(d->cu_q, d->n_seq + 1, &a.cu_q)) WB_TRY(check_starts(d->cu_q, d->n_seq, d->total_q, "cu_q"));
         if (ix.add(d->cu_k, d->n_seq + 1, &a.cu_k)) WB_TRY(check_starts(d->cu_k, d->n_seq, d->total_k, "cu_k"));
-        DevBuf *w;
+        HeldBuf *w;
         size_t extra = wb::gqa_attention_scratch(a, d->dtype);
         WB_TRY(gqa_workspace(ctx, wb::GQA_WS_HEAD + ix.bytes() + extra, &w));
         WB_TRY(ix.upload((char *)w->p + wb::GQA_WS_HEAD, ctx->stream));
@@ -2157,7 +2250,7 @@ int wb_gqa_decode(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *sl
         ProfBind pb(ctx);
         IndexArgs ix;
         if (ix.add(slots, n_seq, &ca.slots)) WB_TRY(check_slots(slots, n_seq, c->n_slots));
-        DevBuf *w;
+        HeldBuf *w;
         const size_t extra = wb::gqa_decode_scratch(ca, n_head, ctx->sm_count);
         WB_TRY(gqa_workspace(ctx, wb::GQA_WS_HEAD + ix.bytes() + extra, &w));
         WB_TRY(ix.upload((char *)w->p + wb::GQA_WS_HEAD, ctx->stream));
