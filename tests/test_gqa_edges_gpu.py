@@ -491,3 +491,44 @@ def test_scratch_of_graphs_is_given_back():
             break
         time.sleep(0.05)
     assert torch.cuda.mem_get_info()[0] >= free - 2 ** 28
+
+
+@pytest.mark.parametrize("slots", [None, [0, 1, 2, 3], [2, 0, 3, 1]])
+def test_starts_that_are_the_lengths(slots):
+    """start = the cache's own lengths: all of them are read before one changes, in a graph too."""
+    import torch
+    import wave_engine_b200 as wb
+    Hkv, hd, held, add = 4, 64, [100, 7, 300, 0], [200, 129, 1, 250]
+    k, v = _rows(60, torch.bfloat16, sum(held), Hkv, hd)
+    k2, v2 = _rows(61, torch.bfloat16, sum(add), Hkv, hd)
+    at = [0, 1, 2, 3] if slots is None else slots
+    cu = _ints(*ref.starts(add))
+    c = wb.GqaCache(1, Hkv, hd, 4, 600, 20)
+    for i in range(4):
+        c.reserve(i, 600)
+    index = None if slots is None else _ints(*slots)
+
+    def call():
+        c.write(0, k2, v2, index, cu, c.lens[0])
+
+    def check():
+        assert wb.default_context(0).take_device_error() == 0
+        want = [0] * 4
+        for i, s in enumerate(at):
+            want[s] = held[i] + add[i]
+        assert c.lens[0].tolist() == want
+        gk, gv = c.read(0, index, cu, sum(add), _ints(*held))
+        assert torch.equal(gk, k2) and torch.equal(gv, v2)
+
+    for _ in range(20):
+        c.write(0, k, v, [0, 1, 2, 3], ref.starts(held), [0, 0, 0, 0])
+        call()
+        check()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        call()
+    c.write(0, k, v, [0, 1, 2, 3], ref.starts(held), [0, 0, 0, 0])
+    graph.replay()
+    check()

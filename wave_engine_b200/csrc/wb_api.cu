@@ -2113,9 +2113,11 @@ int check_slots(const int32_t *slots, int n_seq, int n_slots) {
     return WB_OK;
 }
 
-// What the write and the read share: their index arrays.
+// What the write and the read share: their index arrays.  A write's starts
+// that lie in the lengths it sets (start = lens) are read before: as an append
+// where they are one, else from a copy.
 int gqa_move_indexes(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq, const int32_t *cu,
-                     int64_t total, const int32_t *start, wb::GqaCacheArgs *ca, const int32_t **cu_d,
+                     int64_t total, const int32_t *start, bool write, wb::GqaCacheArgs *ca, const int32_t **cu_d,
                      const int32_t **start_d, unsigned int **ticket) {
     if (total < 0 || total > 0x7fffffff) return fail(WB_EINVAL, "total out of range");
     if (!cu && total != n_seq) return fail(WB_EINVAL, "without cu there is one row per sequence");
@@ -2129,9 +2131,20 @@ int gqa_move_indexes(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t 
             if (start[i] < 0 || start[i] + n > (int64_t)c->max_pages * WB_PAGE)
                 return fail(WB_EINVAL, "positions outside the slot's table");
         }
+    bool copy = false;
+    if (write && *start_d) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(*start_d), b = reinterpret_cast<uintptr_t>(c->lens);
+        if (a == b && !slots) *start_d = nullptr;
+        else copy = a < b + (uintptr_t)c->n_slots * sizeof(int32_t) && b < a + (uintptr_t)n_seq * sizeof(int32_t);
+    }
     HeldBuf *w;
-    WB_TRY(gqa_workspace(ctx, wb::GQA_WS_HEAD + ix.bytes(), &w));
+    WB_TRY(gqa_workspace(ctx, wb::GQA_WS_HEAD + ix.bytes() + (copy ? n_seq * sizeof(int32_t) : 0), &w));
     *ticket = (unsigned int *)w->p + wb::GQA_WS_TICKET;
+    if (copy) {
+        void *to = (char *)w->p + wb::GQA_WS_HEAD + ix.bytes();
+        WB_CUDA(cudaMemcpyAsync(to, *start_d, n_seq * sizeof(int32_t), cudaMemcpyDeviceToDevice, ctx->stream));
+        *start_d = (const int32_t *)to;
+    }
     return ix.upload((char *)w->p + wb::GQA_WS_HEAD, ctx->stream);
 }
 
@@ -2199,7 +2212,7 @@ int wb_gqa_cache_write(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_
         ProfBind pb(ctx);
         const int32_t *cu_d, *start_d;
         unsigned int *ticket;
-        WB_TRY(gqa_move_indexes(ctx, c, slots, n_seq, cu, total, start, &ca, &cu_d, &start_d, &ticket));
+        WB_TRY(gqa_move_indexes(ctx, c, slots, n_seq, cu, total, start, true, &ca, &cu_d, &start_d, &ticket));
         std::string msg;
         int rc = wb::launch_gqa_cache_write(ca, c->dtype, cu_d, total, start_d, k, v, k_ts, k_hs, v_ts, v_hs,
                                             ticket, ctx->stream, &msg);
@@ -2223,7 +2236,7 @@ int wb_gqa_cache_read(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t
         ProfBind pb(ctx);
         const int32_t *cu_d, *start_d;
         unsigned int *ticket;
-        WB_TRY(gqa_move_indexes(ctx, c, slots, n_seq, cu, total, start, &ca, &cu_d, &start_d, &ticket));
+        WB_TRY(gqa_move_indexes(ctx, c, slots, n_seq, cu, total, start, false, &ca, &cu_d, &start_d, &ticket));
         std::string msg;
         int rc = wb::launch_gqa_cache_read(ca, c->dtype, cu_d, total, start_d, k, v, ctx->stream, &msg);
         if (rc != WB_OK) return fail(rc, msg);
