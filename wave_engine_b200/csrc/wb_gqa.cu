@@ -309,11 +309,11 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
         return (int)max(0LL, min((long long)nk, n));
     };
 
+    uint32_t g = 0, nq_loads = 0;  // warp W_TMA, lane 0: ring stages and Q pairs loaded
     if (warp >= F::W_TMA) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::R_OTHER));
         if (warp == F::W_TMA) {
             // ---- items and loads
-            uint32_t g = 0, nq_loads = 0;  // ring stages and Q pairs loaded
             bool ok = true;
             for (int k = 0;; k++) {
                 const long long index = (long long)k * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
@@ -384,13 +384,7 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                                                  q0 + tok0 + t * TT);
                         nq_loads++;
                     }
-                    if (!ok) {
-                        // copies in flight land before the CTA leaves
-                        atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
-                        if (nq_loads > 0) ptx::mbar_wait(qfull, (nq_loads - 1) & 1, 200000000LL);
-                        for (uint32_t i = g > ST ? g - ST : 0; i < g; i++)
-                            ptx::mbar_wait(full + i % ST, (i / ST) & 1, 200000000LL);
-                    }
+                    if (!ok) atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
                 }
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 if (!ok) break;
@@ -490,13 +484,12 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                         if (j + 2 == nmax) commit(qfree);
                     }
                 }
-                if (!ok && lane == 0) {
-                    atomicOr(a.dev_err, WB_DERR_TIMEOUT_MMA);
-                    // the MMAs issued have completed before TMEM is released
-                    ptx::mma_commit(done);
-                    ptx::mbar_wait(done, 0, 200000000LL);
-                }
-                __syncwarp();
+                if (!ok && lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_MMA);
+                // Every product and its arrivals, also those that no other
+                // role waits for, come before TMEM and shared memory are given
+                // back (off the softmax warps' path: it costs nothing).
+                commit(done);
+                ptx::mbar_wait(done, 0, 200000000LL);
             }
         } else {
             // ---- V tiles at the edges: 8 threads per row, one 16-byte piece
@@ -765,6 +758,14 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
     __syncwarp();
     ptx::tc_fence_before();
     __syncthreads();
+    // When some role gave up, copies may be under way, whichever it was and
+    // whether or not warp W_TMA had finished: they land before the shared
+    // memory is given back.  (Else the products have waited for each of them.)
+    if (*gave_up && warp == F::W_TMA && lane == 0) {
+        if (nq_loads > 0) ptx::mbar_wait(qfull, (nq_loads - 1) & 1, 200000000LL);
+        for (uint32_t i = g > ST ? g - ST : 0; i < g; i++) ptx::mbar_wait(full + i % ST, (i / ST) & 1, 200000000LL);
+    }
+    __syncwarp();
     if (warp == F::W_MMA) ptx::tmem_dealloc(tmem, F::TMEM);
 }
 
