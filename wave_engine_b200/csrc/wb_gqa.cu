@@ -90,7 +90,11 @@ struct GaConf {
 };
 
 // Bounded mbarrier wait that also gives up once another role has: a timeout
-// then does not chain into one per barrier.
+// then does not chain into one per barrier.  Lanes may give up apart from each
+// other, so no lane leaves a loop on its own answer: after a timeout a role
+// goes on to the item's end for nothing (every wait returns at once), where
+// the warp leaves as one (a vote in every wait: 62.3 us instead of 61.5, packed
+// 768-wide batch).
 __device__ __forceinline__ bool ga_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up) {
     if (ptx::mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
@@ -319,7 +323,8 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                 const long long index = (long long)k * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
                 if (k > 0) any = index < ga.items * a.Hkv && finder.find(a, NT * TT, index / a.Hkv, lane, &seq, &place);
                 GaItem *it = items + k % GA_SLOTS;
-                if (k >= GA_SLOTS && !ga_wait(itemfree + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS - 1) & 1, gave_up)) {
+                if (k >= GA_SLOTS &&
+                    !__all_sync(0xffffffffu, ga_wait(itemfree + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS - 1) & 1, gave_up))) {
                     if (lane == 0) atomicOr(a.dev_err, WB_DERR_TIMEOUT_TMA);
                     ok = false;
                     break;
@@ -503,19 +508,18 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
             };
             uint32_t g = 0, vgo_ph = 0;
             bool ok = true;
-            for (int k = 0; ok; k++) {
+            for (int k = 0;; k++) {
                 GaItem *it = items + k % GA_SLOTS;
-                ok = ga_wait(itemfull + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS) & 1, gave_up);
+                ok = __all_sync(0xffffffffu, ok && ga_wait(itemfull + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS) & 1, gave_up));
                 if (!ok || it->q0 < 0) break;
                 const int nmax = max(it->nt[0], it->nt[1]), edge = it->edge, nk = it->nk;
                 for (int j = edge; j < nmax; j++) {
                     const uint32_t gj = g + 1 + j;
                     const int st = (int)(gj % ST), left = nk - j * GA_KEYS;
-                    ok = ga_wait(vgo + st, (vgo_ph >> st) & 1, gave_up) && ga_wait(full + st, (gj / ST) & 1, gave_up);
-                    if (!ok) break;
+                    ok = ok && ga_wait(vgo + st, (vgo_ph >> st) & 1, gave_up) && ga_wait(full + st, (gj / ST) & 1, gave_up);
                     vgo_ph ^= 1u << st;
                     uint8_t *v0 = sm + F::OFF_V + st * F::KV_BYTES + (x >> 3) * 128 + (x & 7) * 16;
-                    for (int i0 = 0; i0 < NC * 16; i0 += 8) {  // rows x / 8 + 8 i of an atom
+                    for (int i0 = 0; ok && i0 < NC * 16; i0 += 8) {  // rows x / 8 + 8 i of an atom
                         uint4 v[8];
 #pragma unroll
                         for (int i = 0; i < 8; i++) v[i] = *reinterpret_cast<const uint4 *>(v0 + (i0 + i) * 1024);
@@ -560,12 +564,10 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
         const int row_tok = t * TT + row / G, row_g = row % G;
         uint32_t n_s = 0, n_o = 0;
         bool ok = true;
-        for (int k = 0; ok; k++) {
+        for (int k = 0;; k++) {
             const GaItem *it = items + k % GA_SLOTS;
-            if (!ga_wait(itemfull + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS) & 1, gave_up)) {
-                ok = false;
-                break;
-            }
+            ok = __all_sync(0xffffffffu, ok && ga_wait(itemfull + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS) & 1, gave_up));
+            if (!ok) break;
             const int q0 = it->q0;
             if (q0 < 0) break;
             const int mine = it->nt[t], edge = it->edge, nq = it->nq, k0 = it->k0, hk = it->hk, tok = it->tok0 + row_tok;
@@ -587,8 +589,7 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
             uint64_t c2 = ptx::f2_pack(ga.c, ga.c);
             uint64_t l2[2] = {0, 0};
             for (int j = 0; j < mine; j++, n_s++) {
-                ok = ga_wait(sfull + t, n_s & 1, gave_up);
-                if (!ok) break;
+                ok = ok && ga_wait(sfull + t, n_s & 1, gave_up);
                 ptx::tc_fence_after();
                 uint32_t s[4][32];
 #pragma unroll
@@ -669,7 +670,6 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
                     }
                 }
             }
-            if (!ok) break;
             // ---- epilogue: O / l
             float l0, l1;
             ptx::f2_unpack(ptx::f2_add(l2[0], l2[1]), l0, l1);
@@ -680,8 +680,9 @@ __global__ void __launch_bounds__(GaConf<HDP>::THREADS, 1)
             const long long at = (long long)(q0 + tok) * a.o_ts + (long long)h * a.o_hs;  // the row's place in out
             const uint32_t rows = __ballot_sync(0xffffffffu, real);
             // keys noted at the edges that this row may see
-            ok = ga_wait(fixed + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS) & 1, gave_up);
-            if (ok && mine > 0) ok = ga_wait(ofull + t, n_o++ & 1, gave_up);
+            ok = ok && ga_wait(fixed + k % GA_SLOTS, (uint32_t)(k / GA_SLOTS) & 1, gave_up);
+            if (mine > 0) ok = ok && ga_wait(ofull + t, n_o++ & 1, gave_up);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             ptx::tc_fence_after();
             const bool noted = it->any_bad;
