@@ -532,3 +532,32 @@ def test_starts_that_are_the_lengths(slots):
     c.write(0, k, v, [0, 1, 2, 3], ref.starts(held), [0, 0, 0, 0])
     graph.replay()
     check()
+
+
+def test_gradients_are_not_lost_silently():
+    """Forward only: tensors that want a gradient are refused where autograd records."""
+    import torch
+    import wave_engine_b200 as wb
+    q, _ = _rows(16, torch.bfloat16, 5, 4, 64)
+    k, v = _rows(17, torch.bfloat16, 5, 2, 64)
+    c = _cache(k, v, [5])
+    calls = [lambda q, k, v: wb.gqa_attention(q, k, v, [0, 5]), lambda q, k, v: c.write(0, k, v, [0], [0, 5], [0]),
+             lambda q, k, v: c.decode(0, q[:1])]
+    for i, call in enumerate(calls):
+        for x in range(3):
+            args = [t.clone().requires_grad_(y == x) for y, t in enumerate((q, k, v))]
+            used = x == 0 if i == 2 else x > 0 if i == 1 else True
+            if used:
+                with pytest.raises(ValueError, match="gradient"):
+                    call(*args)
+            else:
+                call(*args)
+            with torch.no_grad():
+                call(*args)
+            with torch.inference_mode():
+                call(*args)
+    out = torch.zeros_like(q, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        wb.gqa_attention(q, k, v, [0, 5], out=out)
+    with pytest.raises(ValueError, match="gradient"):
+        c.decode(0, q[:1], out=out[:1])

@@ -11,7 +11,8 @@ Tensors are torch CUDA tensors, bf16 or fp16, used in place on torch's
 current stream; q, k and v may be slices of a fused projection's rows (only
 the last dimension has to be contiguous).  Index arrays (``cu``, ``start``,
 ``slots``) are int32 CUDA tensors, which the host does not read, or host
-sequences, which are checked (not while a CUDA graph is captured).  The work runs in the CUDA library
+sequences, which are checked (not while a CUDA graph is captured).  Tensors that want a
+gradient are refused where autograd records.  The work runs in the CUDA library
 (``wb_gqa_*``, include/wave_b200.h); there is no CPU path.
 """
 from __future__ import annotations
@@ -78,6 +79,8 @@ def _rows(x, name: str, dtype=None):
     t = x.dtype
     if t not in _DTYPES or (dtype is not None and t is not dtype):
         raise ValueError(f"{name} must be bfloat16 or float16, as the others")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} wants a gradient, which these operators do not give: call them under torch.no_grad()")
     ts, hs, ds = x.stride()
     if ds != 1 and x.shape[2] > 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")
@@ -97,11 +100,10 @@ def _context(ctx, index: int) -> Context:
 
 
 def _out(out, q):
-    if out is None:
-        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    """Strides of a caller's output, checked."""
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError(f"out must be {tuple(q.shape)} {q.dtype} on {q.device}")
-    return out
+    return _rows(out, "out", q.dtype)
 
 
 def gqa_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float | None = None,
@@ -131,8 +133,7 @@ def gqa_attention(q, k, v, cu_q, cu_k=None, *, causal: bool = True, scale: float
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         o_ts, o_hs = H * hd, hd
     else:
-        out = _out(out, q)
-        o_ts, o_hs = _rows(out, "out", dtype)
+        o_ts, o_hs = _out(out, q)
     lse = q.new_empty((H, Tq), dtype=torch.float32) if return_lse else None
     ctx = _context(ctx, device)
     d = _ATTN.pack(_DTYPES[dtype], H, Hkv, hd, n_seq, bool(causal), hd ** -0.5 if scale is None else scale, Tq, Tk,
@@ -250,9 +251,12 @@ def gqa_decode(q, k_pages, v_pages, table, lens, *, slots=None, k_scale=None, v_
     if k_pages.get_device() != device:
         raise _elsewhere(device, k_pages.get_device())
     pl, keep_l = _index(slots, n_seq, "slots", device)
-    out = _out(out, q)
-    if not out.is_contiguous():
-        raise ValueError("out must be contiguous")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        _out(out, q)
+        if not out.is_contiguous():
+            raise ValueError("out must be contiguous")
     lse = q.new_empty((n_seq, H), dtype=torch.float32) if return_lse else None
     ctx = _context(ctx, device)
     _lib.call("wb_gqa_decode", ctx.handle, d, pl, n_seq, H, q.data_ptr(), q_ss, q_hs,
