@@ -65,7 +65,12 @@ def _index(a, n: int, name: str, device: int):
             raise _elsewhere(device, at)
         keep, size, ptr = a, shape[0], a.data_ptr()
     else:
-        keep = np.ascontiguousarray(a.numpy() if isinstance(a, torch.Tensor) else a, dtype=np.int32)
+        keep = np.asarray(a.numpy() if isinstance(a, torch.Tensor) else a)
+        if keep.ndim != 1 or (keep.size and keep.dtype.kind not in "iu"):
+            raise ValueError(f"{name} must be a vector of integers")
+        if keep.size and keep.dtype != np.int32 and not -2 ** 31 <= keep.min() <= keep.max() < 2 ** 31:
+            raise ValueError(f"{name} must be in int32's range")
+        keep = np.ascontiguousarray(keep, dtype=np.int32)
         size, ptr = keep.size, keep.ctypes.data
     if size != n:
         raise ValueError(f"{name} must have {n} entries, has {size}")
