@@ -561,3 +561,19 @@ def test_gradients_are_not_lost_silently():
         wb.gqa_attention(q, k, v, [0, 5], out=out)
     with pytest.raises(ValueError, match="gradient"):
         c.decode(0, q[:1], out=out[:1])
+
+
+def test_no_dimensions_are_refused():
+    import torch
+    import wave_engine_b200 as wb
+    q, _ = _rows(62, torch.bfloat16, 3, 4, 64)
+    k, v = _rows(63, torch.bfloat16, 3, 2, 64)
+    c = _cache(k, v, [3])
+    with pytest.raises(ValueError):
+        wb.gqa_attention(q[:, :, :0], k[:, :, :0], v[:, :, :0], [0, 3])
+    with pytest.raises(ValueError):
+        c.decode(0, q[:1, :, :0])
+    with pytest.raises(ValueError):
+        c.write(0, k[:, :, :0], v[:, :, :0], [0], [0, 3], [0])
+    with pytest.raises((ValueError, wb.WaveB200Error)):
+        wb.gqa_attention(q[:, :0], k, v, [0, 3])

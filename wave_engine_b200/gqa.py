@@ -87,8 +87,10 @@ def _rows(x, name: str, dtype=None):
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} wants a gradient, which these operators do not give: call them under torch.no_grad()")
     ts, hs, ds = x.stride()
-    if ds != 1 and x.shape[2] > 1:
+    if ds != 1 and x.shape[2] != 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")
+    if not x.shape[2]:
+        raise ValueError(f"{name} has a head_dim of 0")
     return ts, hs
 
 
