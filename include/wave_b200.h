@@ -520,7 +520,8 @@ WB_API int wb_gqa_cache_write(wb_context *ctx, const wb_gqa_cache_desc *c, const
 WB_API int wb_gqa_cache_read(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq,
                              const int32_t *cu, int64_t total, const int32_t *start, void *k, void *v);
 /* Attention of one new token per sequence over positions 0 .. lens-1 of its
- * slot (the token's own key and value among them: write it first).  q
+ * slot (the token's own key and value among them: write it first); up to
+ * 16777215 sequences.  q
  * element (sequence, head, d) at sequence*q_ss + head*q_hs + d; out [n_seq]
  * [n_head][head_dim] contiguous, lse NULL or [n_seq][n_head].  An empty slot,
  * or scores of -infinity alone, gives 0 and -inf; positions before the length whose page is unmapped are

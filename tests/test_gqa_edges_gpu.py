@@ -577,3 +577,14 @@ def test_no_dimensions_are_refused():
         c.write(0, k[:, :, :0], v[:, :, :0], [0], [0, 3], [0])
     with pytest.raises((ValueError, wb.WaveB200Error)):
         wb.gqa_attention(q[:, :0], k, v, [0, 3])
+
+
+def test_decode_of_too_many_sequences_is_refused():
+    import torch
+    import wave_engine_b200 as wb
+    n = 2 ** 24
+    pages = torch.zeros(1, 1, 128, 16, dtype=torch.bfloat16, device="cuda")
+    table, lens = (torch.zeros(*s, dtype=torch.int32, device="cuda") for s in ((n, 1), (n,)))
+    q = torch.zeros(n, 1, 1, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(wb.WaveB200Error, match="sequences"):
+        wb.gqa_decode(q, pages, pages, table, lens)

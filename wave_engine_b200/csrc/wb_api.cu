@@ -2255,6 +2255,7 @@ int wb_gqa_decode(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *sl
         if (!good_strides(q_ss, q_hs)) return fail(WB_EINVAL, "negative or huge stride");
         if (!std::isfinite(scale)) return fail(WB_EINVAL, "scale is not finite");
         if (n_seq == 0) return WB_OK;
+        if (n_seq > 0xffffff) return fail(WB_EINVAL, "more than 16777215 sequences");  // the kernel counts them in 24 bits
         if (!q || !out) return fail(WB_EINVAL, "NULL argument");
         DeviceGuard g(ctx->device);
         if (!g.ok) return fail(WB_ECUDA, "cudaSetDevice failed");
