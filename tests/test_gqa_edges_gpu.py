@@ -588,3 +588,38 @@ def test_decode_of_too_many_sequences_is_refused():
     q = torch.zeros(n, 1, 1, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(wb.WaveB200Error, match="sequences"):
         wb.gqa_decode(q, pages, pages, table, lens)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("H,Hkv,hd", [(2, 2, 64), (8, 1, 128), (3, 1, 42)])
+def test_infinite_queries(dtype, H, Hkv, hd):
+    """A query with an infinity: NaN where it sees a score of +infinity, 0 and -inf where all it sees is -infinity."""
+    import torch
+    import wave_engine_b200 as wb
+    dtype = getattr(torch, dtype)
+    n, T = 150, 400
+    k, v = _rows(64, dtype, T, Hkv, hd)
+    q = _rows(65, dtype, T, H, hd)[0]
+    k[:, :, 0] = -1.0
+    k[n, :, 0] = 1.0
+    clean, clean_lse = wb.gqa_attention(q, k, v, [0, T], return_lse=True)
+    hit = [0, 63, n - 1, n, n + 1, 256, T - 1]
+    q[hit, H - 1, 0] = float("inf")
+    out, lse = wb.gqa_attention(q, k, v, [0, T], return_lse=True)
+    for t in hit:
+        if t < n:
+            assert not out[t, H - 1].any() and lse[H - 1, t] == -float("inf")
+        else:
+            assert out[t, H - 1].isnan().all() and lse[H - 1, t].isnan()
+    other = torch.ones(T, H, dtype=torch.bool, device="cuda")
+    other[hit, H - 1] = False
+    assert torch.equal(out[other], clean[other]) and torch.equal(lse.T[other], clean_lse.T[other])
+    c = _cache(k, v, [T])
+    for held in (1, n, n + 1, T):
+        c.lens[0, 0] = held
+        out, lse = c.decode(0, q[-1:], return_lse=True)
+        if held <= n:
+            assert not out[0, H - 1].any() and lse[0, H - 1] == -float("inf")
+        else:
+            assert out[0, H - 1].isnan().all() and lse[0, H - 1].isnan()
+        assert torch.isfinite(out[0, :H - 1]).all()
