@@ -120,8 +120,8 @@ struct HeldBuf {
     int device;
     std::atomic<int> refs{1};
 };
-std::mutex g_held_mutex;
-std::vector<HeldBuf *> g_held;
+std::mutex &g_held_mutex = *new std::mutex;  // never destroyed: a context may end after statics do
+std::vector<HeldBuf *> &g_held = *new std::vector<HeldBuf *>;
 
 // Takes over p (freed when it fails).
 HeldBuf *buf_hold(void *p, size_t n, int device) {
