@@ -33,6 +33,7 @@ except Exception:  # pragma: no cover
     torch, _DTYPES, _STORES, _raw_stream = None, {}, {}, None
 
 PAGE = 128  # positions per page (WB_KV_PAGE)
+_INT32 = np.dtype(np.int32)
 
 
 # wb_gqa_attn_desc and wb_gqa_cache_desc (include/wave_b200.h) in C's layout
@@ -65,13 +66,14 @@ def _index(a, n: int, name: str, device: int):
             raise _elsewhere(device, at)
         keep, size, ptr = a, shape[0], a.data_ptr()
     else:
-        keep = np.asarray(a.numpy() if isinstance(a, torch.Tensor) else a)
-        if keep.ndim != 1 or (keep.size and keep.dtype.kind not in "iu"):
+        given = np.asarray(a.numpy() if isinstance(a, torch.Tensor) else a)
+        kind, size = given.dtype, given.size
+        if given.ndim != 1 or (size and kind.kind not in "iu"):
             raise ValueError(f"{name} must be a vector of integers")
-        if keep.size and keep.dtype != np.int32 and not -2 ** 31 <= keep.min() <= keep.max() < 2 ** 31:
+        keep = np.ascontiguousarray(given, dtype=np.int32)
+        if kind is not _INT32 and keep.astype(kind).tobytes() != given.tobytes():
             raise ValueError(f"{name} must be in int32's range")
-        keep = np.ascontiguousarray(keep, dtype=np.int32)
-        size, ptr = keep.size, keep.ctypes.data
+        ptr = keep.ctypes.data
     if size != n:
         raise ValueError(f"{name} must have {n} entries, has {size}")
     return ptr, keep
