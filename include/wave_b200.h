@@ -524,8 +524,11 @@ WB_API int wb_gqa_cache_read(wb_context *ctx, const wb_gqa_cache_desc *c, const 
  * 16777215 sequences.  q
  * element (sequence, head, d) at sequence*q_ss + head*q_hs + d; out [n_seq]
  * [n_head][head_dim] contiguous, lse NULL or [n_seq][n_head].  An empty slot,
- * or scores of -infinity alone, gives 0 and -inf; positions before the length whose page is unmapped are
- * left out and flagged. */
+ * or scores of -infinity alone, gives 0 and -inf; positions before the length
+ * whose page is unmapped are left out and flagged.  Weights are rounded as in
+ * wb_gqa_attention, over bf16 values to twice as many bits; bf16 queries meet
+ * 8-bit keys in fp16, relative to their head's largest (dimensions below
+ * 2^-17 of it lose bits, below 2^-25 they are 0). */
 WB_API int wb_gqa_decode(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq, int n_head,
                          const void *q, int64_t q_ss, int64_t q_hs, float scale, void *out, float *lse);
 

@@ -14,10 +14,11 @@
 // reading, four rows a thread under way at once.  The rows of a
 // block are loaded before their places in the cache are looked up (sequence,
 // slot, start, page: dependent loads that take as long as the data).
-// 8 x 4096 positions of 8 heads x 128, fp16 to e4m3 and back: 43.6 + 35.2 us
-// apart, 74 us in a row (203 MB each way, 5.5 TB/s of 6.5; below it stays what
-// a warp has to do a row: the maximum over its lanes, the quotients).  One
-// position of 32 sequences: 7.0 us for both, launches and the dependent loads.
+// 8 x 4096 positions of 8 heads x 128, fp16 to e4m3 and back: 43.4 + 35.1 us
+// apart, 75 us in a row (203 MB each way, 5.4 TB/s of 6.5; below it stays what
+// a warp has to do a row: the maximum over its lanes, the quotients); as they
+// are 48.5 + 44.2 us apart, 93 in a row (5.8 TB/s).  One
+// position of 32 sequences: 7.2 us for both, launches and the dependent loads.
 #include "wb_gqa.h"
 
 #include <algorithm>
@@ -36,7 +37,7 @@ struct GqaMove {
 };
 
 static constexpr int GM_THREADS = 128, GM_ROWS = 4;  // rows of a thread
-static constexpr int GM_CTAS = 8;  // write blocks per SM (256 threads and 4 blocks: 76 us instead of 74, 64 and 16: 82)
+static constexpr int GM_CTAS = 8;  // write blocks per SM (256 threads and 4 blocks: 77 us instead of 75, 64 and 16: 82)
 
 // Row `local` of a block (counted from its first token's first head): token
 // and head.  inv = 2^32 / Hkv rounded up, so the quotient is right or one

@@ -10,11 +10,12 @@
 // and end inside an item, and the last CTA to finish an item joins its
 // pieces in the order of the keys (same bits every run).
 //
-// One sequence of 131072 positions, 32 heads on 8, head_dim 128, fp16: 88 us,
-// 6.1 TB/s, 94% of the measured copy bandwidth; 256 sequences of 128 to 4096,
-// int8: 189 us, 6.1 TB/s.  Few keys are bound by latencies (launch, lengths and
-// the line 2.5 us, first keys, joins): 32 sequences near 1150, 12 heads on 4,
-// head_dim 64, e4m3, 13.8 us; one of 257, 7.4 us.  Shares are equal but
+// One sequence of 131072 positions, 32 heads on 8, head_dim 128, fp16: 89 us,
+// 6.0 TB/s, 93% of the measured copy bandwidth (bf16, two products with the
+// values: 91 us); 256 sequences of 128 to 4096: int8 189 us, e4m3 192 us, 6.0
+// TB/s, bf16 340 us, 6.5 TB/s.  Few keys are bound by latencies (launch,
+// lengths and the line 2.5 us, first keys, joins): 32 sequences near 1150, 12
+// heads on 4, head_dim 64, e4m3, 14.1 us; one of 257, 7.4 us.  Shares are equal but
 // SMs are not equally fast (with 256 sequences they end between 150 and 200
 // us); shares cut into six chunks, the later ones dealt out by tickets, all
 // ended within 15 us of each other, but 30 us later: a part's start and end
@@ -282,10 +283,13 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
     const long long units = (total >> 24) * ips, items = (total & 0xffffff) * ips;
     // Few units for the CTAs there are: every item in equal pieces of P
     // units, one for each CTA (a piece that ends with its item has one join
-    // less; 32 sequences near 1150, 12 heads on 4: 13.9 us, 15.3 in equal
-    // shares).  Else positions of one unit, with W more for an item's start and
-    // end, in equal shares (256 sequences of 128 to 4096: 190 us, 206 without
-    // W).
+    // less; 32 sequences, 12 heads on 4, at 4 units a CTA 13.9 us, 15.4 in
+    // equal shares; at 8 units 18.3, 20.6; at 15 units 25.2, 24.6).  P is at
+    // least 6: a shorter piece saves less than its join costs (one sequence of
+    // 257: 7.5 us, 8.7 with 3, 7.6 with 12; 4 near 1150: 11.5, 10.3, 14.1; 32:
+    // 14.1, 14.1, 17.3).  Else positions of one unit, with W more for an
+    // item's start and end, in equal shares (256 sequences of 128 to 4096: 189
+    // us, 204 without W).
     int P = 1, W = GD_ITEM;
     if (2 * items <= gridDim.x && units <= (long long)gridDim.x * GD_FEW) {
         W = 0;
@@ -484,8 +488,8 @@ __global__ void __launch_bounds__(GD_THREADS, GdConf<KIND, HDP, NB>::CTAS) gqa_d
             float f = a.scale * 1.4426950408889634f;
             if (QUANT && !__is_same(T, __half)) {
                 // bf16 queries meet fp16 keys: divided by a power of two so
-                // that the head's largest is in [1, 2) (exact down to 2^-14
-                // of it)
+                // that the head's largest is in [1, 2) (exact down to 2^-17
+                // of it, 0 below 2^-25)
                 uint32_t top = 0;
 #pragma unroll
                 for (int t = 0; t < NK; t++)
@@ -928,7 +932,9 @@ static int gd_launch_as(const GqaDecodeArgs &a, int sm_count, cudaStream_t st, s
 template <class T, int KIND, int HDP>
 static int gd_launch(const GqaDecodeArgs &a, int sm_count, cudaStream_t st, std::string *msg) {
     // up to 8 heads on a key-value head: one product's 8 columns; more: two
-    // (two for 4 heads: 242 us instead of 190, 256 sequences of int8)
+    // (256 sequences of int8: two for 4 heads 234 us instead of 190, for 8
+    // heads 241 instead of 195; 9 heads as two items of one each 372 instead
+    // of 246, 16 heads 379 instead of 259)
     const bool full = a.c.row == HDP;
     if (a.H / a.c.Hkv <= 8)
         return full ? gd_launch_as<T, KIND, HDP, 1, true>(a, sm_count, st, msg)
@@ -943,7 +949,7 @@ int launch_gqa_decode(const GqaCacheArgs &c, int dtype, int H, const void *q, lo
     GqaDecodeArgs a{c, q, out, lse, q_ss, q_hs, H, scale, counters, (float *)scratch};
     auto by_store = [&](auto t) {
         using T = decltype(t);
-        // rows of up to 64 in 64 columns (in 128: 17.5 us instead of 13.8, 32
+        // rows of up to 64 in 64 columns (in 128: 17.8 us instead of 14.1, 32
         // sequences near 1150)
         const bool wide = c.hd > 64;
         if (c.store == WB_INT8)
