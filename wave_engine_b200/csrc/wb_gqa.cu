@@ -29,13 +29,13 @@
 // cycles for the maximum, 1350 to 1700 for the exponentials (the other tile's
 // among them), then 700 (400) to issue and run P V and the next Q K^T and 350
 // until the scores are seen.  One sequence of 8192 tokens, 32 heads on 8,
-// head_dim 128, causal: 440 us, 1250 TFLOP/s, 75% of the measured cuBLAS
-// burst rate, in bursts of a few calls; call after call for seconds 509 us at
-// 1640 of 1965 MHz, 1080 TFLOP/s, 76% of the sustained rate: there the chip is
+// head_dim 128, causal: 437 us, 1258 TFLOP/s, 75% of the measured cuBLAS
+// burst rate, in bursts of a few calls; call after call for seconds 509 to 520
+// us at 1590 to 1640 of 1965 MHz, 75% of the sustained rate: there the chip is
 // at its power limit (with the two tiles half a period apart a pair takes
 // 3310 cycles at a clock 4% lower: the same time).
 // Short sequences pay the start and end of an item, about 4000 cycles: 32
-// sequences of 1 to 1024 tokens, 12 heads on 4, head_dim 64: 61.5 us.
+// sequences of 1 to 1024 tokens, 12 heads on 4, head_dim 64: 61.3 us.
 //
 // Measured and not kept: exponentials by a polynomial on the FMA pipe (a
 // quarter of them cost 4% at 8192 tokens, three eighths 7%); eight softmax
@@ -176,10 +176,10 @@ __device__ __forceinline__ int ga_items(const GqaAttnArgs &a, int b, int per_ite
 // 64 sequences: tiles late in their sequences (with the most keys) first --
 // the largest t with more than `index` items at or behind place t, then by
 // sequence -- so that long items are dealt out first (8 sequences up to 4096:
-// 136 us, 164 in the sequences' order; 32 up to 1024: 61.5, 68; 64 up to 600:
-// 63, 66).  More: in the order of the sequences, one pass over them for all
-// items of the CTA (65 up to 600: 66 us, 65 with the longest first; 255 up to
-// 400: 127 us, 140).
+// 135 us, 164 in the sequences' order; 32 up to 1024: 61.3, 68; 64 up to 600:
+// 62, 66).  More: in the order of the sequences, one pass over them for all
+// items of the CTA (65 up to 600: 65 us both ways; 255 up to 400: 125 us, 140
+// with the longest first).
 struct GaFinder {
     static constexpr int N = 2;
     int n[N];                // items of sequences lane + 32 x (or of sequences b0 + lane, in n[0])
@@ -913,8 +913,8 @@ int launch_gqa_attention(const GqaAttnArgs &args, int dtype, void *scratch, int 
         ProfScope ps("gqa_rows", st);
         gqa_rows_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(js);
     }
-    // rows of up to 64 in 64 columns (in 128: 71.5 us instead of 61.5, packed
-    // 768-wide batch; 26.4 instead of 21.7, 16 x 512 tokens of 48)
+    // rows of up to 64 in 64 columns (in 128: 71.5 us instead of 61.3, packed
+    // 768-wide batch; 26.4 instead of 21.2, 16 x 512 tokens of 48)
     if (dtype == WB_BF16)
         return a.hd <= 64 ? ga_launch<__nv_bfloat16, 64>(ga, sm_count, st, msg) : ga_launch<__nv_bfloat16, 128>(ga, sm_count, st, msg);
     return a.hd <= 64 ? ga_launch<__half, 64>(ga, sm_count, st, msg) : ga_launch<__half, 128>(ga, sm_count, st, msg);
