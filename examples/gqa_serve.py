@@ -81,9 +81,10 @@ def serve(store="e4m3", prompts=(5, 300, 1, 129), chunk=70, steps=16, n_layers=2
         keys, values = cache.read(layer, slots=slots, cu=cu_k, total=sum(held))
         return wb.gqa_attention(q, keys, values, cu_q, cu_k)
 
-    y = model.forward(torch.cat([x[i][prompts[i]:prompts[i] + more[i]] for i in slots]), continued)
-    for i, part in zip(slots, y.split([more[i] for i in slots])):
-        done[i].append(part)
+    if slots:
+        y = model.forward(torch.cat([x[i][prompts[i]:prompts[i] + more[i]] for i in slots]), continued)
+        for i, part in zip(slots, y.split([more[i] for i in slots])):
+            done[i].append(part)
 
     # one token each per step: the whole step is one CUDA graph (lengths and
     # the table stay on the device)

@@ -623,3 +623,14 @@ def test_infinite_queries(dtype, H, Hkv, hd):
         else:
             assert out[0, H - 1].isnan().all() and lse[0, H - 1].isnan()
         assert torch.isfinite(out[0, :H - 1]).all()
+
+
+@pytest.mark.parametrize("sizes", [dict(prompts=(5,)), dict(prompts=(130, 7), chunk=0), dict(prompts=(3, 4), steps=0)])
+def test_example_without_a_chunk(sizes):
+    """examples/gqa_serve.py with one sequence, no continued chunk, no steps."""
+    import torch
+    from tests.test_gqa_example_gpu import _example
+    got, whole, _ = _example().serve("native", **sizes)
+    for u, w in zip(got, whole):
+        assert u.shape == w.shape and (u.float() - w.float()).pow(2).mean(1).sqrt().max().item() <= 2 * 2.0 ** -6
+    assert torch.cuda.current_stream() == torch.cuda.default_stream()
