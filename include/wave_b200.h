@@ -518,14 +518,15 @@ WB_API int wb_gqa_cache_write(wb_context *ctx, const wb_gqa_cache_desc *c, const
                               int64_t k_hs, const void *v, int64_t v_ts, int64_t v_hs);
 /* Read positions back, in the layout of the write: k, v [total][n_kv_head]
  * [head_dim] contiguous, of dtype (an 8-bit row as value * scale, rounded
- * once).  start NULL: from position 0; a slot at most once.  Positions outside the table's pages
- * read 0. */
+ * once).  start NULL: from position 0; a slot at most once.  Positions outside
+ * the table's pages read 0. */
 WB_API int wb_gqa_cache_read(wb_context *ctx, const wb_gqa_cache_desc *c, const int32_t *slots, int n_seq,
                              const int32_t *cu, int64_t total, const int32_t *start, void *k, void *v);
 /* Attention of one new token per sequence over positions 0 .. lens-1 of its
  * slot (the token's own key and value among them: write it first); up to
- * 16777215 sequences, a slot at most once.  q element (sequence, head, d) at sequence*q_ss + head*q_hs + d; out [n_seq]
- * [n_head][head_dim] contiguous, lse NULL or [n_seq][n_head].  An empty slot,
+ * 16777215 sequences, a slot at most once.  q element (sequence, head, d) at
+ * sequence*q_ss + head*q_hs + d; out [n_seq][n_head][head_dim] contiguous,
+ * lse NULL or [n_seq][n_head].  An empty slot,
  * or scores of -infinity alone, gives 0 and -inf; positions before the length
  * whose page is unmapped are left out and flagged.  Weights are rounded as in
  * wb_gqa_attention, over bf16 values to twice as many bits; bf16 queries meet
